@@ -23,10 +23,12 @@ OUT_DIR = CSRC.parent / "gpu" / "nf4"
 LIB = OUT_DIR / "libchr_nf4.so"
 OBJ_DIR = CSRC / "build"
 
-CUDA_SOURCES = ("gemv.cu", "decode_ops.cu", "prefill_ops.cu", "prefill_attn.cu", "gemm.cu", "gemm_tc.cu", "codec_dev.cu",
+CUDA_SOURCES = ("gemv.cu", "decode_ops.cu", "prefill_ops.cu", "prefill_attn.cu", "paged_append.cu", "paged_attn.cu",
+                "sample.cu", "gemm.cu", "gemm_tc.cu", "codec_dev.cu",
                 "version.cu")
 CXX_SOURCES = ("codec.cpp",)
-HEADERS = ("nf4_common.cuh", "gemv_ring.cuh", "gemv_cols.cuh", "gemv_n.cuh", "attn_core.cuh", "attn_mma.cuh", "gemm_plan.h")
+HEADERS = ("nf4_common.cuh", "gemv_ring.cuh", "gemv_cols.cuh", "gemv_n.cuh", "attn_core.cuh", "attn_mma.cuh", "paged.cuh",
+           "gemm_plan.h")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -19,13 +19,18 @@ import torch
 
 from . import _lib
 from ._lib import ChrNf4Dev, ChrNf4Plan
+from .paged import (PAGED_HEAD_DIMS, SAMPLE_MAX_VOCAB, nf4_attn_paged, nf4_rope_kv_paged,
+                    nf4_sample_commit_batch)
 from .plan import LIVE_MAX_N, PLAN_MAX_N, k_pad as _k_pad
 
 __all__ = [
     "ATTN_SPLIT",
     "LIVE_MAX_N",
+    "PAGED_HEAD_DIMS",
     "PLAN_MAX_N",
+    "SAMPLE_MAX_VOCAB",
     "nf4_attn",
+    "nf4_attn_paged",
     "nf4_embed_rows",
     "nf4_gemm",
     "nf4_gemm_rows",
@@ -42,7 +47,9 @@ __all__ = [
     "nf4_qkv",
     "nf4_rms",
     "nf4_rms_rows",
+    "nf4_rope_kv_paged",
     "nf4_rope_kv_rows",
+    "nf4_sample_commit_batch",
     "nf4_silu_mul",
     "nf4_attn_prefill",
     "nf4_pick_commit_batch",

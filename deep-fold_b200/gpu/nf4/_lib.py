@@ -58,7 +58,17 @@ class ChrNf4Peers(Structure):
                 ("flags", c_void_p * AR_MAX_RANKS), ("epoch", c_void_p), ("status", c_void_p)]
 
 
+class ChrNf4Pages(Structure):
+    """Mirror of ``chr_nf4_pages_t``."""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("table", c_void_p), ("k_page_stride", c_int64),
+                ("v_page_stride", c_int64), ("table_stride", c_int64), ("n_pages", c_int32),
+                ("page", c_int32), ("n_kv", c_int32), ("hd", c_int32), ("batch", c_int32),
+                ("max_pages", c_int32)]
+
+
 _DEV = POINTER(ChrNf4Dev)
+_PAGES = POINTER(ChrNf4Pages)
 
 # name -> (restype, argtypes); every symbol include/chr_gpu.h declares.
 SIGNATURES = {
@@ -151,6 +161,23 @@ SIGNATURES = {
         c_int,
         [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
          c_int32, c_float, c_void_p],
+    ),
+    "chr_nf4_rope_kv_paged": (
+        c_int,
+        [_PAGES, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+         c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_int32,
+         c_int32, c_int32, c_void_p],
+    ),
+    "chr_nf4_attn_paged_ws": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "chr_nf4_attn_paged": (
+        c_int,
+        [_PAGES, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,
+         c_float, c_void_p, c_int64, c_int32, c_void_p],
+    ),
+    "chr_nf4_sample_commit_batch": (
+        c_int,
+        [c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
     ),
     "chr_nf4_silu_mul": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
     "chr_nf4_encode_f32": (c_int, [c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_int32]),

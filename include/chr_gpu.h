@@ -389,6 +389,90 @@ int chr_nf4_rope_kv_rows(const void *q, int64_t q_stride, const void *k, int64_t
  * the activation on the output of the stacked gate/up GEMM (bf16 [N, 2*I]). */
 int chr_nf4_silu_mul(const void *gate_up, void *out, int32_t N, int32_t I, void *stream);
 
+/* ---- Paged KV cache --------------------------------------------------------
+ * The cache of many sequences as pages of rows in one pool per layer (additive; the
+ * reference reserves one [max_seq, n_kv, hd] block, gpu/decodev2/kv.py:14-120). */
+
+/* k, v: bf16 pools [n_pages, page, n_kv, hd]; the pages of a pool lie k_page_stride /
+ * v_page_stride elements apart, each page is contiguous. Cache row a of sequence s is row
+ * a % page of page table[s * table_stride + a / page]. page: a power of two, 16..65536.
+ * Page ids may repeat between sequences (shared prefixes); an id outside [0, n_pages)
+ * is no page: rows on it are neither written nor attended. */
+typedef struct {
+  void *k, *v;
+  const int32_t *table;   /* device int32 [batch, max_pages] */
+  int64_t k_page_stride, v_page_stride, table_stride;
+  int32_t n_pages, page, n_kv, hd, batch, max_pages;
+} chr_nf4_pages_t;
+
+/* Rotary positions for T rows and the append of their k and v to the cache, in one launch.
+ * Row t belongs to sequence seq[t] (device int32; NULL: sequence t), takes its cache row
+ * slot[t] (device int64) and is rotated for position[t] (device int64; NULL: slot[t]).
+ * q [T, n_q, hd], k and v [T, n_kv, hd]: bf16, rows *_stride elements apart; q rotated goes
+ * to q_out (bf16, rows q_out_stride apart; may be q itself); n_q = 0 leaves q out.
+ * cos, sin: [tab_rows, rot / 2], FP32 (tab_f32 != 0) or bf16, rows tab_stride apart; the
+ * first rot elements of a head are rotated, the rest pass through. interleaved = 0 pairs
+ * element i with i + rot / 2, else 2i with 2i + 1. FP32 products and sum, one rounding.
+ * A row whose sequence, slot, position or page lies outside is skipped: it writes no cache
+ * row, and its q_out row is left alone (zero_skipped = 0) or zeroed. Two rows of one call
+ * must not take the same cache row, and no row a page that another sequence shares.
+ * Returns 0, -1 (null), -3 (dims), -6 (launch). Capturable. */
+int chr_nf4_rope_kv_paged(const chr_nf4_pages_t *pages, const void *q, int64_t q_stride,
+                          const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                          void *q_out, int64_t q_out_stride, const void *cos, const void *sin,
+                          int64_t tab_stride, int32_t tab_rows, int32_t tab_f32, int32_t rot,
+                          int32_t interleaved, const void *seq, const void *slot,
+                          const void *position, int32_t T, int32_t n_q, int32_t zero_skipped,
+                          void *stream);
+
+/* Attention of T new rows over the paged cache. Sequence b owns rows q_start[b] ..
+ * q_start[b+1]-1 of q (device int32 [batch + 1], not decreasing, within 0..T; NULL: T ==
+ * batch, row b is sequence b's) and kv_len[b] cache rows (device int32), its n_b new rows
+ * the last n_b of them. New row i sees cache row t < base = kv_len[b] - n_b, and of the new
+ * rows those with t - base <= i, or, with tree given, those whose bit t - base is set in
+ * the tree_words 64-bit words of the row's mask (device uint64 [T, tree_words]; a bit past
+ * the words is clear). GQA: n_q a multiple of n_kv, hd in {16, 32, 64, 128}.
+ *   out[i, h, :] = softmax_t( scale * q[i, h, :] . k[t, h / n_rep] ) . v[t, h / n_rep]
+ * q: bf16, rows q_stride elements apart (a multiple of 8), rotated already; out: bf16
+ * [T, n_q * hd] contiguous. A row that sees nothing gives zeros; rows behind the last
+ * sequence's are left alone (zero_tail = 0) or zeroed. FP32 scores, running softmax and
+ * accumulation; probabilities are rounded to bf16 for the value product. Cache rows at
+ * kv_len and beyond may hold anything; the new rows' own v must be finite, since a
+ * masked one enters the product with weight zero.
+ * ws: chr_nf4_attn_paged_ws(...) floats, no initial contents needed; two calls that may
+ * overlap on the device need one each. Two launches. Capturable: lengths, tables and
+ * masks are read on the device, and a replay follows what they hold then.
+ * Returns 0, -1 (null), -3 (dims), -5 (alignment: q, out, pools 16 bytes), -6, -7. */
+int64_t chr_nf4_attn_paged_ws(int32_t T, int32_t batch, int32_t n_q, int32_t n_kv, int32_t hd);
+int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, int64_t q_stride, void *out,
+                       const void *q_start, const void *kv_len, const void *tree,
+                       int32_t tree_words, int32_t T, int32_t n_q, float scale, float *ws,
+                       int64_t ws_floats, int32_t zero_tail, void *stream);
+
+/* ---- Sampled pick ----------------------------------------------------------
+ * One token per row drawn from its logits with the row's own settings and its own given
+ * random number, then the commit of chr_nf4_pick_commit_batch (additive; the reference
+ * picks the argmax, gpu/decodev2/step.py:182).
+ * logits: bf16 [batch, n], rows row_stride elements apart, n <= 524280. With x a row, m
+ * its maximum and w_i = exp((x_i - m) / temperature), tokens in the order "x descending,
+ * index ascending" and cum the running sum of w in that order:
+ *   top_k   > 0: the first top_k tokens stay (else all);
+ *   top_p   < 1: of those, the tokens before which cum < top_p * (their sum) stay;
+ *   min_p   > 0: of those, the tokens with w >= min_p stay; the first always stays.
+ * What stays is the first n' tokens; the pick is the first one with cum > u * cum(n').
+ * Arithmetic in 64 bits. u: device float32 [batch] in [0, 1) (outside: the nearest).
+ * temperature, top_p, min_p: device float32 [batch], top_k: device int32 [batch], each
+ * optional (1, 1, 0, 0). prob: optional device float32 [batch], w of the pick / cum(n').
+ * A temperature <= 0 or NaN, or a row whose maximum is not finite, picks greedily as
+ * chr_nf4_pick_commit does (lowest index of the maximum, NaN above everything), prob 1.
+ * next_token etc. as in chr_nf4_pick_commit_batch. No scratch, one launch, capturable.
+ * Returns 0, -1 (null), -3 (dims), -6 (launch). */
+int chr_nf4_sample_commit_batch(const void *logits, int64_t row_stride, int32_t n, int32_t batch,
+                                const void *u, const void *temperature, const void *top_k,
+                                const void *top_p, const void *min_p, void *prob,
+                                void *next_token, void *token, void *position, void *finished,
+                                int64_t eos, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

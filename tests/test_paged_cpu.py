@@ -1,0 +1,134 @@
+"""Refusals of the paged-cache ops and the sampled pick that need no GPU: the C entries check
+their arguments before any CUDA call, and the Python ops before any entry."""
+
+from __future__ import annotations
+
+import ctypes
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+ROOT = Path(__file__).resolve().parents[1]
+P = ctypes.c_void_p(4096)  # a non-null address that no entry reads on the host
+
+
+def _pages(**kw):
+    from gpu.nf4._lib import ChrNf4Pages
+
+    d = dict(k=4096, v=4096, table=4096, k_page_stride=16 * 2 * 64, v_page_stride=16 * 2 * 64, table_stride=4, n_pages=8,
+             page=16, n_kv=2, hd=64, batch=2, max_pages=4)
+    d.update(kw)
+    return ChrNf4Pages(**d)
+
+
+def _append(pages=None, **kw):
+    from gpu.nf4 import _lib
+
+    d = dict(q=P, qs=512, k=P, ks=128, v=P, vs=128, qo=P, qos=512, cos=P, sin=P, ts=32, rows=64, f32=1, rot=64, inter=0,
+             seq=P, slot=P, pos=None, T=3, n_q=8, zero=0)
+    d.update(kw)
+    return _lib.load().chr_nf4_rope_kv_paged(_pages() if pages is None else pages, *d.values(), None)
+
+
+def _attn(pages=None, **kw):
+    from gpu.nf4 import _lib
+
+    d = dict(q=P, qs=512, out=P, q_start=P, kv=P, tree=None, words=0, T=3, n_q=8, scale=0.1, ws=P, floats=1 << 30, zero=0)
+    d.update(kw)
+    return _lib.load().chr_nf4_attn_paged(_pages() if pages is None else pages, *d.values(), None)
+
+
+def _sample(**kw):
+    from gpu.nf4 import _lib
+
+    d = dict(logits=P, rs=100, n=100, batch=2, u=P, t=None, k=None, p=None, m=None, prob=None, nxt=P, tok=None, pos=None,
+             fin=None, eos=-1)
+    d.update(kw)
+    return _lib.load().chr_nf4_sample_commit_batch(*d.values(), None)
+
+
+@pytest.mark.parametrize("bad", [dict(page=8), dict(page=24), dict(page=1 << 17), dict(n_pages=0), dict(n_kv=0), dict(hd=63),
+                                 dict(batch=0), dict(max_pages=0), dict(table_stride=3), dict(k_page_stride=100),
+                                 dict(v_page_stride=2047), dict(max_pages=1 << 28, table_stride=1 << 28)])
+def test_a_cache_that_is_none_is_refused(bad):
+    assert _append(_pages(**bad)) == -3 and _attn(_pages(**bad)) == -3
+
+
+@pytest.mark.parametrize("null", ["k", "v", "table"])
+def test_null_pools_are_refused(null):
+    assert _append(_pages(**{null: None})) == -1 and _attn(_pages(**{null: None})) == -1
+
+
+@pytest.mark.parametrize("kw,rc", [(dict(k=None), -1), (dict(v=None), -1), (dict(q=None), -1), (dict(qo=None), -1),
+                                   (dict(cos=None), -1), (dict(sin=None), -1), (dict(slot=None), -1), (dict(T=0), -3),
+                                   (dict(n_q=-1), -3), (dict(rot=0), -3), (dict(rot=3), -3), (dict(rot=66), -3),
+                                   (dict(ts=31), -3), (dict(rows=0), -3), (dict(qs=511), -3), (dict(ks=127), -3),
+                                   (dict(vs=127), -3), (dict(qos=511), -3), (dict(seq=None), -3)])
+def test_append_refusals(kw, rc):
+    assert _append(**kw) == rc
+
+
+@pytest.mark.parametrize("kw,rc", [(dict(q=None), -1), (dict(out=None), -1), (dict(kv=None), -1), (dict(ws=None), -1),
+                                   (dict(T=0), -3), (dict(n_q=0), -3), (dict(n_q=7), -3), (dict(qs=511), -3),
+                                   (dict(tree=P), -3), (dict(q_start=None), -3), (dict(T=1 << 30), -3),
+                                   (dict(q=ctypes.c_void_p(4098)), -5), (dict(out=ctypes.c_void_p(4104)), -5),
+                                   (dict(qs=516), -5), (dict(tree=ctypes.c_void_p(4100), words=1), -5), (dict(floats=0), -7)])
+def test_attention_refusals(kw, rc):
+    assert _attn(**kw) == rc
+
+
+@pytest.mark.parametrize("hd", [8, 24, 48, 96, 256])
+def test_attention_refuses_other_head_dims(hd):
+    assert _attn(_pages(hd=hd, k_page_stride=1 << 16, v_page_stride=1 << 16), qs=1 << 14) == -3
+
+
+def test_attention_refuses_unaligned_pools():
+    assert _attn(_pages(k=4098)) == -5 and _attn(_pages(v=4104)) == -5
+    assert _attn(_pages(k_page_stride=16 * 2 * 64 + 4)) == -5
+
+
+def test_workspace_query_answers_zero_for_what_the_call_refuses():
+    from gpu.nf4 import _lib
+
+    ws = _lib.load().chr_nf4_attn_paged_ws
+    assert ws(3, 2, 8, 2, 64) > 0
+    for bad in ((0, 2, 8, 2, 64), (3, 0, 8, 2, 64), (3, 2, 7, 2, 64), (3, 2, 8, 0, 64), (3, 2, 8, 2, 48)):
+        assert ws(*bad) == 0
+
+
+@pytest.mark.parametrize("kw,rc", [(dict(logits=None), -1), (dict(u=None), -1), (dict(nxt=None), -1), (dict(n=0), -3),
+                                   (dict(n=524281, rs=524281), -3), (dict(batch=0), -3), (dict(batch=65536), -3),
+                                   (dict(rs=99), -3)])
+def test_sample_refusals(kw, rc):
+    assert _sample(**kw) == rc
+
+
+def test_python_ops_refuse_cpu_tensors():
+    from gpu.nf4 import nf4_attn_paged, nf4_rope_kv_paged, nf4_sample_commit_batch
+
+    pool = torch.zeros((4, 16, 2, 64), dtype=torch.bfloat16)
+    table = torch.zeros((2, 2), dtype=torch.int32)
+    rows = torch.zeros((2, 2, 64), dtype=torch.bfloat16)
+    tab = torch.zeros((32, 32))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        nf4_rope_kv_paged(rows, rows, rows, pool, pool, table, tab, tab, torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        nf4_attn_paged(rows, pool, pool, table, torch.zeros(2, dtype=torch.int32), 1.0)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        nf4_sample_commit_batch(torch.zeros((2, 8), dtype=torch.bfloat16), torch.zeros(2), torch.zeros(2, dtype=torch.int64))
+
+
+def test_pages_struct_matches_the_header(tmp_path):
+    from gpu.nf4._lib import ChrNf4Pages
+
+    src = tmp_path / "sz.c"
+    fields = [f[0] for f in ChrNf4Pages._fields_]
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "chr_gpu.h"\nint main(void) { printf("%zu", '
+                   "sizeof(chr_nf4_pages_t));\n"
+                   + "".join(f'printf(" %zu", offsetof(chr_nf4_pages_t, {f}));\n' for f in fields) + "return 0; }\n")
+    exe = tmp_path / "sz"
+    subprocess.run(["gcc", f"-I{ROOT / 'include'}", str(src), "-o", str(exe)], check=True)
+    got = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [ctypes.sizeof(ChrNf4Pages)] + [getattr(ChrNf4Pages, f).offset for f in fields]
