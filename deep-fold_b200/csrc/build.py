@@ -28,6 +28,7 @@ CUDA_SOURCES = ("gemv.cu", "decode_ops.cu", "prefill_ops.cu", "prefill_attn.cu",
                 "version.cu")
 CXX_SOURCES = ("codec.cpp",)
 HEADERS = ("nf4_common.cuh", "gemv_ring.cuh", "gemv_cols.cuh", "gemv_n.cuh", "attn_core.cuh", "attn_mma.cuh", "paged.cuh",
+           "paged_attn_wide.cuh", "tma_tc.cuh",
            "gemm_plan.h")
 
 NVCC_FLAGS = [

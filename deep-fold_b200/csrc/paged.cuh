@@ -51,16 +51,17 @@ inline int paged_cache(const chr_nf4_pages_t *p, PagedCache &c) {
 // the order (sequence, kv head, item), lie on one axis with a length that is what they
 // cost, and CTA c of G takes the piece [total c / G, total (c+1) / G) of it: every CTA
 // has the same amount of cache to read whatever the lengths, and the host needs to know
-// none of them. A piece border inside an item falls on the tile border next to it;
-// items cut by borders leave FP32 partials (at most two per CTA: its first and its last
-// item) that a second kernel joins, deriving the same split.
-// The length of an item is its cache rows times n_rep, the causal part counted exactly
-// up to rounding: base n_rep + (rows up to its last), so that the axis has a closed form.
+// none of them. A piece border inside an item falls on the tile border next to it; an
+// item that a border cuts is left as FP32 partials (at most two per CTA: of its first
+// and of its last item) that a second kernel joins.
+// The length of an item is its cache rows plus `extra` (what starting and ending it costs,
+// in rows), times n_rep; the causal part is counted exactly up to rounding - base n_rep
+// plus the rows up to its last - so that the axis has a closed form.
 struct PagedRows {
   const int32_t *q_start;  // [batch + 1], or null: row b is sequence b's only one
   const int32_t *kv_len;   // [batch]
   int T, batch, n_kv, n_rep, cap;
-  int M, tile;             // rows of an item, cache rows of a tile
+  int M, tile, extra;      // rows of an item, cache rows of a tile, an item's own cost
   int causal;
 };
 
@@ -92,9 +93,9 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedRows &p, int b) {
 
 // Length of items 0 .. j-1, and of item j.
 __device__ __forceinline__ long long paged_before(const PagedRows &p, const PagedSeq &s, int j) {
-  if (!s.stairs) return static_cast<long long>(j) * max(static_cast<long long>(s.len) * p.n_rep, 1ll);
   const long long jj = j;
-  long long v = jj * s.base * p.n_rep + jj * (jj + 1) / 2 * p.M;
+  if (!s.stairs) return jj * (static_cast<long long>(s.len) + p.extra) * p.n_rep;
+  long long v = jj * (static_cast<long long>(s.base) + p.extra) * p.n_rep + jj * (jj + 1) / 2 * p.M;
   if (j >= s.J) v -= jj * p.M - s.R;  // the last item is not full
   return v;
 }
@@ -112,54 +113,74 @@ __device__ __forceinline__ int paged_kv_end(const PagedRows &p, const PagedSeq &
   return max(s.base + last + 1, 0);
 }
 
-struct PagedAt {
-  int b, kvh, j;
-  long long start;  // the item's place on the axis
-};
-
-// The item that holds position x of the axis, given its sequence and that one's start.
-__device__ __forceinline__ PagedAt paged_item_at(const PagedRows &p, const PagedSeq &s, int b,
-                                                 long long b_start, long long x) {
-  PagedAt at;
-  at.b = b;
-  const long long one = paged_before(p, s, s.J);
-  const long long rem0 = x - b_start;
-  at.kvh = static_cast<int>(rem0 / one);
-  const long long rem = rem0 - at.kvh * one;
-  int lo = 0, hi = s.J - 1;  // the last j with before(j) <= rem
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (paged_before(p, s, mid) <= rem) {
-      lo = mid;
-    } else {
-      hi = mid - 1;
-    }
-  }
-  at.j = lo;
-  at.start = b_start + at.kvh * one + paged_before(p, s, lo);
-  return at;
-}
-
-// Tile border that stands for place `off` of an item of cost `cost` and nt tiles.
+// Tile border that stands for place `off` of an item of cost `cost` and nt tiles: any
+// function of the three that does not fall as `off` grows will do, and each step of this
+// one is rounded monotonically.
 __device__ __forceinline__ int paged_border(long long off, long long cost, int nt) {
   if (off <= 0) return 0;
   if (off >= cost) return nt;
-  return static_cast<int>((off * nt + (cost >> 1)) / cost);
+  const float f = __fdiv_rn(__ll2float_rn(off), __ll2float_rn(cost));
+  return min(__float2int_rn(__fmul_rn(f, __int2float_rn(nt))), nt);
 }
 
-// Total length of the axis and, for position x = total * c / G of it (c < G), the
-// sequence that holds x and its start. All NT threads of the block call it.
-struct PagedScan {
-  long long part[32];
-  long long total, b_start;
-  int b;
+// floor(a / b) for 0 <= a < 2^62, b > 0, quotient below 2^52. The axis of most batches fits 32
+// bits; else a guess in binary64 is put right.
+__device__ __forceinline__ long long floor_div(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  long long q = static_cast<long long>(__ddiv_rn(static_cast<double>(a), static_cast<double>(b)));
+  while (q * b > a) --q;
+  while ((q + 1) * b <= a) ++q;
+  return q;
+}
+
+// The axis: its length, the pieces it is cut into (no more than the grid has CTAs, and none
+// shorter than a tile), and where piece c starts.
+struct PagedAxis {
+  long long total, whole;  // whole = total / G
+  int G, rest;             // rest = total % G
 };
-template <int NT>
-__device__ __forceinline__ void paged_find(const PagedRows &p, PagedScan &sm, int c, int G,
-                                           long long &total, int &b, long long &b_start) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (p.batch + NT - 1) / NT;
-  const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+__device__ __forceinline__ PagedAxis paged_axis(const PagedRows &p, long long total, int ctas) {
+  PagedAxis x;
+  x.total = total;
+  const long long unit = static_cast<long long>(p.tile) * p.n_rep;
+  x.G = ctas;
+  if (total < unit * ctas) x.G = max(static_cast<int>(floor_div(total, unit)), 1);
+  x.whole = floor_div(total, x.G);
+  x.rest = static_cast<int>(total - x.whole * x.G);
+  return x;
+}
+__device__ __forceinline__ long long paged_piece(const PagedAxis &x, int c) {
+  return x.whole * c + static_cast<unsigned>(x.rest) * static_cast<unsigned>(c) / static_cast<unsigned>(x.G);
+}
+
+// One piece of a CTA's share: tiles t0 .. t1-1 of an item.
+struct Seg {
+  int b, kvh, row0, rows;   // the item's rows among the sequence's R
+  int r0, base, len, kv_end;
+  int t0, t1, whole, slot;  // whole: no border cuts it; slot: which of the CTA's partials else
+};
+constexpr int kSegs = 32;   // segments described at a time
+
+// An item that borders cut, described by the CTA that holds its start: pieces first ..
+// first + n - 1 hold a partial each (the first in slot 1, the others in slot 0).
+struct PagedCut {
+  int n, first;
+  int kvh, row0, rows, r0;
+};
+
+// The walk along a CTA's piece. One warp starts it, its first thread goes on.
+struct SegWalk {
+  long long x_hi, x_lo, start;  // the piece, and the item the walk is at
+  PagedSeq s;
+  int b, kvh, j;
+  PagedAxis axis;
+};
+
+// Called by a whole warp; false: nothing to do for CTA c.
+__device__ __forceinline__ bool walk_start(const PagedRows &p, SegWalk &w, int c, int ctas) {
+  const int lane = threadIdx.x & 31;
+  const int per = (p.batch + 31) / 32;
+  const int b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
   long long mine = 0;
   for (int i = b0; i < b1; ++i) mine += paged_seq_cost(p, paged_seq(p, i));
   long long incl = mine;
@@ -168,36 +189,87 @@ __device__ __forceinline__ void paged_find(const PagedRows &p, PagedScan &sm, in
     const long long o = __shfl_up_sync(0xffffffffu, incl, off);
     if (lane >= off) incl += o;
   }
-  if (lane == 31) sm.part[warp] = incl;
-  __syncthreads();
-  if (warp == 0) {
-    long long w = lane < NT / 32 ? sm.part[lane] : 0;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, w, off);
-      if (lane >= off) w += o;
-    }
-    if (lane < NT / 32) sm.part[lane] = w;
-    if (lane == NT / 32 - 1) sm.total = w;
-  }
-  __syncthreads();
-  total = sm.total;
-  const long long x = total * c / G;
-  long long at = (warp > 0 ? sm.part[warp - 1] : 0) + incl - mine;
-  if (x >= at && x < at + mine) {
-    for (int i = b0; i < b1; ++i) {
-      const long long cost = paged_seq_cost(p, paged_seq(p, i));
-      if (x < at + cost) {
-        sm.b = i;
-        sm.b_start = at;
-        break;
-      }
+  const long long total = __shfl_sync(0xffffffffu, incl, 31);
+  if (total <= 0) return false;
+  const PagedAxis axis = paged_axis(p, total, ctas);
+  if (c >= axis.G) return false;
+  const long long x = paged_piece(axis, c);
+  const int from = __ffs(__ballot_sync(0xffffffffu, x < incl)) - 1;
+  if (lane == from) {
+    long long at = incl - mine;
+    int b = b0;
+    PagedSeq s = paged_seq(p, b);
+    for (;;) {
+      const long long cost = paged_seq_cost(p, s);
+      if (x < at + cost) break;
       at += cost;
+      s = paged_seq(p, ++b);
+    }
+    const long long one = paged_before(p, s, s.J);
+    w.b = b;
+    w.kvh = static_cast<int>(floor_div(x - at, one));
+    at += w.kvh * one;
+    int lo = 0, hi = s.J - 1;  // the last item that starts at x or before
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (paged_before(p, s, mid) <= x - at) {
+        lo = mid;
+      } else {
+        hi = mid - 1;
+      }
+    }
+    w.j = lo;
+    w.start = at + paged_before(p, s, lo);
+    w.s = s;
+    w.x_lo = x;
+    w.x_hi = paged_piece(axis, c + 1);
+    w.axis = axis;
+  }
+  __syncwarp();
+  return true;
+}
+
+// The item at the walk's place as a segment of CTA c's piece, then on to the next one.
+// `cut` is filled when the piece holds the start but not the end of the item.
+__device__ __forceinline__ void walk_next(const PagedRows &p, SegWalk &w, int c, Seg &g, PagedCut &cut) {
+  const long long cost = paged_cost(p, w.s, w.j), end = w.start + cost;
+  g.b = w.b;
+  g.kvh = w.kvh;
+  g.row0 = w.j * p.M;
+  g.rows = min(p.M, w.s.R - g.row0);
+  g.r0 = w.s.r0;
+  g.base = w.s.base;
+  g.len = w.s.len;
+  g.kv_end = paged_kv_end(p, w.s, w.j);
+  const int nt = max((g.kv_end + p.tile - 1) / p.tile, 1);
+  g.t0 = paged_border(w.x_lo - w.start, cost, nt);
+  g.t1 = paged_border(w.x_hi - w.start, cost, nt);
+  g.whole = w.start >= w.x_lo && end <= w.x_hi;
+  g.slot = w.start < w.x_lo ? 0 : 1;
+  if (g.slot == 1 && end > w.x_hi) {
+    // the last piece that starts before the item's end
+    int last = static_cast<int>(floor_div(end, w.axis.whole + (w.axis.rest > 0 ? 1 : 0)));
+    last = min(max(last, c + 1), w.axis.G - 1);
+    while (last + 1 < w.axis.G && paged_piece(w.axis, last + 1) < end) ++last;
+    while (last > c + 1 && paged_piece(w.axis, last) >= end) --last;
+    cut.n = last - c + 1;
+    cut.first = c;
+    cut.kvh = g.kvh;
+    cut.row0 = g.row0;
+    cut.rows = g.rows;
+    cut.r0 = g.r0;
+  }
+  w.start = end;
+  if (++w.j == w.s.J) {
+    w.j = 0;
+    if (++w.kvh == p.n_kv) {
+      w.kvh = 0;
+      while (++w.b < p.batch) {
+        w.s = paged_seq(p, w.b);
+        if (w.s.J > 0) break;
+      }
     }
   }
-  __syncthreads();
-  b = sm.b;
-  b_start = sm.b_start;
 }
 
 }  // namespace chr

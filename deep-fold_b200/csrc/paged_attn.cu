@@ -14,12 +14,16 @@
 // is split over the CTAs by what it costs (paged.cuh).
 
 #include <algorithm>
+#include <cmath>
 
 #include "attn_mma.cuh"
 #include "paged.cuh"
+#include "tma_tc.cuh"
 
 namespace chr {
 namespace {
+
+__device__ int g_attn_paged_status = 0;
 
 struct PagedAttnArgs {
   PagedCache c;
@@ -44,116 +48,110 @@ __device__ __forceinline__ void ldm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
                : "r"(addr));
 }
 
-// One piece of a CTA's share: tiles t0 .. t1-1 of an item.
-struct Seg {
-  int b, kvh, row0, rows;   // the item's rows among the sequence's R
-  int r0, base, len, kv_end;
-  int t0, t1, nt, slot;     // slot: which of the CTA's two partials
+// The workspace: [G] descriptions of cut items, then the partials, [G][2][M] each: the
+// running maximum (log2 units) and sum of a row, and its HD unnormalised outputs.
+struct PagedWs {
+  PagedCut *cut;
+  float2 *ml;
+  float *o;
 };
-
-// Partial results: [CTA][2][M][HD + 2] floats, the row's unnormalised output, its running
-// maximum (log2 units) and its sum.
-__device__ __forceinline__ float *partial_of(const PagedAttnArgs &a, int cta, int slot, int row) {
-  return a.ws + ((static_cast<long long>(cta) * 2 + slot) * a.p.M + row) * (a.c.hd + 2);
+__host__ __device__ __forceinline__ long long ws_floats_of(int ctas, int M, int hd) {
+  return (static_cast<long long>(ctas) * static_cast<int>(sizeof(PagedCut)) + 15) / 16 * 4 +
+         static_cast<long long>(ctas) * 2 * M * (hd + 2);
+}
+__device__ __forceinline__ PagedWs ws_of(const PagedAttnArgs &a, int ctas) {
+  PagedWs w;
+  w.cut = reinterpret_cast<PagedCut *>(a.ws);
+  w.o = a.ws + (static_cast<long long>(ctas) * static_cast<int>(sizeof(PagedCut)) + 15) / 16 * 4;
+  w.ml = reinterpret_cast<float2 *>(w.o + static_cast<long long>(ctas) * 2 * a.p.M * a.c.hd);
+  return w;
 }
 
-// ---- thin form: up to 16 MT query rows per item ----------------------------------------
-// Eight warps on warp-level matrix instructions (m16n8k16, FP32 accumulate). Warp w owns
-// cache rows 16w .. 16w+15 of every 128-row tile: it copies them itself (cp.async ring of
-// its own, the K and the V half of a block as separate stages, so no block-wide barrier
-// stands in the loop), runs its own softmax and its own output accumulator; the warps are
-// folded through shared memory at the end of a segment while the next segment's copies
-// are in flight. Bound by HBM: 16 query rows cost 32 matrix instructions per 16 cache rows,
-// a tenth of what the copy of those rows takes. kStages x 4 KB x 8 warps keep 128 KB in flight per SM
-// (the latency-bandwidth product needs about 55).
-// Probabilities are rounded to bf16 for the second product (their sum is not); q, k and v
-// are bf16 already.
-constexpr int kThinWarps = 8;
-constexpr int kThinThreads = kThinWarps * 32;
-constexpr int kThinTile = kThinWarps * 16;
-constexpr int kSegs = 32;  // segments described at a time
-
-template <int HD, int MT>
-struct ThinLayout {
-  static constexpr int kM = 16 * MT;
-  static constexpr int kHalf = 16 * HD * 2;                                 // 16 rows of K or V
-  static constexpr int kStages = 5;
-  static constexpr int kRing = kThinWarps * kStages * kHalf;
-  static constexpr int kFoldCols = HD < 64 / MT ? HD : 64 / MT;             // columns folded at a time
-  static constexpr int kFold = kThinWarps * kM * kFoldCols * 4;
-  static constexpr int kMl = kThinWarps * kM * 2 * 4;
-  static constexpr int kQ = kM * HD * 2;
-  static constexpr int kSegB = kSegs * static_cast<int>(sizeof(Seg));
-  static constexpr int kBytes = kRing + kFold + kMl + kQ + kSegB + static_cast<int>(sizeof(PagedScan)) + 64;
-};
-
-// Row r, 16-byte chunk c of a block whose rows are HD bf16: the chunk index is mixed with
-// the row so that eight rows of one chunk column fall into eight bank groups.
-template <int HD>
-__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
-  constexpr int C = HD / 8;
-  if (C >= 8) return static_cast<uint32_t>(r * HD * 2 + ((c ^ (r & 7)) << 4));
-  if (C == 4) return static_cast<uint32_t>(r * HD * 2 + ((c ^ ((r >> 1) & 3)) << 4));
-  return static_cast<uint32_t>(r * HD * 2 + ((c ^ ((r >> 2) & 1)) << 4));
-}
-
-// Describes up to kSegs segments from position (at, x) of the CTA's piece on; returns how
-// many, and leaves the place where it stopped. One thread.
-struct SegWalk {
-  long long x_lo, x_hi, b_start;
-  int b;
-  PagedAt at;
-  PagedSeq s;
-};
-__device__ __forceinline__ void walk_start(const PagedAttnArgs &a, SegWalk &w, long long total, int c,
-                                           int G, int b, long long b_start) {
-  w.x_lo = total * c / G;
-  w.x_hi = total * (c + 1) / G;
-  if (w.x_lo >= w.x_hi) return;
-  w.s = paged_seq(a.p, b);
-  w.at = paged_item_at(a.p, w.s, b, b_start, w.x_lo);
-}
-// The item at the walk's place: its segment in this CTA's piece (false: empty), then on.
-__device__ __forceinline__ bool walk_next(const PagedAttnArgs &a, SegWalk &w, Seg &g) {
-  const PagedRows &p = a.p;
-  const long long cost = paged_cost(p, w.s, w.at.j);
-  g.b = w.at.b;
-  g.kvh = w.at.kvh;
-  g.row0 = w.at.j * p.M;
-  g.rows = min(p.M, w.s.R - g.row0);
-  g.r0 = w.s.r0;
-  g.base = w.s.base;
-  g.len = w.s.len;
-  g.kv_end = paged_kv_end(p, w.s, w.at.j);
-  g.nt = max((g.kv_end + p.tile - 1) / p.tile, 1);
-  g.t0 = paged_border(w.x_lo - w.at.start, cost, g.nt);
-  g.t1 = paged_border(w.x_hi - w.at.start, cost, g.nt);
-  g.slot = w.at.start < w.x_lo ? 0 : 1;
-  const bool some = g.t0 < g.t1;
-  // on to the next item
-  w.at.start += cost;
-  if (++w.at.j == w.s.J) {
-    w.at.j = 0;
-    if (++w.at.kvh == p.n_kv) {
-      w.at.kvh = 0;
-      while (++w.at.b < p.batch) {
-        w.s = paged_seq(p, w.at.b);
-        if (w.s.J > 0) break;
+// Describes up to kSegs segments of CTA c's piece from the walk's place on: their number.
+// One thread. An empty piece of a cut item is noted as such, and so is a cut item that
+// starts in the piece (at most its last).
+__device__ __forceinline__ int walk_fill(const PagedAttnArgs &a, SegWalk &w, int c, int ctas, Seg *segs) {
+  int n = 0;
+  PagedCut cut;
+  cut.n = 0;
+  const PagedWs ws = ws_of(a, ctas);
+  while (n < kSegs && w.start < w.x_hi && w.b < a.p.batch) {
+    Seg g;
+    walk_next(a.p, w, c, g, cut);
+    if (g.t0 < g.t1) {
+      segs[n++] = g;
+    } else if (!g.whole) {
+      for (int r = 0; r < g.rows; ++r) {
+        ws.ml[(static_cast<long long>(c) * 2 + g.slot) * a.p.M + r] = make_float2(-INFINITY, 0.f);
       }
     }
   }
-  return some;
-}
-__device__ __forceinline__ int walk_fill(const PagedAttnArgs &a, SegWalk &w, Seg *segs) {
-  int n = 0;
-  while (n < kSegs && w.x_lo < w.x_hi && w.at.start < w.x_hi && w.at.b < a.p.batch) {
-    Seg g;
-    if (walk_next(a, w, g)) segs[n++] = g;
-  }
+  if (cut.n != 0) ws.cut[c] = cut;
   return n;
 }
 
-// Whether query row r (of the sequence's R) sees cache row t >= base, t < len.
+// Zeros for the rows behind the last sequence's, when the call asks for them.
+template <int HD>
+__device__ __forceinline__ void zero_tail_rows(const PagedAttnArgs &a, int cta, int G) {
+  if (a.zero_tail == 0 || a.p.q_start == nullptr) return;
+  const int last = min(max(__ldg(a.p.q_start + a.p.batch), 0), a.p.T);
+  const long long width = static_cast<long long>(a.p.n_kv) * a.p.n_rep * HD / 8;
+  const long long n16 = (a.p.T - last) * width;
+  uint4 *dst = reinterpret_cast<uint4 *>(a.out) + last * width;
+  for (long long i = static_cast<long long>(cta) * blockDim.x + threadIdx.x; i < n16;
+       i += static_cast<long long>(G) * blockDim.x) {
+    dst[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// ---- thin form: up to 8 NQ query rows per item -----------------------------------------
+// Four warps on warp-level matrix instructions (m16n8k16, FP32 accumulate). Warp w owns
+// cache rows 16w .. 16w+15 of every 64-row tile: it requests them itself (TMA, a ring of
+// its own, the K and the V half of a block as separate stages), keeps its own running
+// maximum, sum and output, and no block-wide barrier stands in the loop; the warps are
+// folded through shared memory at the end of a segment, while the next one's copies are
+// in flight. Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T: the cache
+// rows are the 16-row operand and the queries the 8-column one, so a kv group of up to 8
+// heads fills its tiles (as 16-row operand it would leave half of every product empty),
+// and P^T comes out of S^T by one 8x8 transpose per tile.
+// Bound by HBM: a 16-row block costs about 100 + 60 NQ warp instructions, and two CTAs of four
+// warps with 4 x 4 KB requested each keep 128 KB in flight per SM (the latency-bandwidth
+// product needs about 55).
+// The subtracted maximum follows a row's scores with a slack of 8 (in log2): it is raised, and
+// the accumulator rescaled, only when a score exceeds it by more, so that a block without
+// such a score costs one vote instead of a maximum over its lanes; P stays below 2^8.
+// Probabilities are rounded to bf16 for the second product (their sum is not); q, k and v
+// are bf16 already.
+constexpr int kThinWarps = 4;
+constexpr int kThinThreads = kThinWarps * 32;
+constexpr int kThinTile = kThinWarps * 16;
+constexpr float kSlack = 8.f;
+
+template <int HD, int NQ>
+struct ThinLayout {
+  static constexpr int kM = 8 * NQ;
+  static constexpr int kHalf = 16 * HD * 2;                                 // 16 rows of K or V
+  static constexpr int kStages = 5;
+  static constexpr int kRing = kThinWarps * kStages * kHalf;
+  static constexpr int kFoldCols = HD < 128 / NQ ? HD : 128 / NQ;           // columns folded at a time
+  static constexpr int kFold = kThinWarps * kM * kFoldCols * 4;
+  static constexpr int kMl = kThinWarps * kM * 2 * 4;
+  static constexpr int kQ = NQ > 2 ? kM * HD * 2 : 0;
+  static constexpr int kSegB = kSegs * static_cast<int>(sizeof(Seg));
+  static constexpr int kBytes = kRing + kFold + kMl + kQ + kSegB + kThinWarps * kStages * 8 + 1024;
+};
+
+// Row r, 16-byte chunk c of a 16-row block as TMA lays it: pieces of (up to) 64 elements, the
+// chunk index mixed with the row so that eight rows of a chunk column fall into eight bank groups.
+template <int HD>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  constexpr int C = HD / 8;
+  if (C >= 8) return static_cast<uint32_t>((c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+  if (C == 4) return static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+  return static_cast<uint32_t>(r * 32 + ((c ^ ((r >> 2) & 1)) << 4));
+}
+
+// Whether a token's row sees cache row t, base <= t < len.
 __device__ __forceinline__ bool sees_draft(const PagedAttnArgs &a, const Seg &g, int token, int t) {
   const int d = t - g.base;
   if (a.tree == nullptr) return d <= token;
@@ -163,13 +161,23 @@ __device__ __forceinline__ bool sees_draft(const PagedAttnArgs &a, const Seg &g,
   return (w >> (d & 63)) & 1ull;
 }
 
-template <int HD, int MT>
-__global__ void __launch_bounds__(kThinThreads, 1) attn_paged_thin_kernel(const PagedAttnArgs a) {
-  using L = ThinLayout<HD, MT>;
-  constexpr int KS = HD / 16, NT = HD / 8, C = HD / 8;
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <int HD, int NQ>
+__global__ void __launch_bounds__(kThinThreads, 2)
+attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                       const PagedAttnArgs a) {
+  using L = ThinLayout<HD, NQ>;
+  constexpr int KS = HD / 16, C = HD / 8;
   constexpr int M = L::kM;
   constexpr int S = L::kStages;
-  extern __shared__ __align__(128) unsigned char smem[];
+  constexpr bool KEEP = NQ == 1;  // the next segment's queries in registers
+  extern __shared__ __align__(16) unsigned char thin_smem[];
+  unsigned char *smem = thin_smem + ((1024u - (smem_u32(thin_smem) & 1023u)) & 1023u);
   unsigned char *at = smem + L::kRing;
   float *fold = reinterpret_cast<float *>(at);
   at += L::kFold;
@@ -179,278 +187,322 @@ __global__ void __launch_bounds__(kThinThreads, 1) attn_paged_thin_kernel(const 
   at += L::kQ;
   Seg *segs = reinterpret_cast<Seg *>(at);
   at += L::kSegB;
-  PagedScan &scan = *reinterpret_cast<PagedScan *>(at);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(at);  // [warp][stage]
   __shared__ int n_segs;
+  __shared__ SegWalk walk;  // thread 0's: not worth the registers of a thread
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g8 = lane >> 2, t4 = lane & 3;
   const int G = gridDim.x, cta = blockIdx.x;
-  pdl_wait();
-  pdl_trigger();  // behind the wait: the join kernel reads q_start and kv_len before its own
-  long long total, b_start;
-  int b_first;
-  paged_find<kThinThreads>(a.p, scan, cta, G, total, b_first, b_start);
-  SegWalk walk;
-  walk.x_lo = walk.x_hi = 0;
-  if (tid == 0 && total > 0) walk_start(a, walk, total, cta, G, b_first, b_start);
-
-  // rows behind the last sequence's
-  if (a.zero_tail != 0) {
-    const int last = a.p.q_start != nullptr
-                         ? min(max(__ldg(a.p.q_start + a.p.batch), 0), a.p.T) : min(a.p.batch, a.p.T);
-    const long long width = static_cast<long long>(a.p.n_kv) * a.p.n_rep * HD / 8;
-    const long long n16 = (a.p.T - last) * width;
-    uint4 *dst = reinterpret_cast<uint4 *>(a.out) + last * width;
-    for (long long i = static_cast<long long>(cta) * kThinThreads + tid; i < n16;
-         i += static_cast<long long>(G) * kThinThreads) {
-      dst[i] = make_uint4(0, 0, 0, 0);
-    }
+  if (tid < kThinWarps * S) bar_init(bars + tid, 1);
+  if (tid == 0) {
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&k_map);
+    prefetch_map(&v_map);
   }
+  pdl_wait();
+  pdl_trigger();
+  if (warp == 0) {
+    if (lane == 0) ws_of(a, G).cut[cta].n = 0;
+    const bool some = walk_start(a.p, walk, cta, G);
+    if (lane == 0) n_segs = some ? walk_fill(a, walk, cta, G, segs) : 0;
+  }
+  zero_tail_rows<HD>(a, cta, G);
+  __syncthreads();
 
   const uint32_t ring = smem_u32(smem) + warp * S * L::kHalf;
+  uint64_t *bar = bars + warp * S;
   const uint32_t q_base = smem_u32(q_s);
   const int shift = a.c.page_shift;
-  const long long row_el = static_cast<long long>(a.c.n_kv) * HD;
+  bool ok = true;       // this warp's copies have all arrived in time
+  int slot = 0;         // ring slot of the half block consumed next
+  int ahead = 0;        // ring slot requested next
+  uint32_t phase = 0;   // parity of each slot's next completed copy
 
-  for (;;) {
-    if (tid == 0) n_segs = walk_fill(a, walk, segs);
-    __syncthreads();
-    const int n_now = n_segs;
-    if (n_now == 0) break;
-
-    // The copies run ahead of the arithmetic over this batch of segments: (cs, ct) is the
-    // block whose half `ch` (0 K, 1 V) is requested next, its page looked up in advance.
-    int cs = 0, ct = segs[0].t0, ch = 0;
-    int c_page = -1;
-    // whether the blocks requested and not yet used have rows at all (a block past the
-    // item's end, or on a page outside the pool, has none); bit: the block's number
+  for (int n_now = n_segs; n_now != 0;) {
+    // A segment's queries (where they fit registers next to the running ones) and the pages of
+    // its first 32 tiles (lane i: this warp's block of tile t0 + i) are fetched one segment early.
+    uint32_t qn[KEEP ? KS : 1][2];
+    int n_ids = -1;
+    auto q_row = [&](const Seg &g, int r) {
+      const int token = (g.row0 + r) / a.p.n_rep;
+      const int head = g.kvh * a.p.n_rep + (g.row0 + r) - token * a.p.n_rep;
+      return a.q + (g.r0 + token) * a.q_stride + head * HD;
+    };
+    auto ids_of = [&](int seg, int t) {
+      const int row = (t + lane) * kThinTile + warp * 16;
+      if (t + lane < segs[seg].t1 && row < segs[seg].kv_end) {
+        return __ldg(a.c.table + segs[seg].b * a.c.table_stride + (row >> shift));
+      }
+      return -1;
+    };
+    auto fetch_early = [&](int seg) {
+      if (seg >= n_now) return;
+      n_ids = ids_of(seg, segs[seg].t0);
+      if (KEEP) {
+        const Seg &g = segs[seg];
+        const uint32_t *src = reinterpret_cast<const uint32_t *>(q_row(g, min(g8, g.rows - 1)));
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          qn[KEEP ? ks : 0][0] = __ldcg(src + ks * 8 + t4);
+          qn[KEEP ? ks : 0][1] = __ldcg(src + ks * 8 + 4 + t4);
+        }
+      }
+    };
+    fetch_early(0);
+    // The copies run ahead of the arithmetic over this batch of segments: half `c_half` (0 K,
+    // 1 V) of tile c_t of segment c_s is requested next. Lane i holds the page of this
+    // warp's block of tile c_first + i.
+    int c_s = 0, c_t = segs[0].t0, c_half = 0, c_end = segs[0].t1;
+    int c_kvh = segs[0].kvh, c_first = c_t, c_ids = n_ids, c_early = 0;  // c_early: the segment n_ids is of
+    // whether the blocks requested and not yet used have rows at all (a block past the item's
+    // end, or on a page outside the pool, has none and is not copied); bit: the block's number
     unsigned has_rows = 0, n_asked = 0, n_used = 0;
-    auto look_up = [&]() {
-      if (cs >= n_now) return;
-      const int row = ct * kThinTile + warp * 16;
-      c_page = -1;
-      if (row < segs[cs].kv_end) {
-        const int id = __ldg(a.c.table + segs[cs].b * a.c.table_stride + (row >> shift));
-        c_page = id >= 0 && id < a.c.n_pages ? id : -1;
-      }
-    };
-    // Requests one half block into ring slot `slot` (nothing when all are requested); every
-    // call is one commit group, so that groups and half blocks count alike.
-    auto request = [&](int slot) {
-      if (cs < n_now) {
-        const int row = ct * kThinTile + warp * 16;
-        const int live = c_page < 0 ? 0 : min(max(segs[cs].kv_end - row, 0), 16);
-        const __nv_bfloat16 *src =
-            (ch == 0 ? a.c.k : a.c.v) +
-            (live > 0 ? c_page * (ch == 0 ? a.c.k_page_stride : a.c.v_page_stride) +
-                            (row & ((1 << shift) - 1)) * row_el + segs[cs].kvh * HD
-                      : 0);
-        const uint32_t dst = ring + slot * L::kHalf;
-        constexpr int kPer = 16 * C / 32;  // 16-byte pieces per lane
+    auto request = [&]() {
+      if (c_s >= n_now) return;
+      const int row = c_t * kThinTile + warp * 16;
+      const int c_page = __shfl_sync(0xffffffffu, c_ids, c_t - c_first);
+      const bool live = static_cast<unsigned>(c_page) < static_cast<unsigned>(a.c.n_pages) && ok;
+      if (live && lane == 0) {
+        const uint32_t dst = ring + ahead * L::kHalf;
+        const CUtensorMap *map = c_half == 0 ? &k_map : &v_map;
+        bar_expect(bar + ahead, L::kHalf);
 #pragma unroll
-        for (int i = 0; i < (kPer > 0 ? kPer : 1); ++i) {
-          const int piece = i * 32 + lane;
-          const int r = piece / C, c = piece % C;
-          // rows past the end are filled with zeros: whatever the page holds there must not
-          // reach the products (0 x NaN)
-          const bool on = r < live;
-          mma_cp16(dst + chunk_at<HD>(r, c), on ? src + r * row_el + c * 8 : a.c.k, on ? 16 : 0);
-        }
-        if (ch == 0) {
-          has_rows = (has_rows & ~(1u << (n_asked & 31))) | ((live > 0 ? 1u : 0u) << (n_asked & 31));
-          ++n_asked;
-          ch = 1;
-        } else {
-          ch = 0;
-          if (++ct == segs[cs].t1) {
-            if (++cs < n_now) ct = segs[cs].t0;
-          }
-          look_up();
+        for (int h = 0; h < (HD > 64 ? HD / 64 : 1); ++h) {
+          tma_page(dst + h * 2048, map, bar + ahead, h * 64, c_kvh, row & ((1 << shift) - 1), c_page);
         }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      ahead = ahead + 1 == S ? 0 : ahead + 1;
+      if (c_half == 0) {
+        has_rows = (has_rows & ~(1u << (n_asked & 31))) | ((live ? 1u : 0u) << (n_asked & 31));
+        ++n_asked;
+        c_half = 1;
+        return;
+      }
+      c_half = 0;
+      if (++c_t == c_end) {
+        if (++c_s < n_now) {
+          c_t = segs[c_s].t0;
+          c_end = segs[c_s].t1;
+          c_kvh = segs[c_s].kvh;
+          c_first = c_t;
+          c_ids = c_s == c_early ? n_ids : ids_of(c_s, c_t);
+        }
+      } else if (c_t - c_first == 32) {
+        c_first = c_t;
+        c_ids = ids_of(c_s, c_t);
+      }
     };
-    look_up();
+    // The copy into the slot consumed next (bounded; nothing is in it when !live).
+    auto arrived = [&](bool live) {
+      if (live && ok) {
+        ok = __all_sync(0xffffffffu, bar_poll(bar + slot, (phase >> slot) & 1u));
+        if (!ok && lane == 0) atomicExch(&g_attn_paged_status, 20);
+        phase ^= 1u << slot;
+      }
+      return live && ok;
+    };
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) request(i);
-    int slot = 0;  // ring slot of the half block consumed next
-    int ahead = S - 1;  // ring slot requested next
+    for (int i = 0; i < S - 1; ++i) request();
 
     for (int si = 0; si < n_now; ++si) {
       const Seg g = segs[si];
-      // ---- the item's queries: rows of the matrix tiles, zero past the last ----
-      for (int i = tid; i < M * C; i += kThinThreads) {
-        const int r = i / C, c = i - r * C;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < g.rows) {
-          const int token = (g.row0 + r) / a.p.n_rep;
-          const int head = g.kvh * a.p.n_rep + (g.row0 + r) - token * a.p.n_rep;
-          v = ld_act16(a.q + (g.r0 + token) * a.q_stride + head * HD + c * 8);
+      // ---- the item's queries as 8-column operands, zero past the last row ----
+      uint32_t qf[NQ <= 2 ? NQ : 1][NQ <= 2 ? KS : 1][2];
+      if (NQ <= 2) {
+#pragma unroll
+        for (int n = 0; n < (NQ <= 2 ? NQ : 1); ++n) {
+          const int r = n * 8 + g8;
+          const uint32_t *src = reinterpret_cast<const uint32_t *>(q_row(g, min(r, g.rows - 1)));
+#pragma unroll
+          for (int ks = 0; ks < (NQ <= 2 ? KS : 1); ++ks) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t v = KEEP ? qn[KEEP ? ks : 0][h] : __ldcg(src + ks * 8 + h * 4 + t4);
+              qf[n][ks][h] = r < g.rows ? v : 0u;
+            }
+          }
         }
-        *reinterpret_cast<uint4 *>(q_s + chunk_at<HD>(r, c)) = v;
+      } else {
+        for (int i = tid; i < M * C; i += kThinThreads) {
+          const int r = i / C, c = i - r * C;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (r < g.rows) v = ld_act16(q_row(g, r) + c * 8);
+          *reinterpret_cast<uint4 *>(q_s + (r >> 4) * L::kHalf + chunk_at<HD>(r & 15, c)) = v;
+        }
+        __syncthreads();
       }
-      __syncthreads();
-      // thread rows: mt * 16 + g8 and + 8
-      int token[MT][2];
+      if (c_s <= si + 1) {  // the copies have not passed the next segment's start yet
+        fetch_early(si + 1);
+        c_early = si + 1;
+      } else if (KEEP) {
+        fetch_early(si + 1);
+        c_early = -1;
+      }
+      // this thread's queries: n * 8 + 2 t4 and + 1
+      int token[NQ][2];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
+      for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = mt * 16 + h * 8 + g8;
-          token[mt][h] = r < g.rows ? (g.row0 + r) / a.p.n_rep : -1;
+        for (int e = 0; e < 2; ++e) {
+          const int r = n * 8 + 2 * t4 + e;
+          token[n][e] = r < g.rows ? (g.row0 + r) / a.p.n_rep : -1;
         }
       }
-      const uint32_t qa = (lane & 15), qc = lane >> 4;  // this lane's row and chunk of an A load
-      uint32_t qf[MT == 1 ? KS : 1][4];
-      if (MT == 1) {
+      float o[NQ][KS][4];  // O^T: element rows ks * 16 + g8 (+ 8), queries 2 t4 (+ 1)
+      float m_run[NQ][2], l_run[NQ][2];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) ldm_x4(q_base + chunk_at<HD>(qa, ks * 2 + qc), qf[ks]);
-      }
-      float o[MT][NT][4];
-      float m_run[MT][2], l_run[MT][2];
+      for (int n = 0; n < NQ; ++n) {
+        m_run[n][0] = m_run[n][1] = -INFINITY;
+        l_run[n][0] = l_run[n][1] = 0.f;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        m_run[mt][0] = m_run[mt][1] = -INFINITY;
-        l_run[mt][0] = l_run[mt][1] = 0.f;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) o[mt][n][0] = o[mt][n][1] = o[mt][n][2] = o[mt][n][3] = 0.f;
+        for (int ks = 0; ks < KS; ++ks) o[n][ks][0] = o[n][ks][1] = o[n][ks][2] = o[n][ks][3] = 0.f;
       }
 
       for (int t = g.t0; t < g.t1; ++t) {
         const int row = t * kThinTile + warp * 16;
-        const uint32_t k_blk = ring + slot * L::kHalf;
-        const int v_slot = slot + 1 == S ? 0 : slot + 1;
-        const uint32_t v_blk = ring + v_slot * L::kHalf;
-        // K half: all but the S - 2 latest groups have landed; each is this warp's own
-        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
-        __syncwarp();
-        const bool live = (has_rows >> (n_used & 31)) & 1u;
+        bool live = (has_rows >> (n_used & 31)) & 1u;
         ++n_used;
-        float s[MT][2][4];
+        const uint32_t k_blk = ring + slot * L::kHalf;
+        live = arrived(live);
+        slot = slot + 1 == S ? 0 : slot + 1;
+        float s[NQ][4];  // keys g8 (0, 1) and g8 + 8 (2, 3) of the block, queries 2 t4, 2 t4 + 1
         if (live) {
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
-          }
-          const int kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
+          for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
-            uint32_t b[4];
-            ldm_x4(k_blk + chunk_at<HD>(kr, ks * 2 + kc), b);
+            uint32_t k4[4];  // (rows 0-7, k 0-7), (rows 8-15, k 0-7), (rows 0-7, k 8-15), (rows 8-15, k 8-15)
+            ldm_x4(k_blk + chunk_at<HD>(lane & 15, ks * 2 + (lane >> 4)), k4);
+            if (NQ <= 2) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              uint32_t q4[4];
-              if (MT == 1) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) q4[e] = qf[ks][e];
-              } else {
-                ldm_x4(q_base + chunk_at<HD>(mt * 16 + qa, ks * 2 + qc), q4);
+              for (int n = 0; n < NQ; ++n) {
+                mma_bf16(s[n], k4[0], k4[1], k4[2], k4[3], qf[NQ <= 2 ? n : 0][NQ <= 2 ? ks : 0][0],
+                         qf[NQ <= 2 ? n : 0][NQ <= 2 ? ks : 0][1]);
               }
-              mma_bf16(s[mt][0], q4[0], q4[1], q4[2], q4[3], b[0], b[1]);
-              mma_bf16(s[mt][1], q4[0], q4[1], q4[2], q4[3], b[2], b[3]);
+            } else {
+#pragma unroll
+              for (int n = 0; n < NQ; n += 2) {
+                uint32_t q4[4];  // queries 0-7 then 8-15 of the pair, k 0-7 and 8-15 each
+                ldm_x4(q_base + (n >> 1) * L::kHalf +
+                           chunk_at<HD>((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)), q4);
+                mma_bf16(s[n], k4[0], k4[1], k4[2], k4[3], q4[0], q4[1]);
+                mma_bf16(s[n + 1 < NQ ? n + 1 : n], k4[0], k4[1], k4[2], k4[3], q4[2], q4[3]);
+              }
             }
           }
         }
         __syncwarp();
-        request(ahead);
-        ahead = ahead + 1 == S ? 0 : ahead + 1;
-        uint32_t pa[MT][4];
+        request();  // into the slot freed a half block ago
+        uint32_t p[NQ][2];
         if (live) {
-          // all of the block is older than the new rows: every row sees it
-          const bool plain = row + 16 <= g.base;
+          // a block that reaches the new rows, or the item's end, is masked key by key
+          const bool masked = row + 16 > g.base;
+          bool over = false;
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
+          for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float sv[4];
-              float mx = -INFINITY;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int key = row + (e >> 1) * 8 + 2 * t4 + (e & 1);
-                const float x = s[mt][e >> 1][h * 2 + (e & 1)] * a.c2;
-                bool on = true;
-                if (!plain) {
-                  on = key < g.kv_end &&
-                       (key < g.base || (token[mt][h] >= 0 && sees_draft(a, g, token[mt][h], key)));
-                }
-                sv[e] = on ? x : -INFINITY;
-                mx = fmaxf(mx, sv[e]);
+            for (int e = 0; e < 4; ++e) {
+              s[n][e] *= a.c2;
+              if (masked) {
+                const int key = row + g8 + (e >> 1) * 8;
+                const int tok = token[n][e & 1];
+                const bool on = key < g.kv_end && (key < g.base || (tok >= 0 && sees_draft(a, g, tok, key)));
+                s[n][e] = on ? s[n][e] : -INFINITY;
               }
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-              const float m_new = fmaxf(m_run[mt][h], mx);
-              const float m_use = m_new == -INFINITY ? 0.f : m_new;  // nothing seen so far
-              const float alpha = exp2f(m_run[mt][h] - m_use);
-              float psum = 0.f;
+              over |= s[n][e] > m_run[n][e & 1] + kSlack;
+            }
+          }
+          if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                sv[e] = exp2f(sv[e] - m_use);
-                psum += sv[e];
-              }
-              l_run[mt][h] = fmaf(l_run[mt][h], alpha, psum);
-              m_run[mt][h] = m_new;
-              if (__any_sync(0xffffffffu, alpha != 1.f)) {
+            for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                  o[mt][n][h * 2] *= alpha;
-                  o[mt][n][h * 2 + 1] *= alpha;
+              for (int e = 0; e < 2; ++e) {
+                float mx = fmaxf(s[n][e], s[n][e + 2]);
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                const float m_new = fmaxf(m_run[n][e], mx);
+                const float alpha = m_new == -INFINITY ? 1.f : exp2f(m_run[n][e] - m_new);
+                m_run[n][e] = m_new;
+                l_run[n][e] *= alpha;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                  o[n][ks][e] *= alpha;
+                  o[n][ks][e + 2] *= alpha;
                 }
               }
-              pa[mt][h] = mma_pack(sv[0], sv[1]);
-              pa[mt][2 + h] = mma_pack(sv[2], sv[3]);
             }
           }
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float m = m_run[n][e & 1];
+              x[e] = fast_exp2(s[n][e] - (m == -INFINITY ? 0.f : m));  // nothing seen so far: all -inf
+              l_run[n][e & 1] += x[e];
+            }
+            p[n][0] = transpose8(mma_pack(x[0], x[1]));
+            p[n][1] = transpose8(mma_pack(x[2], x[3]));
+          }
         }
-        // V half
-        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
-        __syncwarp();
+        const uint32_t v_blk = ring + slot * L::kHalf;
+        live = arrived(live);
+        slot = slot + 1 == S ? 0 : slot + 1;
         if (live) {
-          const int vr = (lane & 7) + (((lane >> 3) & 1) << 3), vc = lane >> 4;
-#pragma unroll
-          for (int n2 = 0; n2 < NT / 2; ++n2) {
-            uint32_t b[4];
-            ldm_x4_trans(v_blk + chunk_at<HD>(vr, n2 * 2 + vc), b);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              mma_bf16(o[mt][2 * n2], pa[mt][0], pa[mt][1], pa[mt][2], pa[mt][3], b[0], b[1]);
-              mma_bf16(o[mt][2 * n2 + 1], pa[mt][0], pa[mt][1], pa[mt][2], pa[mt][3], b[2], b[3]);
+          if (row + 16 > g.kv_end) {
+            // rows behind the last may hold anything (0 x NaN): zeros for the product
+            for (int i = lane; i < 16 * C; i += 32) {
+              const int r = i / C;
+              if (row + r >= g.kv_end) {
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v_blk + chunk_at<HD>(r, i - r * C)), "r"(0)
+                             : "memory");
+              }
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            uint32_t v4[4];  // V^T: (d 0-7, key 0-7), (d 8-15, key 0-7), (d 0-7, key 8-15), (d 8-15, key 8-15)
+            ldm_x4_trans(v_blk + chunk_at<HD>((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)), v4);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) mma_bf16(o[n][ks], v4[0], v4[1], v4[2], v4[3], p[n][0], p[n][1]);
           }
         }
         __syncwarp();
-        request(ahead);
-        ahead = ahead + 1 == S ? 0 : ahead + 1;
-        slot = v_slot + 1 == S ? 0 : v_slot + 1;
+        request();
       }
 
       // ---- fold the warps, kFoldCols columns at a time ----
+      __syncthreads();  // the last segment's fold has been read
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
+      for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float l = l_run[mt][h];
-          l += __shfl_xor_sync(0xffffffffu, l, 1);
-          l += __shfl_xor_sync(0xffffffffu, l, 2);
-          if (t4 == 0) {
-            float *w = ml + (warp * M + mt * 16 + h * 8 + g8) * 2;
-            w[0] = m_run[mt][h];
+        for (int e = 0; e < 2; ++e) {
+          float l = l_run[n][e];
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+          if (g8 == 0) {
+            float *w = ml + (warp * M + n * 8 + 2 * t4 + e) * 2;
+            w[0] = m_run[n][e];
             w[1] = l;
           }
         }
       }
-      const bool whole = g.t0 == 0 && g.t1 == g.nt;
+      const PagedWs ws = ws_of(a, G);
+      const long long part = (static_cast<long long>(cta) * 2 + g.slot) * M;
       constexpr int FC = L::kFoldCols;
 #pragma unroll
       for (int f = 0; f < HD / FC; ++f) {
+        if (f > 0) __syncthreads();  // the last columns have been read
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-          for (int n = 0; n < FC / 8; ++n) {
+          for (int k = 0; k < FC / 16; ++k) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              *reinterpret_cast<float2 *>(fold + (warp * M + mt * 16 + h * 8 + g8) * FC + n * 8 + 2 * t4) =
-                  make_float2(o[mt][f * (FC / 8) + n][h * 2], o[mt][f * (FC / 8) + n][h * 2 + 1]);
+            for (int e = 0; e < 4; ++e) {
+              fold[(warp * M + n * 8 + 2 * t4 + (e & 1)) * FC + k * 16 + (e >> 1) * 8 + g8] = o[n][f * (FC / 16) + k][e];
             }
           }
         }
@@ -464,142 +516,259 @@ __global__ void __launch_bounds__(kThinThreads, 1) attn_paged_thin_kernel(const 
           float ll = 0.f, oo = 0.f;
 #pragma unroll
           for (int w = 0; w < kThinWarps; ++w) {
-            const float e = exp2f(ml[(w * M + r) * 2] - m_use);
+            const float e = fast_exp2(ml[(w * M + r) * 2] - m_use);
             ll = fmaf(e, ml[(w * M + r) * 2 + 1], ll);
             oo = fmaf(e, fold[(w * M + r) * FC + d], oo);
           }
           const int col = f * FC + d;
-          if (whole) {
+          if (g.whole) {
             const int tok = (g.row0 + r) / a.p.n_rep;
             const int head = g.kvh * a.p.n_rep + (g.row0 + r) - tok * a.p.n_rep;
             a.out[(static_cast<long long>(g.r0 + tok) * a.p.n_kv * a.p.n_rep + head) * HD + col] =
                 __float2bfloat16(ll != 0.f ? oo / ll : 0.f);
           } else {
-            float *dst = partial_of(a, cta, g.slot, r);
-            dst[col] = oo;
-            if (col == 0) {
-              dst[HD] = mm;
-              dst[HD + 1] = ll;
-            }
+            ws.o[(part + r) * HD + col] = oo;
+            if (col == 0) ws.ml[part + r] = make_float2(mm, ll);
           }
         }
-        __syncthreads();
       }
     }
-    // the ring holds nothing that is still wanted; groups in flight are empty
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
+    if (tid == 0) n_segs = walk_fill(a, walk, cta, G, segs);
+    __syncthreads();
+    n_now = n_segs;
+    __syncthreads();
+  }
+  if (!ok) {
+    // a copy is late: nothing leaves before the others in flight have landed
+    for (int i = 0; i < S; ++i) bar_poll(bar + i, (phase >> i) & 1u);
   }
 }
 
+}  // namespace
+}  // namespace chr
+
+#include "paged_attn_wide.cuh"
+
+namespace chr {
+namespace {
+
 // ---- joins the partials of items that CTA borders cut -------------------------------
-// Block c looks at the border between CTAs c and c+1: the first border inside an item
-// joins that item's partials, a warp per row.
+// Block (x, y) looks at the descriptions of eight CTAs, a warp each, and joins every
+// gridDim.y-th row from y on of the items they hold the start of: a warp per item where it lies
+// in a few pieces, the whole block, its pieces dealt over the warps, where it lies in many.
 constexpr int kJoinThreads = 256;
-constexpr int kMaxCtas = 256;
+constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr int kJoinFew = 16;
+
+__device__ __forceinline__ void join_store(const PagedAttnArgs &a, const PagedCut &cut, int r, int lane, float4 acc,
+                                           float l) {
+  if (lane * 4 >= a.c.hd) return;
+  const int tok = (cut.row0 + r) / a.p.n_rep;
+  const int head = cut.kvh * a.p.n_rep + (cut.row0 + r) - tok * a.p.n_rep;
+  const float by = l != 0.f ? 1.f / l : 0.f;
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * by, acc.y * by);
+  const __nv_bfloat162 hi = __floats2bfloat162_rn(acc.z * by, acc.w * by);
+  *reinterpret_cast<uint2 *>(a.out + (static_cast<long long>(cut.r0 + tok) * a.p.n_kv * a.p.n_rep + head) * a.c.hd +
+                             lane * 4) =
+      make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+}
+
 __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const PagedAttnArgs a, int G) {
-  __shared__ PagedScan scan;
-  __shared__ int from[kMaxCtas];                            // partial of each piece, -1: empty
-  __shared__ float weight[kJoinThreads / 32][kMaxCtas];
+  __shared__ PagedCut cuts[kJoinWarps];
+  __shared__ float4 fold[kJoinWarps][32];
+  __shared__ float red[2][kJoinWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int c = blockIdx.x + 1;
   const int hd = a.c.hd;
-  // The split is derived before the wait: the attention kernel raises its trigger only
-  // behind its own wait, so what q_start and kv_len hold is there already.
   pdl_trigger();
-  long long total, b_start;
-  int b;
-  paged_find<kJoinThreads>(a.p, scan, c, G, total, b, b_start);
-  if (total <= 0) return;
-  const long long x = total * c / G;
-  const PagedSeq s = paged_seq(a.p, b);
-  const PagedAt at = paged_item_at(a.p, s, b, b_start, x);
-  if (at.start >= x || total * (c - 1) / G > at.start) return;  // not inside, or not the first
-  const long long cost = paged_cost(a.p, s, at.j);
-  const int nt = max((paged_kv_end(a.p, s, at.j) + a.p.tile - 1) / a.p.tile, 1);
-  // the CTA that holds the item's end: the last one whose piece starts before it
-  const int first = c - 1;
-  const int last = min(static_cast<int>(((at.start + cost) * G - 1) / total), G - 1);
-  const int n = last - first + 1;
-  const int row0 = at.j * a.p.M, rows = min(a.p.M, s.R - row0);
-  bool whole = false;  // a piece that was rounded to the whole item has been written by its CTA
-  for (int i = tid; i < n; i += kJoinThreads) {
-    const long long lo = total * (first + i) / G;
-    const int t0 = paged_border(lo - at.start, cost, nt);
-    const int t1 = paged_border(total * (first + i + 1) / G - at.start, cost, nt);
-    from[i] = t0 < t1 ? (first + i) * 2 + (at.start < lo ? 0 : 1) : -1;
-    whole |= t0 == 0 && t1 == nt;
-  }
-  if (__syncthreads_or(whole)) return;
   pdl_wait();
-  for (int r = warp; r < rows; r += kJoinThreads / 32) {
-    auto src = [&](int i) { return a.ws + (static_cast<long long>(from[i]) * a.p.M + r) * (hd + 2); };
-    float mm = -INFINITY;
-    for (int i = lane; i < n; i += 32) {
-      if (from[i] >= 0) mm = fmaxf(mm, __ldcg(src(i) + hd));
+  const PagedWs ws = ws_of(a, G);
+  const int c = blockIdx.x * kJoinWarps + warp;
+  PagedCut cut;
+  cut.n = 0;
+  if (c < G) {
+    static_assert(sizeof(PagedCut) == 24, "three 8-byte loads");
+    const int2 *src = reinterpret_cast<const int2 *>(ws.cut + c);
+    const int2 d0 = __ldcg(src), d1 = __ldcg(src + 1), d2 = __ldcg(src + 2);
+    cut.n = d0.x;
+    cut.first = d0.y;
+    cut.kvh = d1.x;
+    cut.row0 = d1.y;
+    cut.rows = d2.x;
+    cut.r0 = d2.y;
+  }
+  if (lane == 0) cuts[warp] = cut;
+  // row r's partial in piece i: slot 1 of the first CTA, slot 0 of the others
+  auto part = [&](const PagedCut &t, int i, int r) {
+    return ((t.first + i) * 2ll + (i == 0 ? 1 : 0)) * a.p.M + r;
+  };
+  auto add = [&](float4 &acc, float w, long long at) {
+    if (w != 0.f && lane * 4 < hd) {  // an empty piece wrote no outputs
+      const float4 v = __ldcg(reinterpret_cast<const float4 *>(ws.o + at * hd) + lane);
+      acc.x = fmaf(w, v.x, acc.x);
+      acc.y = fmaf(w, v.y, acc.y);
+      acc.z = fmaf(w, v.z, acc.z);
+      acc.w = fmaf(w, v.w, acc.w);
     }
-    mm = warp_max_xor(mm);
-    const float m_use = mm == -INFINITY ? 0.f : mm;
-    float l = 0.f;
-    for (int i = lane; i < n; i += 32) {
-      float w = 0.f;
-      if (from[i] >= 0) {
-        w = exp2f(__ldcg(src(i) + hd) - m_use);
-        l = fmaf(w, __ldcg(src(i) + hd + 1), l);
-      }
-      weight[warp][i] = w;
-    }
-    l = warp_sum_xor(l);
-    __syncwarp();
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};  // hd <= 128: columns lane, lane + 32, ...
+  };
+  if (cut.n > 0 && cut.n <= kJoinFew) {
+    for (int r = blockIdx.y; r < cut.rows; r += gridDim.y) {
+      const float2 ml = lane < cut.n ? __ldcg(ws.ml + part(cut, lane, r)) : make_float2(-INFINITY, 0.f);
+      const float mm = warp_max_xor(ml.x);
+      const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mm);
+      const float l = warp_sum_xor(w * ml.y);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      if (from[i] < 0) continue;
-      const float w = weight[warp][i];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (e * 32 + lane < hd) acc[e] = fmaf(w, __ldcg(src(i) + e * 32 + lane), acc[e]);
-      }
+      for (int i = 0; i < cut.n; ++i) add(acc, __shfl_sync(0xffffffffu, w, i), part(cut, i, r));
+      join_store(a, cut, r, lane, acc, l);
     }
-    __syncwarp();
-    const int tok = (row0 + r) / a.p.n_rep;
-    const int head = at.kvh * a.p.n_rep + (row0 + r) - tok * a.p.n_rep;
-    __nv_bfloat16 *dst = a.out + (static_cast<long long>(s.r0 + tok) * a.p.n_kv * a.p.n_rep + head) * hd;
+  }
+  __syncthreads();
+  for (int k = 0; k < kJoinWarps; ++k) {
+    const PagedCut t = cuts[k];
+    if (t.n <= kJoinFew) continue;
+    for (int r = blockIdx.y; r < t.rows; r += gridDim.y) {
+      // pieces warp * 32 + lane, + 256, ... for the maximum and the sum
+      float mm = -INFINITY;
+      for (int i = tid; i < t.n; i += kJoinThreads) mm = fmaxf(mm, __ldcg(ws.ml + part(t, i, r)).x);
+      mm = warp_max_xor(mm);
+      if (lane == 0) red[0][warp] = mm;
+      __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (e * 32 + lane < hd) dst[e * 32 + lane] = __float2bfloat16(l != 0.f ? acc[e] / l : 0.f);
+      for (int w = 0; w < kJoinWarps; ++w) mm = fmaxf(mm, red[0][w]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.f;
+      for (int i0 = warp * 8; i0 < t.n; i0 += kJoinThreads / 4) {
+        // eight pieces of this warp at a time: their weights in lanes, then their outputs
+        const float2 ml = lane < 8 && i0 + lane < t.n ? __ldcg(ws.ml + part(t, i0 + lane, r)) : make_float2(-INFINITY, 0.f);
+        const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mm);
+        l = fmaf(w, ml.y, l);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) add(acc, __shfl_sync(0xffffffffu, w, i), part(t, min(i0 + i, t.n - 1), r));
+      }
+      l = warp_sum_xor(l);
+      if (lane == 0) red[1][warp] = l;
+      fold[warp][lane] = acc;
+      __syncthreads();
+      if (warp == 0) {
+        l = 0.f;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) {
+          l += red[1][w];
+          const float4 v = fold[w][lane];
+          acc.x += v.x;
+          acc.y += v.y;
+          acc.z += v.z;
+          acc.w += v.w;
+        }
+        join_store(a, t, r, lane, acc, l);
+      }
+      __syncthreads();
     }
   }
 }
 
 struct AttnForm {
-  int M, tile, ctas;
+  int M, tile, extra, ctas;
 };
 // The form of a call: from the head layout and the mean number of new rows per sequence,
 // which the host knows, never from the lengths, which it does not.
-AttnForm form_of(int T, int batch, int n_rep) {
+AttnForm form_of(int T, int batch, int n_rep, int n_kv, int hd, long long cap) {
   const long long rows = (static_cast<long long>(T) + batch - 1) / batch * n_rep;
+  const long long sms = sm_count();
   AttnForm f;
-  f.M = rows <= 16 ? 16 : 32;
+  if (rows > 32 && (hd == 64 || hd == 128)) {
+    f.M = kWideM;
+    f.tile = kWideTile;
+    f.extra = kWideTile;
+    f.ctas = static_cast<int>(sms);  // one resident CTA per SM
+    return f;
+  }
+  f.M = rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
   f.tile = kThinTile;
-  f.ctas = std::min(sm_count(), kMaxCtas);
+  f.extra = kThinTile;
+  // Two resident CTAs per SM, and up to eight in all, so that an SM that is served faster
+  // takes more of them; no more than one for every 512 cache rows the tables can hold.
+  const long long items = (rows + f.M - 1) / f.M * batch * n_kv;
+  const long long want = items * (cap + f.extra) / 512;
+  f.ctas = static_cast<int>(std::min(std::max(want, 2 * sms), 2 * sms));
   return f;
 }
-long long ws_floats_of(const AttnForm &f, int hd) {
-  return static_cast<long long>(f.ctas) * 2 * f.M * (hd + 2);
-}
 
-template <int HD, int MT>
-cudaError_t launch_thin(const PagedAttnArgs &a, int ctas, cudaStream_t st) {
-  static int done[64] = {};
-  if (!ensure_smem_attr(attn_paged_thin_kernel<HD, MT>, ThinLayout<HD, MT>::kBytes, done)) {
-    return cudaErrorInvalidValue;
-  }
-  return launch_chain(attn_paged_thin_kernel<HD, MT>, dim3(static_cast<unsigned>(ctas)), dim3(kThinThreads),
-                      ThinLayout<HD, MT>::kBytes, st, a);
+using TensorMapEncode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                     const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                     CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                     CUtensorMapFloatOOBfill);
+TensorMapEncode tensor_map_encode() {
+  static TensorMapEncode fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+      return static_cast<TensorMapEncode>(nullptr);
+    }
+    return reinterpret_cast<TensorMapEncode>(p);
+  }();
+  return fn;
 }
 
 bool head_dim_ok(int hd) { return hd == 16 || hd == 32 || hd == 64 || hd == 128; }
+
+// The pools as [page][row][kv head][element]; a copy is one head's (up to) 64 elements of
+// `rows` rows of a page, laid out with the swizzle the matrix loads expect.
+bool pool_maps(const PagedCache &c, int rows, CUtensorMap (&maps)[2]) {
+  TensorMapEncode enc = tensor_map_encode();
+  if (enc == nullptr) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.hd), static_cast<cuuint64_t>(c.n_kv),
+                              static_cast<cuuint64_t>(1) << c.page_shift, static_cast<cuuint64_t>(c.n_pages)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(std::min(c.hd, 64)), 1, static_cast<cuuint32_t>(rows), 1};
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
+  const CUtensorMapSwizzle swizzle = c.hd >= 64 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : c.hd == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+  for (int i = 0; i < 2; ++i) {
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(c.hd) * 2, static_cast<cuuint64_t>(c.n_kv) * c.hd * 2,
+                                   static_cast<cuuint64_t>(i == 0 ? c.k_page_stride : c.v_page_stride) * 2};
+    if (enc(&maps[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, i == 0 ? c.k : c.v, dims, strides, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+      return false;
+    }
+  }
+  return true;
+}
+
+template <int HD, int NQ>
+cudaError_t launch_thin(const PagedAttnArgs &a, int ctas, cudaStream_t st) {
+  static int done[64] = {};
+  CUtensorMap maps[2];
+  if (!ensure_smem_attr(attn_paged_thin_kernel<HD, NQ>, ThinLayout<HD, NQ>::kBytes, done) ||
+      !pool_maps(a.c, 16, maps)) {
+    return cudaErrorInvalidValue;
+  }
+  return launch_chain(attn_paged_thin_kernel<HD, NQ>, dim3(static_cast<unsigned>(ctas)), dim3(kThinThreads),
+                      ThinLayout<HD, NQ>::kBytes, st, maps[0], maps[1], a);
+}
+template <int HD>
+cudaError_t launch_thin_hd(const PagedAttnArgs &a, int ctas, cudaStream_t st) {
+  switch (a.p.M) {
+    case 8: return launch_thin<HD, 1>(a, ctas, st);
+    case 16: return launch_thin<HD, 2>(a, ctas, st);
+    default: return launch_thin<HD, 4>(a, ctas, st);
+  }
+}
+
+template <int HD>
+cudaError_t launch_wide(const PagedAttnArgs &a, int negate, int ctas, cudaStream_t st) {
+  static int done[64] = {};
+  CUtensorMap maps[2];
+  if (!ensure_smem_attr(attn_paged_wide_kernel<HD>, WideLayout<HD>::kBytes, done) ||
+      !pool_maps(a.c, std::min(1 << a.c.page_shift, kWideTile), maps)) {
+    return cudaErrorInvalidValue;
+  }
+  return launch_chain(attn_paged_wide_kernel<HD>, dim3(static_cast<unsigned>(ctas)), dim3(kWideThreads),
+                      WideLayout<HD>::kBytes, st, maps[0], maps[1], a, negate);
+}
 
 }  // namespace
 }  // namespace chr
@@ -607,9 +776,13 @@ bool head_dim_ok(int hd) { return hd == 16 || hd == 32 || hd == 64 || hd == 128;
 using namespace chr;
 
 extern "C" int64_t chr_nf4_attn_paged_ws(int32_t T, int32_t batch, int32_t n_q, int32_t n_kv,
-                                         int32_t hd) {
-  if (T < 1 || batch < 1 || n_q < 1 || n_kv < 1 || n_q % n_kv != 0 || !head_dim_ok(hd)) return 0;
-  return ws_floats_of(form_of(T, batch, n_q / n_kv), hd);
+                                         int32_t hd, int64_t cap) {
+  if (T < 1 || batch < 1 || n_q < 1 || n_kv < 1 || n_q % n_kv != 0 || !head_dim_ok(hd) || cap < 1 ||
+      cap > 0x7fffffffll) {
+    return 0;
+  }
+  const AttnForm f = form_of(T, batch, n_q / n_kv, n_kv, hd, cap);
+  return ws_floats_of(f.ctas, f.M, hd);
 }
 
 extern "C" int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, int64_t q_stride,
@@ -626,33 +799,31 @@ extern "C" int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, i
   const int hd = a.c.hd;
   if (T < 1 || n_q < 1 || n_q % a.c.n_kv != 0 || !head_dim_ok(hd) ||
       q_stride < static_cast<int64_t>(n_q) * hd || (tree != nullptr && tree_words < 1) ||
-      (q_start == nullptr && T != a.c.batch) || static_cast<int64_t>(T) * n_q > 0x3fffffffll) {
+      !std::isfinite(scale) || (q_start == nullptr && T != a.c.batch) || static_cast<int64_t>(T) * n_q > 0x3fffffffll) {
     return kDims;
   }
-  if (!aligned(q, 16) || !aligned(out, 16) || q_stride % 8 != 0 || !aligned(a.c.k, 16) ||
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(ws, 16) || q_stride % 8 != 0 || !aligned(a.c.k, 16) ||
       !aligned(a.c.v, 16) || a.c.k_page_stride % 8 != 0 || a.c.v_page_stride % 8 != 0 ||
       (tree != nullptr && !aligned(tree, 8))) {
     return kAlign;
   }
   const int n_rep = n_q / a.c.n_kv;
-  const AttnForm f = form_of(T, a.c.batch, n_rep);
-  if (ws_floats < ws_floats_of(f, hd)) return kWorkspace;
+  a.p.cap = static_cast<int>(static_cast<long long>(a.c.max_pages) << a.c.page_shift);
+  const AttnForm f = form_of(T, a.c.batch, n_rep, a.c.n_kv, hd, a.p.cap);
+  if (ws_floats < ws_floats_of(f.ctas, f.M, hd)) return kWorkspace;
   a.p.q_start = static_cast<const int32_t *>(q_start);
   a.p.kv_len = static_cast<const int32_t *>(kv_len);
   a.p.T = T;
   a.p.batch = a.c.batch;
   a.p.n_kv = a.c.n_kv;
   a.p.n_rep = n_rep;
-  a.p.cap = static_cast<int>(static_cast<long long>(a.c.max_pages) << a.c.page_shift);
   a.p.M = f.M;
   a.p.tile = f.tile;
+  a.p.extra = f.extra;
   a.p.causal = tree == nullptr;
-  // the split's arithmetic is in 64-bit integers: total axis length x CTAs
+  // the axis is measured in 64-bit integers that binary64 holds exactly
   const double items = static_cast<double>(T) * n_q / f.M + static_cast<double>(a.c.batch) * a.c.n_kv;
-  if (items * a.p.cap * n_rep * f.ctas > 4.0e18 ||
-      static_cast<double>(a.p.cap) * n_rep * (a.p.cap / f.tile + 1.0) > 4.0e18) {
-    return kDims;
-  }
+  if (items * (static_cast<double>(a.p.cap) + f.extra) * n_rep > 4.0e15) return kDims;
   a.q = static_cast<const __nv_bfloat16 *>(q);
   a.out = static_cast<__nv_bfloat16 *>(out);
   a.tree = static_cast<const unsigned long long *>(tree);
@@ -663,19 +834,34 @@ extern "C" int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, i
   a.c2 = scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-#define CHR_THIN(HD)                                                   \
-  e = f.M == 16 ? launch_thin<HD, 1>(a, f.ctas, st) : launch_thin<HD, 2>(a, f.ctas, st)
-  switch (hd) {
-    case 16: CHR_THIN(16); break;
-    case 32: CHR_THIN(32); break;
-    case 64: CHR_THIN(64); break;
-    default: CHR_THIN(128); break;
+  if (f.M == kWideM) {
+    // the sign of the scale goes into the product, so that the maximum of the products is
+    // that of the scores; no scale at all would make a hidden row 0 x -inf
+    a.c2 = std::max(std::fabs(a.c2), 1e-30f);
+    const int negate = scale < 0.f;
+    e = hd == 64 ? launch_wide<64>(a, negate, f.ctas, st) : launch_wide<128>(a, negate, f.ctas, st);
+  } else {
+    switch (hd) {
+      case 16: e = launch_thin_hd<16>(a, f.ctas, st); break;
+      case 32: e = launch_thin_hd<32>(a, f.ctas, st); break;
+      case 64: e = launch_thin_hd<64>(a, f.ctas, st); break;
+      default: e = launch_thin_hd<128>(a, f.ctas, st); break;
+    }
   }
-#undef CHR_THIN
   if (e != cudaSuccess) return kLaunch;
-  if (f.ctas > 1) {
-    e = launch_chain(attn_paged_join_kernel, dim3(static_cast<unsigned>(f.ctas - 1)), dim3(kJoinThreads),
-                     0, st, a, f.ctas);
-  }
+  e = launch_chain(attn_paged_join_kernel,
+                   dim3(static_cast<unsigned>((f.ctas + kJoinWarps - 1) / kJoinWarps), f.M == kWideM ? 64 : 8),
+                   dim3(kJoinThreads), 0, st, a, f.ctas);
   return e == cudaSuccess ? kOk : kLaunch;
+}
+
+extern "C" int chr_nf4_attn_paged_status(void) {
+  int v = 0;
+  const int zero = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess ||
+      cudaMemcpyFromSymbol(&v, g_attn_paged_status, sizeof v) != cudaSuccess ||
+      cudaMemcpyToSymbol(g_attn_paged_status, &zero, sizeof zero) != cudaSuccess) {
+    return kLaunch;
+  }
+  return v;
 }

@@ -1,0 +1,489 @@
+// The wide form of the paged attention (paged_attn.cu): items of up to 256 query rows on the
+// fifth-generation tensor cores, for head dims 64 and 128.
+//
+// One CTA per SM holds two query tiles of 128 rows against one key / value stream of
+// 128-row tiles, so that a cache row crosses from L2 once per 256 query rows (two CTAs of
+// 128 rows each would need 64 bytes per clock and SM, more than L2 delivers to all SMs).
+//   warp 9      page look-up and TMA copies of K and V pages (two stages each)
+//   warp 8      issues tcgen05.mma: S_w = Q_w K^T (128 x 128, FP32, tensor memory) and
+//               O_w += P_w V, P_w read from tensor memory, where it lies over S_w
+//   warps 0-3   softmax of tile 0, warps 4-7 of tile 1: a thread owns a row
+// The order of issue is QK0(i) PV1(i-1) QK1(i) PV0(i): while one tile's softmax runs the
+// other's products do. Both sides need about 2048 clocks per key tile (4 products of
+// 128^3 at 4096 multiply-adds a clock; 32768 exp2 at 16 a clock), so overlap is what
+// counts. The running maximum a row subtracts is raised only when the new one is more than 8
+// (in log2) above it: P then stays below 2^8, which bf16 holds as exactly as 1, and the
+// accumulator in tensor memory is almost never rescaled.
+// P is rounded to bf16 for the second product, its sum is not; everything else is FP32.
+//
+// Every wait is bounded; one that runs out leaves a code in a status word
+// (chr_nf4_attn_paged_status), the roles stop, copies in flight are waited for and the
+// tensor memory is freed.
+
+#pragma once
+
+#include "paged.cuh"
+#include "tma_tc.cuh"
+
+namespace chr {
+namespace {
+
+constexpr int kWideThreads = 320;
+constexpr int kWideM = 256;
+constexpr int kWideTile = 128;
+
+template <int HD>
+struct WideLayout {
+  static constexpr int kHalves = HD / 64;                   // 128-byte wide pieces of a row
+  static constexpr int kPiece = 128 * 128;                  // 128 rows x 128 bytes
+  static constexpr int kTileB = kHalves * kPiece;           // one 128-row tile
+  static constexpr int kQ = 0;                              // two query tiles
+  static constexpr int kK = 2 * kTileB;                     // two stages
+  static constexpr int kV = 4 * kTileB;                     // two stages
+  static constexpr int kBars = 6 * kTileB;
+  static constexpr int kSegOff = kBars + 256;
+  static constexpr int kBytes = kSegOff + kSegs * static_cast<int>(sizeof(Seg)) + 1024;
+};
+
+struct WideBars {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], v_fixed[2];
+  uint64_t s_full[2], p_full[2], pv_done[2], q_full[2];
+  uint32_t bad[4];  // pages of the last tiles that are none, a bit per page
+  uint32_t tmem;
+  int fail;
+};
+
+// False when the phase did not complete within the poll limit, or another role gave up.
+__device__ __forceinline__ bool bar_wait(WideBars &w, uint64_t *b, uint32_t parity, int who) {
+  const uint32_t addr = smem_u32(b);
+  for (uint32_t i = 0; i < kPolls; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((i & 255u) == 255u && *reinterpret_cast<volatile int *>(&w.fail) != 0) return false;
+  }
+  *reinterpret_cast<volatile int *>(&w.fail) = 1;
+  atomicExch(&g_attn_paged_status, who);
+  return false;
+}
+
+// Which of the 32 cache rows k0 .. k0+31 a token's row sees.
+__device__ __forceinline__ uint32_t seen32(const PagedAttnArgs &a, const Seg &g, int token, int k0) {
+  const int older = g.base - k0;  // rows before this one are older than the new rows
+  uint32_t m;
+  if (a.tree == nullptr) {
+    const int n = older + token + 1;
+    m = n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << n) - 1u);
+  } else if (older >= 32) {
+    m = 0xFFFFFFFFu;
+  } else {
+    const unsigned long long *w = a.tree + static_cast<long long>(g.r0 + token) * a.tree_words;
+    const int d0 = -older;
+    if (d0 >= 0) {
+      const int i = d0 >> 6, sh = d0 & 63;
+      unsigned long long v = i < a.tree_words ? __ldg(w + i) >> sh : 0ull;
+      if (sh > 32 && i + 1 < a.tree_words) v |= __ldg(w + i + 1) << (64 - sh);
+      m = static_cast<uint32_t>(v);
+    } else {
+      m = (static_cast<uint32_t>(__ldg(w)) << older) | ((1u << older) - 1u);
+    }
+  }
+  const int n = g.kv_end - k0;
+  if (n < 32) m &= n <= 0 ? 0u : (1u << n) - 1u;
+  return m;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kWideThreads, 1)
+attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                       const PagedAttnArgs a, const int negate) {
+  using L = WideLayout<HD>;
+  extern __shared__ __align__(16) unsigned char wide_smem[];
+  const uint32_t raw = smem_u32(wide_smem);
+  unsigned char *sm = wide_smem + (((raw + 1023u) & ~1023u) - raw);
+  const uint32_t base = smem_u32(sm);
+  WideBars &w = *reinterpret_cast<WideBars *>(sm + L::kBars);
+  Seg *segs = reinterpret_cast<Seg *>(sm + L::kSegOff);
+  __shared__ int n_segs;
+  __shared__ SegWalk walk;  // thread 0's: not worth the registers of a thread
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int G = gridDim.x, cta = blockIdx.x;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&w.k_full[i], 1);
+      bar_init(&w.k_empty[i], 1);
+      bar_init(&w.v_full[i], 1);
+      bar_init(&w.v_empty[i], 1);
+      bar_init(&w.s_full[i], 1);
+      bar_init(&w.p_full[i], 128);
+      bar_init(&w.pv_done[i], 1);
+      bar_init(&w.q_full[i], 128);
+      bar_init(&w.v_fixed[i], 1);
+    }
+    w.fail = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&k_map);
+    prefetch_map(&v_map);
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&w.tmem)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = w.tmem;
+
+  pdl_wait();
+  pdl_trigger();
+  if (warp == 0) {
+    if (lane == 0) ws_of(a, G).cut[cta].n = 0;
+    const bool some = walk_start(a.p, walk, cta, G);
+    if (lane == 0) n_segs = some ? walk_fill(a, walk, cta, G, segs) : 0;
+  }
+  zero_tail_rows<HD>(a, cta, G);
+  __syncthreads();
+
+  const int shift = a.c.page_shift;
+  const int box = min(1 << shift, kWideTile);  // rows of one copy
+  const int boxes = kWideTile / box;
+
+  // counts that run over all segments, each role's own
+  uint32_t n_kv = 0;          // key tiles (copies, products)
+  uint32_t n_k = 0, n_v = 0;  // copy role: tiles requested
+  uint32_t fixed = 0;         // product role: parity of each stage's zeroed tails
+  uint32_t n_q[2] = {0, 0};   // segments a query tile took part in
+  uint32_t n_s = 0;           // softmax role: its tiles
+  uint32_t n_p[2] = {0, 0};   // product role: P tiles consumed
+
+  for (int n_now = n_segs; n_now != 0;) {
+    bool ok = true;
+
+    if (warp == 9) {
+      // ---------------- copies ----------------
+      for (int si = 0; si < n_now && ok; ++si) {
+        const Seg g = segs[si];
+        const int32_t *table = a.c.table + g.b * a.c.table_stride;
+        for (int t = g.t0; t < g.t1 && ok; ++t, ++n_kv) {
+          const int st = n_kv & 1;
+          const uint32_t ph = (n_kv >> 1) & 1;
+          // a page per lane; one past the item's rows, or that is none, is read as zeros
+          const int row = t * kWideTile + lane * box;
+          int id = a.c.n_pages;
+          bool none = false;
+          if (lane < boxes && row < g.kv_end) {
+            id = __ldg(table + (row >> shift));
+            none = id < 0 || id >= a.c.n_pages;
+            if (none) id = a.c.n_pages;
+          }
+          const uint32_t bad = __ballot_sync(0xffffffffu, none);
+          const int in_page = row & ((1 << shift) - 1);
+          if (n_kv >= 2) ok = bar_wait(w, &w.k_empty[st], ph ^ 1, 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) {
+            *reinterpret_cast<volatile uint32_t *>(&w.bad[n_kv & 3]) = bad;
+            bar_expect(&w.k_full[st], L::kTileB);
+          }
+          ++n_k;
+          __syncwarp();
+          if (lane < boxes) {
+#pragma unroll
+            for (int h = 0; h < L::kHalves; ++h) {
+              tma_page(base + L::kK + st * L::kTileB + h * L::kPiece + lane * box * 128, &k_map, &w.k_full[st], h * 64,
+                       g.kvh, in_page, id);
+            }
+          }
+          if (n_kv >= 2) ok = bar_wait(w, &w.v_empty[st], ph ^ 1, 2);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) bar_expect(&w.v_full[st], L::kTileB);
+          ++n_v;
+          __syncwarp();
+          if (lane < boxes) {
+#pragma unroll
+            for (int h = 0; h < L::kHalves; ++h) {
+              tma_page(base + L::kV + st * L::kTileB + h * L::kPiece + lane * box * 128, &v_map, &w.v_full[st], h * 64,
+                       g.kvh, in_page, id);
+            }
+          }
+          if ((t + 1) * kWideTile > g.kv_end) {
+            // rows behind the last may hold anything (0 x NaN): zeros for the second product
+            ok = __all_sync(0xffffffffu, bar_wait(w, &w.v_full[st], ph, 3));
+            if (!ok) break;
+            const int first = max(g.kv_end - t * kWideTile, 0);
+            for (int i = lane; i < (kWideTile - first) * 8 * L::kHalves; i += 32) {
+              const int r = first + (i >> 3) / L::kHalves, h = (i >> 3) % L::kHalves;
+              *reinterpret_cast<uint4 *>(sm + L::kV + st * L::kTileB + h * L::kPiece + r * 128 + (i & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(&w.v_fixed[st]);
+          }
+        }
+      }
+      if (!ok) {
+        // a role gave up: the copies in flight land before the CTA leaves
+        for (uint32_t i = n_k >= 2 ? n_k - 2 : 0; i < n_k; ++i) bar_poll(&w.k_full[i & 1], (i >> 1) & 1);
+        for (uint32_t i = n_v >= 2 ? n_v - 2 : 0; i < n_v; ++i) bar_poll(&w.v_full[i & 1], (i >> 1) & 1);
+      }
+    } else if (warp == 8) {
+      // ---------------- products ----------------
+      if (lane == 0) {
+        const uint32_t qk_desc = (1u << 4) | (1u << 7) | (1u << 10) | (negate ? 1u << 13 : 0u) |
+                                 (static_cast<uint32_t>(kWideTile >> 3) << 17) | (128u >> 4 << 24);
+        const uint32_t pv_desc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
+                                 (static_cast<uint32_t>(HD >> 3) << 17) | (128u >> 4 << 24);
+        auto qk = [&](int tile, int st) {
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t off = (ks >> 2) * L::kPiece + (ks & 3) * 32;
+            tc_mma_ss(tmem + tile * 128, tc_desc(base + L::kQ + tile * L::kTileB + off, 16),
+                      tc_desc(base + L::kK + st * L::kTileB + off, 16), qk_desc, ks > 0 ? 1u : 0u);
+          }
+          tc_commit(&w.s_full[tile]);
+        };
+        auto pv = [&](int tile, int st, bool first) {
+#pragma unroll
+          for (int ks = 0; ks < kWideTile / 16; ++ks) {
+            tc_mma_ts(tmem + 256 + tile * 128, tmem + tile * 128 + ks * 8,
+                      tc_desc(base + L::kV + st * L::kTileB + ks * 16 * 128, L::kPiece), pv_desc,
+                      (!first || ks > 0) ? 1u : 0u);
+          }
+          tc_commit(&w.pv_done[tile]);
+        };
+        auto wait_p = [&](int tile) {
+          ok = ok && bar_wait(w, &w.p_full[tile], n_p[tile] & 1, 4);
+          ++n_p[tile];
+          tc_fence_after();
+        };
+        for (int si = 0; si < n_now && ok; ++si) {
+          const int t0 = segs[si].t0, t1 = segs[si].t1, kv_end = segs[si].kv_end;
+          const bool two = segs[si].rows > 128;
+          for (int t = t0; t < t1 && ok; ++t, ++n_kv) {
+            const int st = n_kv & 1;
+            const uint32_t ph = (n_kv >> 1) & 1;
+            if (t == t0) ok = bar_wait(w, &w.q_full[0], n_q[0]++ & 1, 5);
+            ok = ok && bar_wait(w, &w.k_full[st], ph, 6);
+            if (!ok) break;
+            tc_fence_after();
+            qk(0, st);
+            if (two) {
+              if (t > t0) {
+                wait_p(1);
+                if (!ok) break;
+                pv(1, st ^ 1, t == t0 + 1);
+                tc_commit(&w.v_empty[st ^ 1]);
+              } else {
+                ok = bar_wait(w, &w.q_full[1], n_q[1]++ & 1, 5);
+                if (!ok) break;
+                tc_fence_after();
+              }
+              qk(1, st);
+            }
+            tc_commit(&w.k_empty[st]);
+            ok = bar_wait(w, &w.v_full[st], ph, 7);
+            if (ok && (t + 1) * kWideTile > kv_end) {
+              ok = bar_wait(w, &w.v_fixed[st], (fixed >> st) & 1u, 8);
+              fixed ^= 1u << st;
+            }
+            if (!ok) break;
+            wait_p(0);
+            if (!ok) break;
+            pv(0, st, t == t0);
+            if (!two) tc_commit(&w.v_empty[st]);
+          }
+          if (ok && two) {
+            wait_p(1);
+            if (!ok) break;
+            const int st = (n_kv - 1) & 1;
+            pv(1, st, t1 == t0 + 1);
+            tc_commit(&w.v_empty[st]);
+          }
+        }
+      }
+      __syncwarp();
+    } else {
+      // ---------------- softmax: a thread per query row ----------------
+      const int tile = warp >> 2;
+      const int r = tid & 127;  // row of the tile, and lane of tensor memory
+      const uint32_t quad = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t s_addr = tmem + quad + tile * 128;
+      const uint32_t o_addr = tmem + quad + 256 + tile * 128;
+      uint32_t seg_tiles = 0;  // key tiles of this batch before the segment
+      for (int si = 0; si < n_now && ok; ++si) {
+        const Seg g = segs[si];
+        const int first_row = tile * 128;
+        const uint32_t tiles_before = seg_tiles;
+        seg_tiles += g.t1 - g.t0;
+        if (g.rows <= first_row) continue;
+        // the item's queries, K-major with the 128-byte swizzle, zeros past the last row
+        {
+          constexpr int C = HD / 8;
+#pragma unroll 4
+          for (int i = r; i < 128 * C; i += 128) {
+            const int qr = i / C, c = i % C;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (first_row + qr < g.rows) {
+              const int x = g.row0 + first_row + qr;
+              const int token = x / a.p.n_rep;
+              const int head = g.kvh * a.p.n_rep + x - token * a.p.n_rep;
+              v = ld_act16(a.q + (g.r0 + token) * a.q_stride + head * HD + c * 8);
+            }
+            *reinterpret_cast<uint4 *>(sm + L::kQ + tile * L::kTileB + (c >> 3) * L::kPiece + qr * 128 +
+                                       (((c & 7) ^ (qr & 7)) << 4)) = v;
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          bar_arrive(&w.q_full[tile]);
+        }
+        const bool mine = first_row + r < g.rows;
+        const int x = g.row0 + first_row + r;
+        const int token = mine ? x / a.p.n_rep : 0;
+        float m_run = -INFINITY, l_run = 0.f;
+        const float c2 = a.c2;
+
+        for (int t = g.t0; t < g.t1; ++t) {
+          ok = __all_sync(0xffffffffu, bar_wait(w, &w.s_full[tile], n_s & 1, 9));
+          if (!ok) break;
+          tc_fence_after();
+          uint32_t s[128];
+          tmem_ld32(s_addr, s);
+          tmem_ld32(s_addr + 32, s + 32);
+          tmem_ld32(s_addr + 64, s + 64);
+          tmem_ld32(s_addr + 96, s + 96);
+          tmem_wait_ld();
+          const uint32_t bad =
+              *reinterpret_cast<volatile uint32_t *>(&w.bad[(n_kv + tiles_before + (t - g.t0)) & 3]);
+          if ((t + 1) * kWideTile > g.base || bad != 0u) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t m = seen32(a, g, token, t * kWideTile + k * 32);
+              if (bad != 0u) {
+                for (int i = 0; i < 32; ++i) {
+                  if ((bad >> ((k * 32 + i) / box)) & 1u) m &= ~(1u << i);
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                if (!((m >> e) & 1u)) s[k * 32 + e] = 0xFF800000u;  // -inf
+              }
+            }
+          }
+          float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < 128; e += 4) {
+            mx0 = fmaxf(mx0, __uint_as_float(s[e]));
+            mx1 = fmaxf(mx1, __uint_as_float(s[e + 1]));
+            mx2 = fmaxf(mx2, __uint_as_float(s[e + 2]));
+            mx3 = fmaxf(mx3, __uint_as_float(s[e + 3]));
+          }
+          const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c2;
+          // raise the subtracted maximum only when it is far behind
+          const bool raise = mx > m_run + 8.f || m_run == -INFINITY;
+          const float m_new = raise ? fmaxf(mx, m_run) : m_run;
+          const float alpha = raise ? (m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new)) : 1.f;
+          const bool turn_down = raise && m_run != -INFINITY;
+          m_run = m_new;
+          const float m_use = m_new == -INFINITY ? 0.f : m_new;
+          const f32x2_t c22 = pack_f32x2(c2, c2), mm2 = pack_f32x2(-m_use, -m_use);
+          float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+          for (int e = 0; e < 128; e += 2) {
+            float p0, p1;
+            unpack_f32x2(ffma2(pack_f32x2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c22, mm2), p0, p1);
+            p0 = fast_exp2(p0);
+            p1 = fast_exp2(p1);
+            sum0 += p0;
+            sum1 += p1;
+            const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);
+            s[e >> 1] = *reinterpret_cast<const uint32_t *>(&v);
+          }
+          l_run = fmaf(l_run, alpha, sum0 + sum1);
+          tmem_st32(s_addr, s);
+          tmem_st32(s_addr + 32, s + 32);
+          if (__any_sync(0xffffffffu, turn_down)) {
+            // the accumulator is this thread's once the last product into it is done
+            ok = __all_sync(0xffffffffu, bar_wait(w, &w.pv_done[tile], (n_s & 1) ^ 1, 10));
+            if (!ok) break;
+            tc_fence_after();
+            const float by = turn_down ? alpha : 1.f;
+#pragma unroll
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_addr + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
+              tmem_st32(o_addr + c, o);
+            }
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          bar_arrive(&w.p_full[tile]);
+          ++n_s;
+        }
+        if (!ok) break;
+        // ---- the segment's result ----
+        ok = __all_sync(0xffffffffu, bar_wait(w, &w.pv_done[tile], (n_s & 1) ^ 1, 11));
+        if (!ok) break;
+        tc_fence_after();
+        const bool whole = g.whole;
+        const int head = g.kvh * a.p.n_rep + x - token * a.p.n_rep;
+        const float by = l_run != 0.f ? 1.f / l_run : 0.f;
+        const PagedWs ws = ws_of(a, G);
+        const long long at = (static_cast<long long>(cta) * 2 + g.slot) * kWideM + first_row + r;
+        float *part = ws.o + at * HD;
+        __nv_bfloat16 *dst = a.out + (static_cast<long long>(g.r0 + token) * a.p.n_kv * a.p.n_rep + head) * HD;
+#pragma unroll
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + c, o);
+          tmem_wait_ld();
+          if (mine && whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint32_t v[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(o[e + 2 * i]) * by,
+                                                               __uint_as_float(o[e + 2 * i + 1]) * by);
+                v[i] = *reinterpret_cast<const uint32_t *>(&y);
+              }
+              *reinterpret_cast<uint4 *>(dst + c + e) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          } else if (mine) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              *reinterpret_cast<uint4 *>(part + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+          }
+        }
+        if (mine && !whole) ws.ml[at] = make_float2(m_run, l_run);
+        tc_fence_before();
+      }
+      n_kv += seg_tiles;
+    }
+    __syncthreads();
+    if (tid == 0) n_segs = w.fail != 0 ? 0 : walk_fill(a, walk, cta, G, segs);
+    __syncthreads();
+    n_now = n_segs;
+    __syncthreads();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+}  // namespace
+}  // namespace chr

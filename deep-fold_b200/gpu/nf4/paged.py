@@ -13,7 +13,7 @@ follows what the tensors hold at replay.
 
 from __future__ import annotations
 
-import ctypes
+import functools
 
 import torch
 
@@ -34,15 +34,22 @@ def _fail(msg: str):
     raise RuntimeError(msg)
 
 
+# The host's share of a small call is longer than the kernel's: the raw forms of "current device"
+# and "current stream" take a tenth of what the public ones do.
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(name: str, device: torch.device, *args) -> None:
     """``name(*args, stream)`` with ``device`` current, on its current stream."""
     index = device.index
     fn = getattr(_lib.load(), name)
-    if index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*args, _raw_stream(index))
     if rc != 0:
         _lib.check(rc, name)
 
@@ -230,7 +237,7 @@ def nf4_attn_paged(
         zero = 1
     elif out.dtype is not _BF16 or out.device != device or out.numel() != rows * n_q * hd or not out.is_contiguous():
         _fail(f"out must be contiguous bfloat16 [{rows}, {n_q * hd}] on {device}")
-    need = _ws_floats(device, rows, batch, n_q, pages.n_kv, hd)
+    need = _ws_floats(device.index, rows, batch, n_q, pages.n_kv, hd, pages.max_pages * pages.page)
     ws = torch.empty(need, dtype=_F32, device=device)
     _call("chr_nf4_attn_paged", device, pages, q.data_ptr(), qs, out.data_ptr(),
           _vector(q_start, batch + 1, device, _I32, "q_start"), _vector(kv_len, batch, device, _I32, "kv_len"),
@@ -238,12 +245,10 @@ def nf4_attn_paged(
     return out
 
 
-def _ws_floats(device: torch.device, rows: int, batch: int, n_q: int, n_kv: int, hd: int) -> int:
-    fn = _lib.load().chr_nf4_attn_paged_ws
-    if device.index == torch.cuda.current_device():
-        return fn(rows, batch, n_q, n_kv, hd)
-    with torch.cuda.device(device):
-        return fn(rows, batch, n_q, n_kv, hd)
+@functools.lru_cache(maxsize=4096)
+def _ws_floats(index: int, rows: int, batch: int, n_q: int, n_kv: int, hd: int, cap: int) -> int:
+    with torch.cuda.device(index):
+        return int(_lib.load().chr_nf4_attn_paged_ws(rows, batch, n_q, n_kv, hd, cap))
 
 
 def nf4_sample_commit_batch(

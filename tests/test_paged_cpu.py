@@ -72,9 +72,10 @@ def test_append_refusals(kw, rc):
 
 @pytest.mark.parametrize("kw,rc", [(dict(q=None), -1), (dict(out=None), -1), (dict(kv=None), -1), (dict(ws=None), -1),
                                    (dict(T=0), -3), (dict(n_q=0), -3), (dict(n_q=7), -3), (dict(qs=511), -3),
-                                   (dict(tree=P), -3), (dict(q_start=None), -3), (dict(T=1 << 30), -3),
+                                   (dict(tree=P), -3), (dict(scale=float("nan")), -3),
+                                   (dict(scale=float("inf")), -3), (dict(q_start=None), -3), (dict(T=1 << 30), -3),
                                    (dict(q=ctypes.c_void_p(4098)), -5), (dict(out=ctypes.c_void_p(4104)), -5),
-                                   (dict(qs=516), -5), (dict(tree=ctypes.c_void_p(4100), words=1), -5), (dict(floats=0), -7)])
+                                   (dict(qs=516), -5), (dict(ws=ctypes.c_void_p(4104)), -5), (dict(tree=ctypes.c_void_p(4100), words=1), -5), (dict(floats=0), -7)])
 def test_attention_refusals(kw, rc):
     assert _attn(**kw) == rc
 
@@ -93,8 +94,9 @@ def test_workspace_query_answers_zero_for_what_the_call_refuses():
     from gpu.nf4 import _lib
 
     ws = _lib.load().chr_nf4_attn_paged_ws
-    assert ws(3, 2, 8, 2, 64) > 0
-    for bad in ((0, 2, 8, 2, 64), (3, 0, 8, 2, 64), (3, 2, 7, 2, 64), (3, 2, 8, 0, 64), (3, 2, 8, 2, 48)):
+    assert ws(3, 2, 8, 2, 64, 64) > 0
+    for bad in ((0, 2, 8, 2, 64, 64), (3, 0, 8, 2, 64, 64), (3, 2, 7, 2, 64, 64), (3, 2, 8, 0, 64, 64), (3, 2, 8, 2, 48, 64),
+                (3, 2, 8, 2, 64, 0), (3, 2, 8, 2, 64, 1 << 31)):
         assert ws(*bad) == 0
 
 

@@ -292,3 +292,50 @@ def test_attention_captured_follows_what_the_tensors_hold():
     torch.cuda.synchronize()
     assert torch.equal(out, call(None))
     assert torch.equal(out, call(None))  # and every run gives the same bits
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-3])
+@pytest.mark.parametrize("rows,kv", [([1, 1], [130, 40]), ([50, 33], [300, 33])])
+def test_scales_of_either_sign_and_none(scale, rows, kv):
+    gen = _gen(17)
+    kp, vp, table = ref.make_cache(2, kv, 16, 2, 128, gen)
+    q = torch.randn((sum(rows), 6, 128), generator=gen, device="cuda").to(BF16)
+    _check(q, kp, vp, table, kv, _starts(rows), scale)
+
+
+@pytest.mark.parametrize("n_q,n_kv,hd", [(10, 2, 128), (8, 2, 64), (16, 1, 128), (3, 3, 64)])
+@pytest.mark.parametrize("rows,kv,page", [([52, 51], [700, 51], 256), ([103, 40, 0, 77], [1031, 400, 9, 77], 32),
+                                          ([300], [1300], 512), ([26, 25, 27], [90, 129, 128], 16)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_wide_items(n_q, n_kv, hd, rows, kv, page, tree):
+    """Items of one and of two query tiles, pages longer and shorter than a tile, strided pools."""
+    from gpu.nf4 import _lib
+
+    gen = _gen(sum(rows) * 3 + n_q)
+    kp, vp, table = ref.make_cache(len(kv), kv, page, n_kv, hd, gen, strided=True)
+    q = (2 * torch.randn((sum(rows), n_q, hd), generator=gen, device="cuda")).to(BF16)
+    bits = _tree_bits(rows, 5, gen, empty={1, 40}) if tree else None
+    _check(q, kp, vp, table, kv, _starts(rows), hd ** -0.5, bits)
+    assert _lib.load().chr_nf4_attn_paged_status() == 0
+
+
+def test_wide_rows_whose_maximum_keeps_rising():
+    """Scores that grow along the cache by far more than the slack of the subtracted maximum."""
+    gen = _gen(18)
+    kv, rows = [1500], [60]
+    kp, vp, table = ref.make_cache(1, kv, 16, 2, 128, gen)
+    ramp = torch.linspace(0, 6, 1500, device="cuda")
+    for a in range(1500):
+        kp[int(table[0, a // 16]), a % 16] = (kp[int(table[0, a // 16]), a % 16].float() * 0.2 + ramp[a]).to(BF16)
+    q = torch.rand((60, 8, 128), generator=gen, device="cuda").to(BF16)
+    _check(q, kp, vp, table, kv, _starts(rows), 0.3)
+
+
+def test_wide_missing_pages_and_more_rows_than_cache_rows():
+    gen = _gen(19)
+    kv, rows = [300, 30], [40, 50]
+    kp, vp, table = ref.make_cache(2, kv, 16, 2, 64, gen)
+    table[0, 2], table[0, 17], table[1, 0] = -1, kp.shape[0], 1 << 30
+    q = torch.randn((90, 8, 64), generator=gen, device="cuda").to(BF16)
+    got = _check(q, kp, vp, table, kv, _starts(rows), 0.125)
+    assert not got[40:60].any() and got[79].any()
