@@ -63,6 +63,7 @@ struct PagedRows {
   int T, batch, n_kv, n_rep, cap;
   int M, tile, extra;      // rows of an item, cache rows of a tile, an item's own cost
   int causal;
+  float per_rep;           // 1 / n_rep
 };
 
 struct PagedSeq {
@@ -158,6 +159,7 @@ struct Seg {
   int b, kvh, row0, rows;   // the item's rows among the sequence's R
   int r0, base, len, kv_end;
   int t0, t1, whole, slot;  // whole: no border cuts it; slot: which of the CTA's partials else
+  int tok0, rem0;           // token and head (of the group) of row0
 };
 constexpr int kSegs = 32;   // segments described at a time
 
@@ -176,12 +178,24 @@ struct SegWalk {
   PagedAxis axis;
 };
 
-// Called by a whole warp; false: nothing to do for CTA c.
-__device__ __forceinline__ bool walk_start(const PagedRows &p, SegWalk &w, int c, int ctas) {
+// Token of the sequence that row r of a segment's item belongs to, and the query head. With
+// x = rem0 + r < n_rep + 256 the quotient is exact: (x + 1/2) / n_rep is at least 1 / (2 n_rep)
+// from an integer, its rounding below x 2^-22 / n_rep.
+__device__ __forceinline__ int token_of(const PagedRows &p, const Seg &g, int r) {
+  return g.tok0 + __float2int_rz((static_cast<float>(g.rem0 + r) + 0.5f) * p.per_rep);
+}
+__device__ __forceinline__ int head_of(const PagedRows &p, const Seg &g, int r, int token) {
+  return g.kvh * p.n_rep + g.rem0 + r - (token - g.tok0) * p.n_rep;
+}
+
+// Called by a whole warp; false: nothing to do for CTA c. The walk's functions run once or
+// a few times per CTA: as calls, they leave the instruction cache to the loops.
+static __device__ __noinline__ bool walk_start(const PagedRows &p, SegWalk &w, int c, int ctas) {
   const int lane = threadIdx.x & 31;
   const int per = (p.batch + 31) / 32;
   const int b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
   long long mine = 0;
+#pragma unroll 4
   for (int i = b0; i < b1; ++i) mine += paged_seq_cost(p, paged_seq(p, i));
   long long incl = mine;
 #pragma unroll
@@ -236,6 +250,8 @@ __device__ __forceinline__ void walk_next(const PagedRows &p, SegWalk &w, int c,
   g.b = w.b;
   g.kvh = w.kvh;
   g.row0 = w.j * p.M;
+  g.tok0 = g.row0 / p.n_rep;
+  g.rem0 = g.row0 - g.tok0 * p.n_rep;
   g.rows = min(p.M, w.s.R - g.row0);
   g.r0 = w.s.r0;
   g.base = w.s.base;

@@ -70,7 +70,7 @@ __device__ __forceinline__ PagedWs ws_of(const PagedAttnArgs &a, int ctas) {
 // Describes up to kSegs segments of CTA c's piece from the walk's place on: their number.
 // One thread. An empty piece of a cut item is noted as such, and so is a cut item that
 // starts in the piece (at most its last).
-__device__ __forceinline__ int walk_fill(const PagedAttnArgs &a, SegWalk &w, int c, int ctas, Seg *segs) {
+__device__ __noinline__ int walk_fill(const PagedAttnArgs &a, SegWalk &w, int c, int ctas, Seg *segs) {
   int n = 0;
   PagedCut cut;
   cut.n = 0;
@@ -88,6 +88,31 @@ __device__ __forceinline__ int walk_fill(const PagedAttnArgs &a, SegWalk &w, int
   }
   if (cut.n != 0) ws.cut[c] = cut;
   return n;
+}
+
+// Which of the 32 cache rows that begin `older` rows before the new ones a drafted row sees.
+__device__ __noinline__ uint32_t tree32(const unsigned long long *w, int words, int older) {
+  if (older >= 32) return 0xFFFFFFFFu;
+  const int d0 = -older;
+  if (d0 < 0) return (static_cast<uint32_t>(__ldg(w)) << older) | ((1u << older) - 1u);
+  const int i = d0 >> 6, sh = d0 & 63;
+  unsigned long long v = i < words ? __ldg(w + i) >> sh : 0ull;
+  if (sh > 32 && i + 1 < words) v |= __ldg(w + i + 1) << (64 - sh);
+  return static_cast<uint32_t>(v);
+}
+// Which of the 32 cache rows k0 .. k0+31 a token's row sees.
+__device__ __forceinline__ uint32_t seen32(const PagedAttnArgs &a, const Seg &g, int token, int k0) {
+  const int older = g.base - k0;
+  uint32_t m;
+  if (a.tree == nullptr) {
+    const int n = older + token + 1;
+    m = n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << n) - 1u);
+  } else {
+    m = tree32(a.tree + static_cast<long long>(g.r0 + token) * a.tree_words, a.tree_words, older);
+  }
+  const int n = g.kv_end - k0;
+  if (n < 32) m &= n <= 0 ? 0u : (1u << n) - 1u;
+  return m;
 }
 
 // Zeros for the rows behind the last sequence's, when the call asks for them.
@@ -134,7 +159,8 @@ struct ThinLayout {
   static constexpr int kStages = 5;
   static constexpr int kRing = kThinWarps * kStages * kHalf;
   static constexpr int kFoldCols = HD < 128 / NQ ? HD : 128 / NQ;           // columns folded at a time
-  static constexpr int kFold = kThinWarps * kM * kFoldCols * 4;
+  static constexpr int kFoldPitch = kFoldCols + 4;                          // floats: rows 2 t4 in banks 8 t4
+  static constexpr int kFold = kThinWarps * kM * kFoldPitch * 4;
   static constexpr int kMl = kThinWarps * kM * 2 * 4;
   static constexpr int kQ = NQ > 2 ? kM * HD * 2 : 0;
   static constexpr int kSegB = kSegs * static_cast<int>(sizeof(Seg));
@@ -151,16 +177,6 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return static_cast<uint32_t>(r * 32 + ((c ^ ((r >> 2) & 1)) << 4));
 }
 
-// Whether a token's row sees cache row t, base <= t < len.
-__device__ __forceinline__ bool sees_draft(const PagedAttnArgs &a, const Seg &g, int token, int t) {
-  const int d = t - g.base;
-  if (a.tree == nullptr) return d <= token;
-  if ((d >> 6) >= a.tree_words) return false;
-  const unsigned long long w =
-      __ldg(a.tree + static_cast<long long>(g.r0 + token) * a.tree_words + (d >> 6));
-  return (w >> (d & 63)) & 1ull;
-}
-
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -170,7 +186,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 template <int HD, int NQ>
 __global__ void __launch_bounds__(kThinThreads, 2)
 attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                       const PagedAttnArgs a) {
+                       const __grid_constant__ PagedAttnArgs a) {
   using L = ThinLayout<HD, NQ>;
   constexpr int KS = HD / 16, C = HD / 8;
   constexpr int M = L::kM;
@@ -225,9 +241,8 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     uint32_t qn[KEEP ? KS : 1][2];
     int n_ids = -1;
     auto q_row = [&](const Seg &g, int r) {
-      const int token = (g.row0 + r) / a.p.n_rep;
-      const int head = g.kvh * a.p.n_rep + (g.row0 + r) - token * a.p.n_rep;
-      return a.q + (g.r0 + token) * a.q_stride + head * HD;
+      const int token = token_of(a.p, g, r);
+      return a.q + (g.r0 + token) * a.q_stride + head_of(a.p, g, r, token) * HD;
     };
     auto ids_of = [&](int seg, int t) {
       const int row = (t + lane) * kThinTile + warp * 16;
@@ -250,47 +265,48 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
     };
     fetch_early(0);
-    // The copies run ahead of the arithmetic over this batch of segments: half `c_half` (0 K,
-    // 1 V) of tile c_t of segment c_s is requested next. Lane i holds the page of this
+    // The copies run ahead of the arithmetic over this batch of segments: the block of tile c_t of
+    // segment c_s is requested next, its K half, then its V half. Lane i holds the page of this
     // warp's block of tile c_first + i.
-    int c_s = 0, c_t = segs[0].t0, c_half = 0, c_end = segs[0].t1;
+    int c_s = 0, c_t = segs[0].t0, c_end = segs[0].t1;
     int c_kvh = segs[0].kvh, c_first = c_t, c_ids = n_ids, c_early = 0;  // c_early: the segment n_ids is of
     // whether the blocks requested and not yet used have rows at all (a block past the item's
     // end, or on a page outside the pool, has none and is not copied); bit: the block's number
     unsigned has_rows = 0, n_asked = 0, n_used = 0;
-    auto request = [&]() {
-      if (c_s >= n_now) return;
-      const int row = c_t * kThinTile + warp * 16;
-      const int c_page = __shfl_sync(0xffffffffu, c_ids, c_t - c_first);
+    int c_page = -1;
+    auto copy = [&](const CUtensorMap *map) {
       const bool live = static_cast<unsigned>(c_page) < static_cast<unsigned>(a.c.n_pages) && ok;
       if (live && lane == 0) {
         const uint32_t dst = ring + ahead * L::kHalf;
-        const CUtensorMap *map = c_half == 0 ? &k_map : &v_map;
+        const int in_page = (c_t * kThinTile + warp * 16) & ((1 << shift) - 1);
         bar_expect(bar + ahead, L::kHalf);
 #pragma unroll
         for (int h = 0; h < (HD > 64 ? HD / 64 : 1); ++h) {
-          tma_page(dst + h * 2048, map, bar + ahead, h * 64, c_kvh, row & ((1 << shift) - 1), c_page);
+          tma_page(dst + h * 2048, map, bar + ahead, h * 64, c_kvh, in_page, c_page);
         }
       }
       ahead = ahead + 1 == S ? 0 : ahead + 1;
-      if (c_half == 0) {
-        has_rows = (has_rows & ~(1u << (n_asked & 31))) | ((live ? 1u : 0u) << (n_asked & 31));
-        ++n_asked;
-        c_half = 1;
-        return;
+      return live;
+    };
+    auto request_k = [&]() {
+      if (c_s >= n_now) return;
+      c_page = __shfl_sync(0xffffffffu, c_ids, c_t - c_first);
+      const uint32_t bit = 1u << (n_asked & 31);
+      has_rows = copy(&k_map) ? has_rows | bit : has_rows & ~bit;
+      ++n_asked;
+    };
+    auto request_v = [&]() {  // of the same block, then on to the next one
+      if (c_s >= n_now) return;
+      copy(&v_map);
+      if (++c_t == c_end && ++c_s < n_now) {
+        c_t = segs[c_s].t0;
+        c_end = segs[c_s].t1;
+        c_kvh = segs[c_s].kvh;
+        c_first = c_t - 32;
       }
-      c_half = 0;
-      if (++c_t == c_end) {
-        if (++c_s < n_now) {
-          c_t = segs[c_s].t0;
-          c_end = segs[c_s].t1;
-          c_kvh = segs[c_s].kvh;
-          c_first = c_t;
-          c_ids = c_s == c_early ? n_ids : ids_of(c_s, c_t);
-        }
-      } else if (c_t - c_first == 32) {
+      if (c_t - c_first == 32 && c_s < n_now) {
         c_first = c_t;
-        c_ids = ids_of(c_s, c_t);
+        c_ids = c_s == c_early && c_t == segs[c_s].t0 ? n_ids : ids_of(c_s, c_t);
       }
     };
     // The copy into the slot consumed next (bounded; nothing is in it when !live).
@@ -302,8 +318,12 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
       return live && ok;
     };
-#pragma unroll
-    for (int i = 0; i < S - 1; ++i) request();
+    static_assert(S == 5, "two blocks ahead of the one in use");
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      request_k();
+      request_v();
+    }
 
     for (int si = 0; si < n_now; ++si) {
       const Seg g = segs[si];
@@ -346,7 +366,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = n * 8 + 2 * t4 + e;
-          token[n][e] = r < g.rows ? (g.row0 + r) / a.p.n_rep : -1;
+          token[n][e] = token_of(a.p, g, min(r, g.rows - 1));
         }
       }
       float o[NQ][KS][4];  // O^T: element rows ks * 16 + g8 (+ 8), queries 2 t4 (+ 1)
@@ -393,7 +413,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           }
         }
         __syncwarp();
-        request();  // into the slot freed a half block ago
+        request_k();  // into the slot freed a half block ago
         uint32_t p[NQ][2];
         if (live) {
           // a block that reaches the new rows, or the item's end, is masked key by key
@@ -402,15 +422,15 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 #pragma unroll
           for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 2; ++e) {
               s[n][e] *= a.c2;
+              s[n][e + 2] *= a.c2;
               if (masked) {
-                const int key = row + g8 + (e >> 1) * 8;
-                const int tok = token[n][e & 1];
-                const bool on = key < g.kv_end && (key < g.base || (tok >= 0 && sees_draft(a, g, tok, key)));
-                s[n][e] = on ? s[n][e] : -INFINITY;
+                const uint32_t m = seen32(a, g, token[n][e], row) >> g8;
+                if ((m & 1u) == 0u) s[n][e] = -INFINITY;
+                if ((m & 256u) == 0u) s[n][e + 2] = -INFINITY;
               }
-              over |= s[n][e] > m_run[n][e & 1] + kSlack;
+              over |= fmaxf(s[n][e], s[n][e + 2]) > m_run[n][e] + kSlack;
             }
           }
           if (__any_sync(0xffffffffu, over)) {
@@ -471,7 +491,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           }
         }
         __syncwarp();
-        request();
+        request_v();
       }
 
       // ---- fold the warps, kFoldCols columns at a time ----
@@ -502,7 +522,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           for (int k = 0; k < FC / 16; ++k) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              fold[(warp * M + n * 8 + 2 * t4 + (e & 1)) * FC + k * 16 + (e >> 1) * 8 + g8] = o[n][f * (FC / 16) + k][e];
+              fold[(warp * M + n * 8 + 2 * t4 + (e & 1)) * L::kFoldPitch + k * 16 + (e >> 1) * 8 + g8] = o[n][f * (FC / 16) + k][e];
             }
           }
         }
@@ -518,12 +538,11 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           for (int w = 0; w < kThinWarps; ++w) {
             const float e = fast_exp2(ml[(w * M + r) * 2] - m_use);
             ll = fmaf(e, ml[(w * M + r) * 2 + 1], ll);
-            oo = fmaf(e, fold[(w * M + r) * FC + d], oo);
+            oo = fmaf(e, fold[(w * M + r) * L::kFoldPitch + d], oo);
           }
           const int col = f * FC + d;
           if (g.whole) {
-            const int tok = (g.row0 + r) / a.p.n_rep;
-            const int head = g.kvh * a.p.n_rep + (g.row0 + r) - tok * a.p.n_rep;
+            const int tok = token_of(a.p, g, r), head = head_of(a.p, g, r, tok);
             a.out[(static_cast<long long>(g.r0 + tok) * a.p.n_kv * a.p.n_rep + head) * HD + col] =
                 __float2bfloat16(ll != 0.f ? oo / ll : 0.f);
           } else {
@@ -687,7 +706,7 @@ AttnForm form_of(int T, int batch, int n_rep, int n_kv, int hd, long long cap) {
   }
   f.M = rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
   f.tile = kThinTile;
-  f.extra = kThinTile;
+  f.extra = 3 * kThinTile;  // what starting and folding a segment takes, in rows (measured)
   // Two resident CTAs per SM, and up to eight in all, so that an SM that is served faster
   // takes more of them; no more than one for every 512 cache rows the tables can hold.
   const long long items = (rows + f.M - 1) / f.M * batch * n_kv;
@@ -799,7 +818,7 @@ extern "C" int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, i
   const int hd = a.c.hd;
   if (T < 1 || n_q < 1 || n_q % a.c.n_kv != 0 || !head_dim_ok(hd) ||
       q_stride < static_cast<int64_t>(n_q) * hd || (tree != nullptr && tree_words < 1) ||
-      !std::isfinite(scale) || (q_start == nullptr && T != a.c.batch) || static_cast<int64_t>(T) * n_q > 0x3fffffffll) {
+      !std::isfinite(scale) || (q_start == nullptr && T != a.c.batch) || static_cast<int64_t>(T) * n_q > 0x3fffffffll || n_q > 65536) {
     return kDims;
   }
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(ws, 16) || q_stride % 8 != 0 || !aligned(a.c.k, 16) ||
@@ -820,6 +839,7 @@ extern "C" int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, i
   a.p.M = f.M;
   a.p.tile = f.tile;
   a.p.extra = f.extra;
+  a.p.per_rep = 1.f / static_cast<float>(n_rep);
   a.p.causal = tree == nullptr;
   // the axis is measured in 64-bit integers that binary64 holds exactly
   const double items = static_cast<double>(T) * n_q / f.M + static_cast<double>(a.c.batch) * a.c.n_kv;
@@ -850,7 +870,7 @@ extern "C" int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, i
   }
   if (e != cudaSuccess) return kLaunch;
   e = launch_chain(attn_paged_join_kernel,
-                   dim3(static_cast<unsigned>((f.ctas + kJoinWarps - 1) / kJoinWarps), f.M == kWideM ? 64 : 8),
+                   dim3(static_cast<unsigned>((f.ctas + kJoinWarps - 1) / kJoinWarps), f.M == kWideM ? 64 : f.M),
                    dim3(kJoinThreads), 0, st, a, f.ctas);
   return e == cudaSuccess ? kOk : kLaunch;
 }

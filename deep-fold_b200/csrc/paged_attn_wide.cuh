@@ -73,36 +73,10 @@ __device__ __forceinline__ bool bar_wait(WideBars &w, uint64_t *b, uint32_t pari
   return false;
 }
 
-// Which of the 32 cache rows k0 .. k0+31 a token's row sees.
-__device__ __forceinline__ uint32_t seen32(const PagedAttnArgs &a, const Seg &g, int token, int k0) {
-  const int older = g.base - k0;  // rows before this one are older than the new rows
-  uint32_t m;
-  if (a.tree == nullptr) {
-    const int n = older + token + 1;
-    m = n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << n) - 1u);
-  } else if (older >= 32) {
-    m = 0xFFFFFFFFu;
-  } else {
-    const unsigned long long *w = a.tree + static_cast<long long>(g.r0 + token) * a.tree_words;
-    const int d0 = -older;
-    if (d0 >= 0) {
-      const int i = d0 >> 6, sh = d0 & 63;
-      unsigned long long v = i < a.tree_words ? __ldg(w + i) >> sh : 0ull;
-      if (sh > 32 && i + 1 < a.tree_words) v |= __ldg(w + i + 1) << (64 - sh);
-      m = static_cast<uint32_t>(v);
-    } else {
-      m = (static_cast<uint32_t>(__ldg(w)) << older) | ((1u << older) - 1u);
-    }
-  }
-  const int n = g.kv_end - k0;
-  if (n < 32) m &= n <= 0 ? 0u : (1u << n) - 1u;
-  return m;
-}
-
 template <int HD>
 __global__ void __launch_bounds__(kWideThreads, 1)
 attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                       const PagedAttnArgs a, const int negate) {
+                       const __grid_constant__ PagedAttnArgs a, const int negate) {
   using L = WideLayout<HD>;
   extern __shared__ __align__(16) unsigned char wide_smem[];
   const uint32_t raw = smem_u32(wide_smem);
@@ -333,9 +307,8 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             const int qr = i / C, c = i % C;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (first_row + qr < g.rows) {
-              const int x = g.row0 + first_row + qr;
-              const int token = x / a.p.n_rep;
-              const int head = g.kvh * a.p.n_rep + x - token * a.p.n_rep;
+              const int token = token_of(a.p, g, first_row + qr);
+              const int head = head_of(a.p, g, first_row + qr, token);
               v = ld_act16(a.q + (g.r0 + token) * a.q_stride + head * HD + c * 8);
             }
             *reinterpret_cast<uint4 *>(sm + L::kQ + tile * L::kTileB + (c >> 3) * L::kPiece + qr * 128 +
@@ -345,8 +318,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           bar_arrive(&w.q_full[tile]);
         }
         const bool mine = first_row + r < g.rows;
-        const int x = g.row0 + first_row + r;
-        const int token = mine ? x / a.p.n_rep : 0;
+        const int token = token_of(a.p, g, min(first_row + r, g.rows - 1));
         float m_run = -INFINITY, l_run = 0.f;
         const float c2 = a.c2;
 
@@ -436,7 +408,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         if (!ok) break;
         tc_fence_after();
         const bool whole = g.whole;
-        const int head = g.kvh * a.p.n_rep + x - token * a.p.n_rep;
+        const int head = head_of(a.p, g, first_row + r, token);
         const float by = l_run != 0.f ? 1.f / l_run : 0.f;
         const PagedWs ws = ws_of(a, G);
         const long long at = (static_cast<long long>(cta) * 2 + g.slot) * kWideM + first_row + r;

@@ -11,11 +11,14 @@
 // floating point. No sort, no sum over the vocabulary, the same result in every run.
 //
 // A cluster of C CTAs owns a row. Each CTA counts its slice of the vocabulary in its own
-// shared memory (65536 16-bit counters, 128 KB; a slice is at most 65535 tokens), the
-// clusters' histograms are read through distributed shared memory: 1024 chunks of 64
-// values get their count and mass, one CTA scans the chunks and walks the three cuts and
-// the draw, and the CTA whose slice holds the token finds its index. One launch, no
-// scratch memory.
+// shared memory (65536 16-bit counters, 128 KB; a slice is at most 65535 tokens) and marks which
+// of the 1024 chunks of 64 values occur. The chunks that do - under a hundred, values of a
+// row spanning a dozen binary orders - are dealt over the cluster's warps: a warp adds the
+// CTAs' counters through distributed shared memory, takes one exp per value, and hands
+// counts and weights to the row's first CTA, one warp of which walks the cuts and the draw.
+// The CTA whose slice holds the drawn token finds its index. One launch, no scratch memory.
+// Bound by latency: counting 19,000 tokens per CTA takes 3 us (shared-memory atomics, about 4 a
+// clock), the rest is a chain of cluster barriers and dependent steps.
 
 #include <cooperative_groups.h>
 
@@ -46,18 +49,24 @@ struct SampleArgs {
   int64_t eos;
 };
 
+constexpr int kCache = 80;  // chunks whose counts and weights the first CTA keeps
+
 struct SampleShared {
   uint32_t hist[kKeys / 2];          // counters 2i (low half) and 2i + 1 (high half)
-  double mass[kChunks];              // rank 0: chunk masses, then what lies before each chunk
-  uint32_t count[kChunks];
-  double part_mass[kSampleWarps];
-  uint32_t part_count[kSampleWarps];
+  uint32_t map[kChunks / 32];        // chunks that occur in this CTA's slice; bit c % 32 of word c / 32
+  uint8_t four[kChunks / 4];         // the same, four chunks a byte
   uint32_t warp_max[kSampleWarps];
   uint32_t max_key;                  // of this CTA's slice
-  // the draw, written by rank 0 into every CTA
+  uint32_t found[kSampleWarps];
+  // the draw, written by the first CTA into every one
   uint32_t pick_key, pick_rank;      // value and its pick_rank-th occurrence
   float pick_prob;
-  uint32_t found[kSampleWarps];
+  // in the first CTA: the chunks that occur, highest values first
+  uint32_t count[kChunks];           // tokens, then tokens before the chunk
+  double mass[kChunks];              // their weight, likewise
+  uint16_t chunk[kChunks];
+  double w[kCache][kChunk];          // values of a chunk, highest first
+  uint32_t n[kCache][kChunk];
 };
 
 // bf16 bits -> a key that orders as the value does (-0 as +0, NaN above everything).
@@ -76,28 +85,43 @@ __device__ __forceinline__ double key_weight(uint32_t key, double m, double temp
   return exp((static_cast<double>(key_value(key)) - m) / temp);
 }
 
-// Calls f(index, bf16 bits) for the elements lo..hi of a row that this thread owns, 16
-// bytes at a time where the row's alignment allows.
-template <typename F>
-__device__ __forceinline__ void for_slice(const __nv_bfloat16 *row, int lo, int hi, F f) {
-  const unsigned short *x = reinterpret_cast<const unsigned short *>(row);
-  const uintptr_t at = reinterpret_cast<uintptr_t>(x + lo);
-  const int head = min(static_cast<int>(((16 - (at & 15)) & 15) >> 1), hi - lo);
-  const int n8 = (hi - lo - head) >> 3;
-  for (int i = threadIdx.x; i < head; i += kSampleThreads) f(lo + i, __ldcg(x + lo + i));
-  const uint4 *body = reinterpret_cast<const uint4 *>(x + lo + head);
-#pragma unroll 4
-  for (int i = threadIdx.x; i < n8; i += kSampleThreads) {
-    const uint4 v = __ldcg(body + i);
-    const int at0 = lo + head + i * 8;
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f(at0 + 2 * e, w[e] & 0xFFFFu);
-      f(at0 + 2 * e + 1, w[e] >> 16);
-    }
+// The 16-byte pieces of elements lo..hi of a row: piece v starts at element first + 8 v; the
+// ones at the ends are read element by element, and what lies outside is marked.
+struct Slice {
+  const unsigned short *x;
+  int lo, hi, first, pieces;
+};
+__device__ __forceinline__ Slice slice_of(const __nv_bfloat16 *row, int lo, int hi) {
+  Slice s;
+  s.x = reinterpret_cast<const unsigned short *>(row);
+  s.lo = lo;
+  s.hi = hi;
+  s.first = lo - static_cast<int>((reinterpret_cast<uintptr_t>(s.x + lo) & 15) >> 1);
+  s.pieces = (hi - s.first + 7) / 8;
+  return s;
+}
+constexpr uint32_t kNegInf = 0xFF80u;
+// Piece v; elements outside the slice read as -inf, `in` tells which are inside.
+__device__ __forceinline__ uint4 slice_piece(const Slice &s, int v, uint32_t &in) {
+  const int at = s.first + v * 8;
+  if (at >= s.lo && at + 8 <= s.hi) {
+    in = 0xFFu;
+    return __ldcg(reinterpret_cast<const uint4 *>(s.x + at));
   }
-  for (int i = lo + head + n8 * 8 + threadIdx.x; i < hi; i += kSampleThreads) f(i, __ldcg(x + i));
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  in = 0u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bool inside = at + e >= s.lo && at + e < s.hi;
+    const uint32_t b = inside ? __ldcg(s.x + at + e) : kNegInf;
+    if (inside) in |= 1u << e;
+    w[e >> 1] |= b << ((e & 1) * 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint32_t element(const uint4 &v, int e) {
+  const uint32_t w = e < 4 ? (e < 2 ? v.x : v.y) : (e < 6 ? v.z : v.w);
+  return (w >> ((e & 1) * 16)) & 0xFFFFu;
 }
 
 // The counts of chunk c over the cluster, two values per lane in descending order: lane l
@@ -121,22 +145,33 @@ __device__ __forceinline__ void chunk_counts(cg::cluster_group &cluster, SampleS
 
 __device__ __forceinline__ double shfl_up(double v, int off) { return __shfl_up_sync(0xffffffffu, v, off); }
 
-// What a warp knows of one chunk: counts, weights and what lies before each value.
+// One chunk of the row as a warp sees it: counts, weights and what lies before each value.
 struct ChunkView {
-  uint32_t n_hi, n_lo, before_hi, before_lo;  // tokens before the lane's two values
-  double w_hi, w_lo, mass_hi, mass_lo;        // weights; mass before the two values
+  uint32_t key;                               // of the lane's higher value
+  uint32_t n_hi, n_lo, before_hi, before_lo;  // tokens; tokens before the lane's two values
+  double w_hi, w_lo, mass_hi, mass_lo;        // weights; weight before the two values
 };
-__device__ __forceinline__ ChunkView view_chunk(cg::cluster_group &cluster, SampleShared &sm, int c,
-                                                int lane, double m, double temp) {
+__device__ __noinline__ ChunkView view_chunk(SampleShared &sm, int i, double m, double temp) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int lane = threadIdx.x & 31;
+  const int c = sm.chunk[i];
   ChunkView v;
-  chunk_counts(cluster, sm, c, lane, v.n_hi, v.n_lo);
-  const uint32_t key = static_cast<uint32_t>(c * kChunk + 63 - 2 * lane);
-  v.w_hi = v.n_hi != 0u ? key_weight(key, m, temp) : 0.0;
-  v.w_lo = v.n_lo != 0u ? key_weight(key - 1u, m, temp) : 0.0;
-  uint32_t cnt = v.n_hi + v.n_lo;
-  double mass = v.n_hi * v.w_hi + v.n_lo * v.w_lo;
-  const uint32_t own_c = cnt;
-  const double own_m = mass;
+  v.key = static_cast<uint32_t>(c * kChunk + 63 - 2 * lane);
+  if (i < kCache) {
+    const uint2 n = *reinterpret_cast<const uint2 *>(&sm.n[i][2 * lane]);
+    const double2 w = *reinterpret_cast<const double2 *>(&sm.w[i][2 * lane]);
+    v.n_hi = n.x;
+    v.n_lo = n.y;
+    v.w_hi = w.x;
+    v.w_lo = w.y;
+  } else {
+    chunk_counts(cluster, sm, c, lane, v.n_hi, v.n_lo);
+    v.w_hi = key_weight(v.key, m, temp);
+    v.w_lo = key_weight(v.key - 1u, m, temp);
+  }
+  const uint32_t own_c = v.n_hi + v.n_lo;
+  uint32_t cnt = own_c;
+  double mass = (v.n_hi != 0u ? v.n_hi * v.w_hi : 0.0) + (v.n_lo != 0u ? v.n_lo * v.w_lo : 0.0);
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const uint32_t oc = __shfl_up_sync(0xffffffffu, cnt, off);
@@ -148,86 +183,52 @@ __device__ __forceinline__ ChunkView view_chunk(cg::cluster_group &cluster, Samp
   }
   double prev = shfl_up(mass, 1);
   if (lane == 0) prev = 0.0;
-  (void)own_m;
-  v.before_hi = sm.count[c] + cnt - own_c;
+  v.before_hi = sm.count[i] + cnt - own_c;
   v.before_lo = v.before_hi + v.n_hi;
-  v.mass_hi = sm.mass[c] + prev;
-  v.mass_lo = v.mass_hi + v.n_hi * v.w_hi;
+  v.mass_hi = sm.mass[i] + prev;
+  v.mass_lo = v.mass_hi + (v.n_hi != 0u ? v.n_hi * v.w_hi : 0.0);
   return v;
 }
 
-// The last chunk, in descending order of value, before which no more than `count` tokens
-// (or mass) lie. Chunk c's entry holds what lies before it; c = 1023 comes first.
+// The last of L ascending values that is at most `limit` (or[strict]: below it); 0 if none is.
 template <typename T>
-__device__ __forceinline__ int last_chunk(const T *before, T limit, int lane) {
-  // 32 groups of 32 chunks
-  const unsigned ga = __ballot_sync(0xffffffffu, before[kChunks - 1 - lane * 32] <= limit);
-  const int g = 31 - __clz(ga | 1u);
-  const unsigned gb = __ballot_sync(0xffffffffu, before[kChunks - 1 - (g * 32 + lane)] <= limit);
-  return kChunks - 1 - (g * 32 + 31 - __clz(gb | 1u));
+__device__ __forceinline__ int last_of(const T *v, int L, T limit, bool below) {
+  const int lane = threadIdx.x & 31;
+  auto ok = [&](int i) { return i < L && (below ? v[i] < limit : v[i] <= limit); };
+  const int g = 31 - __clz(__ballot_sync(0xffffffffu, ok(lane * 32)) | 1u);
+  return g * 32 + 31 - __clz(__ballot_sync(0xffffffffu, ok(g * 32 + lane)) | 1u);
 }
 
-// Value and rank within it of the token with `rank` tokens before it; mass before the
-// value. Called by a whole warp; every lane gets the result.
-struct Token {
-  uint32_t key, in;   // value, occurrences of it before the token
-  double mass, w;     // mass before the value, weight
-};
-__device__ __forceinline__ Token token_at(cg::cluster_group &cluster, SampleShared &sm, uint32_t rank,
-                                          int lane, double m, double temp) {
-  const int c = last_chunk(sm.count, rank, lane);
-  const ChunkView v = view_chunk(cluster, sm, c, lane, m, temp);
-  const bool in_hi = v.n_hi != 0u && rank >= v.before_hi && rank < v.before_hi + v.n_hi;
-  const bool in_lo = v.n_lo != 0u && rank >= v.before_lo && rank < v.before_lo + v.n_lo;
-  const unsigned who = __ballot_sync(0xffffffffu, in_hi || in_lo);
-  const int from = __ffs(who | 0x80000000u) - 1;
-  const uint32_t base = static_cast<uint32_t>(c * kChunk + 63 - 2 * lane);
-  Token t;
-  t.key = __shfl_sync(0xffffffffu, in_hi ? base : base - 1u, from);
-  t.in = __shfl_sync(0xffffffffu, rank - (in_hi ? v.before_hi : v.before_lo), from);
-  t.mass = __shfl_sync(0xffffffffu, in_hi ? v.mass_hi : v.mass_lo, from);
-  t.w = __shfl_sync(0xffffffffu, in_hi ? v.w_hi : v.w_lo, from);
-  return t;
-}
-
-// The first token after which the running mass exceeds `r` (strict) or reaches it: its
-// value's first rank, its count, the mass before the value and the weight.
-struct Crossing {
+// A value of the row: its key, the tokens and the weight before it, its tokens and weight.
+struct Value {
   uint32_t key, before, n;
   double mass, w;
 };
-__device__ __forceinline__ Crossing crossing(cg::cluster_group &cluster, SampleShared &sm, double r,
-                                             bool strict, int lane, double m, double temp) {
-  // the last chunk with no more than r (strict: the crossing token has cum > r) before it;
-  // when the cum has to reach r only, the last with less than r before it
-  int c;
-  if (strict) {
-    c = last_chunk(sm.mass, r, lane);
-  } else {
-    const unsigned ga = __ballot_sync(0xffffffffu, sm.mass[kChunks - 1 - lane * 32] < r || lane == 0);
-    const int g = 31 - __clz(ga);
-    const unsigned gb =
-        __ballot_sync(0xffffffffu, sm.mass[kChunks - 1 - (g * 32 + lane)] < r || lane == 0);
-    c = kChunks - 1 - (g * 32 + 31 - __clz(gb));
-  }
-  const ChunkView v = view_chunk(cluster, sm, c, lane, m, temp);
-  const double end_hi = v.mass_hi + v.n_hi * v.w_hi, end_lo = v.mass_lo + v.n_lo * v.w_lo;
-  const bool hi = v.n_hi != 0u && (strict ? end_hi > r : end_hi >= r);
-  const bool lo = v.n_lo != 0u && (strict ? end_lo > r : end_lo >= r);
-  unsigned who = __ballot_sync(0xffffffffu, hi || lo);
-  // rounding may leave the chunk's end short of r: its last value then
+// Of the chunk a warp sees, the first value with some lane's flag, or else the last one.
+__device__ __forceinline__ Value pick_value(const ChunkView &v, bool hi, bool lo) {
+  const unsigned who = __ballot_sync(0xffffffffu, hi || lo);
   const unsigned any = __ballot_sync(0xffffffffu, v.n_hi != 0u || v.n_lo != 0u);
-  const bool none = who == 0u;
-  const int from = none ? 31 - __clz(any | 1u) : __ffs(who) - 1;
-  const bool take_hi = none ? v.n_lo == 0u : hi;
-  const uint32_t base = static_cast<uint32_t>(c * kChunk + 63 - 2 * lane);
-  Crossing x;
-  x.key = __shfl_sync(0xffffffffu, take_hi ? base : base - 1u, from);
+  const int from = who != 0u ? __ffs(who) - 1 : 31 - __clz(any | 1u);
+  const bool take_hi = who != 0u ? hi : v.n_lo == 0u;
+  Value x;
+  x.key = __shfl_sync(0xffffffffu, take_hi ? v.key : v.key - 1u, from);
   x.before = __shfl_sync(0xffffffffu, take_hi ? v.before_hi : v.before_lo, from);
   x.n = __shfl_sync(0xffffffffu, take_hi ? v.n_hi : v.n_lo, from);
   x.mass = __shfl_sync(0xffffffffu, take_hi ? v.mass_hi : v.mass_lo, from);
   x.w = __shfl_sync(0xffffffffu, take_hi ? v.w_hi : v.w_lo, from);
   return x;
+}
+// The value of the token that has `rank` tokens before it.
+__device__ __forceinline__ Value value_at(SampleShared &sm, int L, uint32_t rank, double m, double temp) {
+  const ChunkView v = view_chunk(sm, last_of(sm.count, L, rank, false), m, temp);
+  return pick_value(v, v.n_hi != 0u && rank < v.before_hi + v.n_hi, v.n_lo != 0u && rank < v.before_lo + v.n_lo);
+}
+// The first value whose end of the running weight exceeds r (or, not strict, reaches it).
+__device__ __forceinline__ Value crossing(SampleShared &sm, int L, double r, bool strict, double m, double temp) {
+  const ChunkView v = view_chunk(sm, last_of(sm.mass, L, r, !strict), m, temp);
+  const double end_hi = v.mass_hi + v.n_hi * v.w_hi, end_lo = v.mass_lo + v.n_lo * v.w_lo;
+  return pick_value(v, v.n_hi != 0u && (strict ? end_hi > r : end_hi >= r),
+                    v.n_lo != 0u && (strict ? end_lo > r : end_lo >= r));
 }
 
 __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleArgs a) {
@@ -246,20 +247,44 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
   pdl_wait();
   const __nv_bfloat16 *row = a.logits + b * a.row_stride;
   const int lo = min(rank * a.slice, a.n), hi = min(lo + a.slice, a.n);
+  const Slice slice = slice_of(row, lo, hi);
 
-  // ---- the slice's histogram and maximum ----
+  // ---- the slice's histogram and maximum; -inf, which weighs nothing, is not counted ----
   uint32_t top = 0u;
-  for_slice(row, lo, hi, [&](int, uint32_t bits) {
-    const uint32_t key = order_key(bits);
-    top = max(top, key);
-    atomicAdd(&sm.hist[key >> 1], (key & 1u) ? 65536u : 1u);
-  });
+#pragma unroll 4
+  for (int v = tid; v < slice.pieces; v += kSampleThreads) {
+    uint32_t in;
+    const uint4 x = slice_piece(slice, v, in);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t bits = element(x, e);
+      const uint32_t key = order_key(bits);
+      top = max(top, key);
+      if (bits != kNegInf) atomicAdd(&sm.hist[key >> 1], (key & 1u) ? 65536u : 1u);
+    }
+  }
   top = __reduce_max_sync(0xffffffffu, top);
   if (lane == 0) sm.warp_max[warp] = top;
   __syncthreads();
+  // chunks that occur: a warp looks at four chunks (512 bytes) at a time
+  for (int i = warp; i < kChunks / 4; i += kSampleWarps) {
+    const uint4 v = reinterpret_cast<const uint4 *>(sm.hist)[i * 32 + lane];
+    const unsigned some = __ballot_sync(0xffffffffu, (v.x | v.y | v.z | v.w) != 0u);
+    const uint32_t four = ((some & 0xFFu) != 0u ? 1u : 0u) | ((some & 0xFF00u) != 0u ? 2u : 0u) |
+                          ((some & 0xFF0000u) != 0u ? 4u : 0u) | ((some & 0xFF000000u) != 0u ? 8u : 0u);
+    if (lane == 0) sm.four[i] = static_cast<uint8_t>(four);
+  }
   if (warp == 0) {
     const uint32_t v = __reduce_max_sync(0xffffffffu, lane < kSampleWarps ? sm.warp_max[lane] : 0u);
     if (lane == 0) sm.max_key = v;
+  }
+  __syncthreads();
+  if (tid < kChunks / 32) {
+    const uint2 v = reinterpret_cast<const uint2 *>(sm.four)[tid];
+    uint32_t w = 0u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w |= ((v.x >> (8 * e)) & 15u) << (4 * e) | ((v.y >> (8 * e)) & 15u) << (16 + 4 * e);
+    sm.map[tid] = w;
   }
   cluster.sync();
 
@@ -274,44 +299,62 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
   uint32_t pick_key = max_key, pick_rank = 0u;
   float pick_prob = 1.f;
   if (!greedy) {
-    // ---- count and mass of every chunk, to rank 0 ----
+    // ---- counts and weights of the chunks that occur, to the first CTA ----
     SampleShared *lead = cluster.map_shared_rank(&sm, 0);
-    for (int i = warp; i * C + rank < kChunks; i += kSampleWarps) {
-      const int c = i * C + rank;
+    // lane l: word 31 - l, so that both lanes and bits run from the highest chunk down
+    uint32_t word = 0u;
+#pragma unroll
+    for (int r = 0; r < kSampleMaxCluster; ++r) {
+      if (r < C) word |= *cluster.map_shared_rank(&sm.map[31 - lane], r);
+    }
+    int upto = __popc(word);
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += o;
+    }
+    const int L = __shfl_sync(0xffffffffu, upto, 31);
+    for (int i = warp * C + rank; i < L; i += kSampleWarps * C) {
+      // the i-th chunk: its word, then the bit with i - (bits before the word) set ones above it
+      const int from = __ffs(__ballot_sync(0xffffffffu, upto > i)) - 1;
+      const uint32_t bits = __shfl_sync(0xffffffffu, word, from);
+      const int nth = i - (__shfl_sync(0xffffffffu, upto, from) - __popc(bits));
+      const bool mine = (bits >> (31 - lane)) & 1u;
+      const unsigned set = __ballot_sync(0xffffffffu, mine);  // lane order: highest bit first
+      const int at = __ffs(__ballot_sync(0xffffffffu, mine && __popc(set & ((1u << lane) - 1u)) == nth)) - 1;
+      const int c = (31 - from) * 32 + 31 - at;
       uint32_t n_hi, n_lo;
       chunk_counts(cluster, sm, c, lane, n_hi, n_lo);
-      double mass = 0.0;
-      uint32_t cnt = 0u;
-      if (__any_sync(0xffffffffu, (n_hi | n_lo) != 0u)) {
-        const uint32_t key = static_cast<uint32_t>(c * kChunk + 63 - 2 * lane);
-        if (n_hi != 0u) mass = n_hi * key_weight(key, m, temp);
-        if (n_lo != 0u) mass += n_lo * key_weight(key - 1u, m, temp);
-        cnt = __reduce_add_sync(0xffffffffu, n_hi + n_lo);
-        // the order of view_chunk's running sum
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const double o = shfl_up(mass, off);
-          if (lane >= off) mass += o;
-        }
+      const uint32_t key = static_cast<uint32_t>(c * kChunk + 63 - 2 * lane);
+      const double w_hi = key_weight(key, m, temp), w_lo = key_weight(key - 1u, m, temp);
+      // a value that does not occur may have no finite weight
+      double mass = (n_hi != 0u ? n_hi * w_hi : 0.0) + (n_lo != 0u ? n_lo * w_lo : 0.0);
+      if (i < kCache) {
+        *reinterpret_cast<uint2 *>(&lead->n[i][2 * lane]) = make_uint2(n_hi, n_lo);
+        *reinterpret_cast<double2 *>(&lead->w[i][2 * lane]) = make_double2(w_hi, w_lo);
       }
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {  // in the order of view_chunk's running sum
+        const double o = shfl_up(mass, off);
+        if (lane >= off) mass += o;
+      }
+      const uint32_t cnt = __reduce_add_sync(0xffffffffu, n_hi + n_lo);
       if (lane == 31) {
-        lead->mass[c] = mass;
-        lead->count[c] = cnt;
+        lead->mass[i] = mass;
+        lead->count[i] = cnt;
+        lead->chunk[i] = static_cast<uint16_t>(c);
       }
     }
     cluster.sync();
-    if (rank == 0) {
-      // ---- what lies before each chunk, in descending order of value ----
-      constexpr int kPer = kChunks / kSampleThreads;
-      double mv[kPer], run = 0.0;
-      uint32_t cv[kPer], run_c = 0u;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int c = kChunks - 1 - (tid * kPer + i);
-        mv[i] = run;
-        cv[i] = run_c;
-        run += sm.mass[c];
-        run_c += sm.count[c];
+    if (rank == 0 && warp == 0) {
+      // ---- what lies before each chunk: a lane sums a run of them ----
+      const int per = (L + 31) / 32;
+      const int i0 = min(lane * per, L), i1 = min(i0 + per, L);
+      double run = 0.0;
+      uint32_t run_c = 0u;
+      for (int i = i0; i < i1; ++i) {
+        run += sm.mass[i];
+        run_c += sm.count[i];
       }
       double incl = run;
       uint32_t incl_c = run_c;
@@ -324,111 +367,77 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
           incl_c += oc;
         }
       }
-      double prev = shfl_up(incl, 1);
-      uint32_t prev_c = __shfl_up_sync(0xffffffffu, incl_c, 1);
-      if (lane == 0) {
-        prev = 0.0;
-        prev_c = 0u;
+      const double total = __shfl_sync(0xffffffffu, incl, 31);
+      const uint32_t finite = __shfl_sync(0xffffffffu, incl_c, 31);  // tokens that are not -inf
+      double at = shfl_up(incl, 1);
+      uint32_t at_c = incl_c - run_c;
+      if (lane == 0) at = 0.0;
+      for (int i = i0; i < i1; ++i) {
+        const double mi = sm.mass[i];
+        const uint32_t ci = sm.count[i];
+        sm.mass[i] = at;
+        sm.count[i] = at_c;
+        at += mi;
+        at_c += ci;
       }
-      if (lane == 31) {
-        sm.part_mass[warp] = incl;
-        sm.part_count[warp] = incl_c;
+      __syncwarp();
+      // ---- the kept prefix: its tokens and their weight, cut by cut ----
+      uint32_t kept = finite;
+      double sum = total;
+      const int k = a.top_k != nullptr ? __ldg(a.top_k + b) : 0;
+      if (k > 0 && static_cast<uint32_t>(k) < finite) {
+        kept = static_cast<uint32_t>(k);
+        const Value x = value_at(sm, L, kept - 1u, m, temp);
+        sum = x.mass + (kept - x.before) * x.w;
       }
-      __syncthreads();
-      double at = 0.0;
-      uint32_t at_c = 0u;
-      for (int w = 0; w < warp; ++w) {
-        at += sm.part_mass[w];
-        at_c += sm.part_count[w];
+      const float p = a.top_p != nullptr ? __ldg(a.top_p + b) : 1.f;
+      const float least = a.min_p != nullptr ? __ldg(a.min_p + b) : 0.f;
+      if (p < 1.f) {
+        const double target = fmax(static_cast<double>(p) * sum, 0.0);
+        const Value x = crossing(sm, L, target, false, m, temp);
+        // of the crossing value's tokens those before which the sum is below the target
+        double q = x.w > 0.0 ? ceil((target - x.mass) / x.w) : 1.0;
+        q = fmin(fmax(q, 1.0), static_cast<double>(x.n));
+        const uint32_t np = max(x.before + static_cast<uint32_t>(q), 1u);
+        if (np < kept) {
+          kept = np;
+          sum = x.mass + q * x.w;
+        }
       }
-      double total = 0.0;
-      for (int w = 0; w < kSampleWarps; ++w) total += sm.part_mass[w];
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int c = kChunks - 1 - (tid * kPer + i);
-        sm.mass[c] = at + prev + mv[i];
-        sm.count[c] = at_c + prev_c + cv[i];
+      if (least > 0.f) {
+        // the last chunk whose highest value still weighs min_p, then the values within
+        auto heavy = [&](int i) {
+          return i < L && key_weight(sm.chunk[i] * kChunk + 63u, m, temp) >= static_cast<double>(least);
+        };
+        const int g = 31 - __clz(__ballot_sync(0xffffffffu, heavy(lane * 32)) | 1u);
+        const int i = g * 32 + 31 - __clz(__ballot_sync(0xffffffffu, heavy(g * 32 + lane)) | 1u);
+        const ChunkView v = view_chunk(sm, i, m, temp);
+        const bool hi_in = v.n_hi != 0u && v.w_hi >= static_cast<double>(least);
+        const bool lo_in = v.n_lo != 0u && v.w_lo >= static_cast<double>(least);
+        const uint32_t nm = __shfl_sync(0xffffffffu, v.before_hi, 0) +
+                            __reduce_add_sync(0xffffffffu, (hi_in ? v.n_hi : 0u) + (lo_in ? v.n_lo : 0u));
+        if (nm < kept) {
+          kept = max(nm, 1u);
+          const Value x = value_at(sm, L, kept - 1u, m, temp);
+          sum = x.mass + (kept - x.before) * x.w;
+        }
       }
-      __syncthreads();
-      if (warp == 0) {
-        // ---- the kept prefix ----
-        const uint32_t n = static_cast<uint32_t>(a.n);
-        uint32_t keep = n;
-        double sum = total;
-        const int k = a.top_k != nullptr ? __ldg(a.top_k + b) : 0;
-        if (k > 0 && static_cast<uint32_t>(k) < n) {
-          keep = static_cast<uint32_t>(k);
-          const Token t = token_at(cluster, sm, keep - 1u, lane, m, temp);
-          sum = t.mass + (t.in + 1u) * t.w;
-        }
-        const float p = a.top_p != nullptr ? __ldg(a.top_p + b) : 1.f;
-        uint32_t kept = keep;
-        if (p < 1.f) {
-          const double target = static_cast<double>(p) * sum;
-          uint32_t np = 1u;
-          if (target > 0.0) {
-            const Crossing x = crossing(cluster, sm, target, false, lane, m, temp);
-            // of the crossing value's tokens those before which the sum is below the target
-            double q = x.w > 0.0 ? ceil((target - x.mass) / x.w) : 1.0;
-            q = fmin(fmax(q, 1.0), static_cast<double>(x.n));
-            np = x.before + static_cast<uint32_t>(q);
-          }
-          kept = min(kept, np);
-        }
-        const float least = a.min_p != nullptr ? __ldg(a.min_p + b) : 0.f;
-        if (least > 0.f) {
-          // the lowest value whose weight is still min_p: 32-way search over the values
-          uint32_t lo_k = 0u, hi_k = max_key;  // weight(hi_k) = 1
-          uint32_t nm = 1u;
-          if (least <= 1.f) {
-            while (lo_k < hi_k) {
-              const uint32_t step = (hi_k - lo_k + 31u) / 32u;
-              const uint32_t key = min(lo_k + step * lane, hi_k);
-              const bool ok = key_weight(key, m, temp) >= static_cast<double>(least);
-              const unsigned yes = __ballot_sync(0xffffffffu, ok);
-              if (yes == 0u) {          // only hi_k itself may do
-                lo_k = min(lo_k + step * 31u + 1u, hi_k);
-              } else {
-                const int f = __ffs(yes) - 1;
-                const uint32_t found = min(lo_k + step * f, hi_k);
-                lo_k = f == 0 ? lo_k : min(lo_k + step * (f - 1) + 1u, found);
-                hi_k = found;
-              }
-            }
-            // tokens of value hi_k and above
-            const int c = static_cast<int>(hi_k / kChunk);
-            const ChunkView v = view_chunk(cluster, sm, c, lane, m, temp);
-            const uint32_t key = static_cast<uint32_t>(c * kChunk + 63 - 2 * lane);
-            const uint32_t here = (key >= hi_k ? v.n_hi : 0u) + (key - 1u >= hi_k ? v.n_lo : 0u);
-            nm = sm.count[c] + __reduce_add_sync(0xffffffffu, here);
-          }
-          kept = min(kept, nm);
-        }
-        kept = max(kept, 1u);
-        if (kept != keep) {
-          const Token t = token_at(cluster, sm, kept - 1u, lane, m, temp);
-          sum = t.mass + (t.in + 1u) * t.w;
-        }
-        // ---- the draw ----
-        const float uf = fminf(fmaxf(__ldg(a.u + b), 0.f), 0.99999994f);  // NaN: 0
-        const double r = static_cast<double>(uf) * sum;
-        const Crossing x = crossing(cluster, sm, r, true, lane, m, temp);
-        double q = x.w > 0.0 ? floor((r - x.mass) / x.w) : 0.0;
-        q = fmin(fmax(q, 0.0), static_cast<double>(x.n - 1u));
-        uint32_t in = static_cast<uint32_t>(q), key = x.key;
-        double w = x.w;
-        if (x.before + in >= kept) {  // rounding took the draw past the last kept token
-          const Token t = token_at(cluster, sm, kept - 1u, lane, m, temp);
-          key = t.key;
-          in = t.in;
-          w = t.w;
-        }
-        if (lane < C) {
-          SampleShared *to = cluster.map_shared_rank(&sm, lane);
-          to->pick_key = key;
-          to->pick_rank = in;
-          to->pick_prob = static_cast<float>(w / sum);
-        }
+      // ---- the draw ----
+      const float uf = fminf(fmaxf(__ldg(a.u + b), 0.f), 0.99999994f);  // NaN: 0
+      const double r = static_cast<double>(uf) * sum;
+      Value x = crossing(sm, L, r, true, m, temp);
+      double q = x.w > 0.0 ? floor((r - x.mass) / x.w) : 0.0;
+      q = fmin(fmax(q, 0.0), static_cast<double>(x.n) - 1.0);
+      uint32_t in = static_cast<uint32_t>(fmax(q, 0.0));
+      if (x.before + in >= kept) {  // rounding took the draw past the last kept token
+        x = value_at(sm, L, kept - 1u, m, temp);
+        in = kept - 1u - x.before;
+      }
+      if (lane < C) {
+        SampleShared *to = cluster.map_shared_rank(&sm, lane);
+        to->pick_key = x.key;
+        to->pick_rank = in;
+        to->pick_prob = static_cast<float>(x.w / sum);
       }
     }
     cluster.sync();
@@ -438,44 +447,76 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
   }
 
   // ---- the pick_rank-th token of value pick_key, in order of index ----
-  const int shift = (pick_key & 1u) ? 16 : 0;
-  uint32_t before = 0u;
-  for (int r = 0; r < rank; ++r) {
-    before += (*cluster.map_shared_rank(&sm.hist[pick_key >> 1], r) >> shift) & 0xFFFFu;
-  }
-  const uint32_t here = (sm.hist[pick_key >> 1] >> shift) & 0xFFFFu;
-  if (pick_rank >= before && pick_rank < before + here) {
-    const uint32_t want = pick_rank - before;  // occurrence within the slice
-    const unsigned short *x = reinterpret_cast<const unsigned short *>(row);
-    // a warp's part of the slice, in order of index
-    const int per = (hi - lo + kSampleWarps - 1) / kSampleWarps;
-    const int w0 = min(lo + warp * per, hi), w1 = min(w0 + per, hi);
-    uint32_t mine = 0u;
-    for (int i = w0 + lane; i < w1; i += 32) mine += order_key(__ldcg(x + i)) == pick_key ? 1u : 0u;
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if (lane == 0) sm.found[warp] = mine;
-    __syncthreads();
-    uint32_t skip = 0u;
-    for (int w = 0; w < warp; ++w) skip += sm.found[w];
-    if (want >= skip && want < skip + mine) {
-      uint32_t left = want - skip;
-      for (int i = w0; i < w1; i += 32) {
-        const bool is = i + lane < w1 && order_key(__ldcg(x + i + lane)) == pick_key;
-        const unsigned hit = __ballot_sync(0xffffffffu, is);
-        const uint32_t cnt = __popc(hit);
-        if (left < cnt) {
-          const unsigned upto = hit & ((2u << lane) - 1u);  // (2 << 31) - 1: all lanes
-          if (is && __popc(upto) == static_cast<int>(left) + 1) {
-            const int64_t idx = i + lane;
-            a.next_token[b] = idx;
-            if (a.token != nullptr) a.token[b] = idx;
-            if (a.position != nullptr) a.position[b] += 1;
-            if (a.finished != nullptr && idx == a.eos) a.finished[b] |= 1;
-            if (a.prob != nullptr) a.prob[b] = pick_prob;
-          }
-          break;
+  auto commit = [&](int64_t idx) {
+    a.next_token[b] = idx;
+    if (a.token != nullptr) a.token[b] = idx;
+    if (a.position != nullptr) a.position[b] += 1;
+    if (a.finished != nullptr && idx == a.eos) a.finished[b] |= 1;
+    if (a.prob != nullptr) a.prob[b] = pick_prob;
+  };
+  if (max_f == -INFINITY) {  // nothing but -inf, which was not counted
+    if (rank == 0 && tid == 0) commit(0);
+  } else {
+    const int shift = (pick_key & 1u) ? 16 : 0;
+    uint32_t counts[kSampleMaxCluster];
+#pragma unroll
+    for (int r = 0; r < kSampleMaxCluster; ++r) {
+      counts[r] = r <= rank ? *cluster.map_shared_rank(&sm.hist[pick_key >> 1], r) : 0u;
+    }
+    uint32_t before = 0u, here = 0u;
+#pragma unroll
+    for (int r = 0; r < kSampleMaxCluster; ++r) {
+      const uint32_t n = (counts[r] >> shift) & 0xFFFFu;
+      if (r < rank) before += n;
+      if (r == rank) here = n;
+    }
+    if (pick_rank >= before && pick_rank < before + here) {
+      uint32_t want = pick_rank - before;  // occurrence within the slice
+      auto matches = [&](int v) {
+        uint32_t in, hit = 0u;
+        const uint4 x = slice_piece(slice, v, in);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) hit |= (order_key(element(x, e)) == pick_key ? 1u : 0u) << e;
+        return hit & in;
+      };
+      // a warp's part of the slice, in order of index
+      const int per = (slice.pieces + kSampleWarps - 1) / kSampleWarps;
+      const int w0 = min(warp * per, slice.pieces), w1 = min(w0 + per, slice.pieces);
+      if (here == 1u) {
+#pragma unroll 4
+        for (int v = w0 + lane; v < w1; v += 32) {
+          const uint32_t hit = matches(v);
+          if (hit != 0u) commit(slice.first + v * 8 + __ffs(hit) - 1);
         }
-        left -= cnt;
+      } else {
+        uint32_t mine = 0u;
+#pragma unroll 4
+        for (int v = w0 + lane; v < w1; v += 32) mine += __popc(matches(v));
+        mine = __reduce_add_sync(0xffffffffu, mine);
+        if (lane == 0) sm.found[warp] = mine;
+        __syncthreads();
+        uint32_t skip = 0u;
+        for (int w = 0; w < warp; ++w) skip += sm.found[w];
+        if (want >= skip && want < skip + mine) {
+          want -= skip;
+          for (int v0 = w0; v0 < w1; v0 += 32) {
+            uint32_t hit = v0 + lane < w1 ? matches(v0 + lane) : 0u;
+            uint32_t incl = __popc(hit);
+            const uint32_t own = incl;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+              const uint32_t o = __shfl_up_sync(0xffffffffu, incl, off);
+              if (lane >= off) incl += o;
+            }
+            if (want >= incl - own && want < incl) {
+              for (uint32_t j = incl - own; j < want; ++j) hit &= hit - 1u;
+              commit(slice.first + (v0 + lane) * 8 + __ffs(hit) - 1);
+            }
+            const uint32_t all = __shfl_sync(0xffffffffu, incl, 31);
+            if (want < all) break;
+            want -= all;
+          }
+        }
       }
     }
   }
