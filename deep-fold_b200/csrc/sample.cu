@@ -29,7 +29,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kSampleThreads = 512;
+constexpr int kSampleThreads = 1024;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kKeys = 65536;
 constexpr int kChunk = 64;                 // values per chunk
@@ -55,7 +55,6 @@ struct SampleShared {
   uint32_t hist[kKeys / 2];          // counters 2i (low half) and 2i + 1 (high half)
   uint32_t map[kChunks / 32];        // chunks that occur in this CTA's slice; bit c % 32 of word c / 32
   uint8_t four[kChunks / 4];         // the same, four chunks a byte
-  uint32_t warp_max[kSampleWarps];
   uint32_t max_key;                  // of this CTA's slice
   uint32_t found[kSampleWarps];
   // the draw, written by the first CTA into every one
@@ -69,12 +68,8 @@ struct SampleShared {
   uint32_t n[kCache][kChunk];
 };
 
-// bf16 bits -> a key that orders as the value does (-0 as +0, NaN above everything).
-__device__ __forceinline__ uint32_t order_key(uint32_t b) {
-  if ((b & 0x7FFFu) > 0x7F80u) return 0xFFFFu;
-  if (b == 0x8000u) b = 0u;
-  return (b & 0x8000u) ? (~b & 0xFFFFu) : (b | 0x8000u);
-}
+// A value's key orders as the value does: the bits of a bf16 with the sign flipped, a
+// negative one with all bits flipped; -0 has +0's key, NaN the highest.
 __device__ __forceinline__ float key_value(uint32_t k) {
   const uint32_t b = (k & 0x8000u) ? (k & 0x7FFFu) : (~k & 0xFFFFu);
   return __uint_as_float(b << 16);
@@ -100,7 +95,7 @@ __device__ __forceinline__ Slice slice_of(const __nv_bfloat16 *row, int lo, int 
   s.pieces = (hi - s.first + 7) / 8;
   return s;
 }
-constexpr uint32_t kNegInf = 0xFF80u;
+constexpr uint32_t kNegInf = 0xFF80u, kNegInfKey = 0x007Fu;
 // Piece v; elements outside the slice read as -inf, `in` tells which are inside.
 __device__ __forceinline__ uint4 slice_piece(const Slice &s, int v, uint32_t &in) {
   const int at = s.first + v * 8;
@@ -119,9 +114,13 @@ __device__ __forceinline__ uint4 slice_piece(const Slice &s, int v, uint32_t &in
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ uint32_t element(const uint4 &v, int e) {
-  const uint32_t w = e < 4 ? (e < 2 ? v.x : v.y) : (e < 6 ? v.z : v.w);
-  return (w >> ((e & 1) * 16)) & 0xFFFFu;
+// Two bf16 values as order keys, but for NaN and -0, which are put right afterwards.
+__device__ __forceinline__ uint32_t raw_keys(uint32_t two) {
+  return two ^ (((two >> 15) & 0x00010001u) * 0xFFFFu | 0x80008000u);
+}
+// One token of key `key`; -inf is not counted (a masked vocabulary would queue up at its counter).
+__device__ __forceinline__ void count_key(SampleShared &sm, uint32_t key) {
+  if (key != kNegInfKey) atomicAdd(&sm.hist[key >> 1], (key & 1u) ? 65536u : 1u);
 }
 
 // The counts of chunk c over the cluster, two values per lane in descending order: lane l
@@ -249,24 +248,45 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
   const int lo = min(rank * a.slice, a.n), hi = min(lo + a.slice, a.n);
   const Slice slice = slice_of(row, lo, hi);
 
-  // ---- the slice's histogram and maximum; -inf, which weighs nothing, is not counted ----
-  uint32_t top = 0u;
+  // ---- the slice's histogram ----
 #pragma unroll 4
   for (int v = tid; v < slice.pieces; v += kSampleThreads) {
     uint32_t in;
     const uint4 x = slice_piece(slice, v, in);
+    const uint32_t two[4] = {raw_keys(x.x), raw_keys(x.y), raw_keys(x.z), raw_keys(x.w)};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t bits = element(x, e);
-      const uint32_t key = order_key(bits);
-      top = max(top, key);
-      if (bits != kNegInf) atomicAdd(&sm.hist[key >> 1], (key & 1u) ? 65536u : 1u);
+    for (int e = 0; e < 4; ++e) {
+      count_key(sm, two[e] & 0xFFFFu);
+      count_key(sm, two[e] >> 16);
     }
   }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) sm.warp_max[warp] = top;
+  __syncthreads();
+  // NaN of either sign to the highest key, -0 to +0
+  if (warp == 0) {
+    uint32_t nans = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int w = i * 32 + lane;  // words 0..63: keys 0..127, 64..127: keys 0xFF80..0xFFFF
+      uint32_t *at = &sm.hist[w < 64 ? w : kKeys / 2 - 128 + w];
+      uint32_t n = *at;
+      // -inf (key 0x7F) has no count; +inf (0xFF80, the low half of its word) keeps its own
+      const uint32_t keep = w == 64 ? n & 0xFFFFu : 0u;
+      n -= keep;
+      if (n != 0u) *at = keep;
+      nans += (n & 0xFFFFu) + (n >> 16);
+    }
+    nans = __reduce_add_sync(0xffffffffu, nans);
+    __syncwarp();
+    if (lane == 0) {
+      if (nans != 0u) sm.hist[kKeys / 2 - 1] += nans << 16;
+      const uint32_t minus = sm.hist[0x7FFF >> 1] >> 16;  // -0: the high half of word 0x3FFF
+      sm.hist[0x7FFF >> 1] &= 0xFFFFu;
+      sm.hist[0x8000 >> 1] += minus;
+    }
+  }
   __syncthreads();
   // chunks that occur: a warp looks at four chunks (512 bytes) at a time
+#pragma unroll
   for (int i = warp; i < kChunks / 4; i += kSampleWarps) {
     const uint4 v = reinterpret_cast<const uint4 *>(sm.hist)[i * 32 + lane];
     const unsigned some = __ballot_sync(0xffffffffu, (v.x | v.y | v.z | v.w) != 0u);
@@ -274,22 +294,32 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
                           ((some & 0xFF0000u) != 0u ? 4u : 0u) | ((some & 0xFF000000u) != 0u ? 8u : 0u);
     if (lane == 0) sm.four[i] = static_cast<uint8_t>(four);
   }
-  if (warp == 0) {
-    const uint32_t v = __reduce_max_sync(0xffffffffu, lane < kSampleWarps ? sm.warp_max[lane] : 0u);
-    if (lane == 0) sm.max_key = v;
-  }
   __syncthreads();
-  if (tid < kChunks / 32) {
-    const uint2 v = reinterpret_cast<const uint2 *>(sm.four)[tid];
+  if (warp == 0) {
+    const uint2 v = reinterpret_cast<const uint2 *>(sm.four)[lane];
     uint32_t w = 0u;
 #pragma unroll
     for (int e = 0; e < 4; ++e) w |= ((v.x >> (8 * e)) & 15u) << (4 * e) | ((v.y >> (8 * e)) & 15u) << (16 + 4 * e);
-    sm.map[tid] = w;
+    sm.map[lane] = w;
+    // the slice's maximum: the highest value of its highest chunk
+    const unsigned words = __ballot_sync(0xffffffffu, w != 0u);
+    uint32_t best = kNegInfKey;
+    if (words != 0u) {
+      const int top = 31 - __clz(words);
+      const int c = top * 32 + 31 - __clz(__shfl_sync(0xffffffffu, w, top));
+      const uint32_t n = sm.hist[c * (kChunk / 2) + lane];
+      const uint32_t key = static_cast<uint32_t>(c * kChunk + 2 * lane) + ((n >> 16) != 0u ? 1u : 0u);
+      best = __reduce_max_sync(0xffffffffu, n != 0u ? key : 0u);
+    }
+    if (lane == 0) sm.max_key = best;
   }
   cluster.sync();
 
   uint32_t max_key = 0u;
-  for (int r = 0; r < C; ++r) max_key = max(max_key, *cluster.map_shared_rank(&sm.max_key, r));
+#pragma unroll
+  for (int r = 0; r < kSampleMaxCluster; ++r) {
+    if (r < C) max_key = max(max_key, *cluster.map_shared_rank(&sm.max_key, r));
+  }
   const float temp_f = a.temperature != nullptr ? __ldg(a.temperature + b) : 1.f;
   const float max_f = key_value(max_key);
   // max_key of NaN is 0xFFFF; +inf and -inf are not finite either
@@ -472,11 +502,18 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
     }
     if (pick_rank >= before && pick_rank < before + here) {
       uint32_t want = pick_rank - before;  // occurrence within the slice
+      // its bits: one pattern, but for zero (either sign) and NaN (many)
+      const uint32_t bits = (pick_key & 0x8000u) ? (pick_key & 0x7FFFu) : (~pick_key & 0xFFFFu);
+      const uint32_t mask = bits == 0u ? 0x7FFFu : 0xFFFFu;
+      const bool nan = pick_key == 0xFFFFu;
+      auto is = [&](uint32_t x) { return nan ? (x & 0x7FFFu) > 0x7F80u : (x & mask) == bits; };
       auto matches = [&](int v) {
-        uint32_t in, hit = 0u;
+        uint32_t in;
         const uint4 x = slice_piece(slice, v, in);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        uint32_t hit = 0u;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) hit |= (order_key(element(x, e)) == pick_key ? 1u : 0u) << e;
+        for (int e = 0; e < 4; ++e) hit |= (is(w[e] & 0xFFFFu) ? 1u << (2 * e) : 0u) | (is(w[e] >> 16) ? 2u << (2 * e) : 0u);
         return hit & in;
       };
       // a warp's part of the slice, in order of index
