@@ -344,11 +344,18 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           }
         }
       } else {
-        for (int i = tid; i < M * C; i += kThinThreads) {
-          const int r = i / C, c = i - r * C;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (r < g.rows) v = ld_act16(q_row(g, r) + c * 8);
-          *reinterpret_cast<uint4 *>(q_s + (r >> 4) * L::kHalf + chunk_at<HD>(r & 15, c)) = v;
+        constexpr int kPer = M * C / kThinThreads > 0 ? M * C / kThinThreads : 1;
+        uint4 v[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int r = (tid + i * kThinThreads) / C, c = (tid + i * kThinThreads) % C;
+          v[i] = ld_act16(q_row(g, min(r, g.rows - 1)) + c * 8);
+          if (r >= g.rows) v[i] = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int r = (tid + i * kThinThreads) / C, c = (tid + i * kThinThreads) % C;
+          if (r < M) *reinterpret_cast<uint4 *>(q_s + (r >> 4) * L::kHalf + chunk_at<HD>(r & 15, c)) = v[i];
         }
         __syncthreads();
       }
@@ -369,6 +376,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           token[n][e] = token_of(a.p, g, min(r, g.rows - 1));
         }
       }
+      const int seen_by_all = a.tree != nullptr ? g.base : g.base + g.tok0 + 1;
       float o[NQ][KS][4];  // O^T: element rows ks * 16 + g8 (+ 8), queries 2 t4 (+ 1)
       float m_run[NQ][2], l_run[NQ][2];
 #pragma unroll
@@ -416,8 +424,8 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         request_k();  // into the slot freed a half block ago
         uint32_t p[NQ][2];
         if (live) {
-          // a block that reaches the new rows, or the item's end, is masked key by key
-          const bool masked = row + 16 > g.base;
+          // a block that reaches beyond what all rows see is masked key by key
+          const bool masked = row + 16 > seen_by_all;
           bool over = false;
 #pragma unroll
           for (int n = 0; n < NQ; ++n) {

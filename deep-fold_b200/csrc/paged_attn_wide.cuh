@@ -28,7 +28,7 @@
 namespace chr {
 namespace {
 
-constexpr int kWideThreads = 320;
+constexpr int kWideThreads = 384;  // ten warps at work; three warpgroups to split the registers
 constexpr int kWideM = 256;
 constexpr int kWideTile = 128;
 
@@ -72,6 +72,9 @@ __device__ __forceinline__ bool bar_wait(WideBars &w, uint64_t *b, uint32_t pari
   atomicExch(&g_attn_paged_status, who);
   return false;
 }
+
+// A barrier of the whole block that the roles reach from different places.
+__device__ __forceinline__ void block_sync() { asm volatile("bar.sync 0;" ::: "memory"); }
 
 template <int HD>
 __global__ void __launch_bounds__(kWideThreads, 1)
@@ -137,155 +140,174 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   uint32_t n_s = 0;           // softmax role: its tiles
   uint32_t n_p[2] = {0, 0};   // product role: P tiles consumed
 
-  for (int n_now = n_segs; n_now != 0;) {
-    bool ok = true;
-
-    if (warp == 9) {
-      // ---------------- copies ----------------
-      for (int si = 0; si < n_now && ok; ++si) {
-        const Seg g = segs[si];
-        const int32_t *table = a.c.table + g.b * a.c.table_stride;
-        for (int t = g.t0; t < g.t1 && ok; ++t, ++n_kv) {
-          const int st = n_kv & 1;
-          const uint32_t ph = (n_kv >> 1) & 1;
-          // a page per lane; one past the item's rows, or that is none, is read as zeros
-          const int row = t * kWideTile + lane * box;
-          int id = a.c.n_pages;
-          bool none = false;
-          if (lane < boxes && row < g.kv_end) {
-            id = __ldg(table + (row >> shift));
-            none = id < 0 || id >= a.c.n_pages;
-            if (none) id = a.c.n_pages;
-          }
-          const uint32_t bad = __ballot_sync(0xffffffffu, none);
-          const int in_page = row & ((1 << shift) - 1);
-          if (n_kv >= 2) ok = bar_wait(w, &w.k_empty[st], ph ^ 1, 1);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (lane == 0) {
-            *reinterpret_cast<volatile uint32_t *>(&w.bad[n_kv & 3]) = bad;
-            bar_expect(&w.k_full[st], L::kTileB);
-          }
-          ++n_k;
-          __syncwarp();
-          if (lane < boxes) {
-#pragma unroll
-            for (int h = 0; h < L::kHalves; ++h) {
-              tma_page(base + L::kK + st * L::kTileB + h * L::kPiece + lane * box * 128, &k_map, &w.k_full[st], h * 64,
-                       g.kvh, in_page, id);
-            }
-          }
-          if (n_kv >= 2) ok = bar_wait(w, &w.v_empty[st], ph ^ 1, 2);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (lane == 0) bar_expect(&w.v_full[st], L::kTileB);
-          ++n_v;
-          __syncwarp();
-          if (lane < boxes) {
-#pragma unroll
-            for (int h = 0; h < L::kHalves; ++h) {
-              tma_page(base + L::kV + st * L::kTileB + h * L::kPiece + lane * box * 128, &v_map, &w.v_full[st], h * 64,
-                       g.kvh, in_page, id);
-            }
-          }
-          if ((t + 1) * kWideTile > g.kv_end) {
-            // rows behind the last may hold anything (0 x NaN): zeros for the second product
-            ok = __all_sync(0xffffffffu, bar_wait(w, &w.v_full[st], ph, 3));
-            if (!ok) break;
-            const int first = max(g.kv_end - t * kWideTile, 0);
-            for (int i = lane; i < (kWideTile - first) * 8 * L::kHalves; i += 32) {
-              const int r = first + (i >> 3) / L::kHalves, h = (i >> 3) % L::kHalves;
-              *reinterpret_cast<uint4 *>(sm + L::kV + st * L::kTileB + h * L::kPiece + r * 128 + (i & 7) * 16) =
-                  make_uint4(0, 0, 0, 0);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) bar_arrive(&w.v_fixed[st]);
-          }
-        }
-      }
-      if (!ok) {
-        // a role gave up: the copies in flight land before the CTA leaves
-        for (uint32_t i = n_k >= 2 ? n_k - 2 : 0; i < n_k; ++i) bar_poll(&w.k_full[i & 1], (i >> 1) & 1);
-        for (uint32_t i = n_v >= 2 ? n_v - 2 : 0; i < n_v; ++i) bar_poll(&w.v_full[i & 1], (i >> 1) & 1);
-      }
-    } else if (warp == 8) {
-      // ---------------- products ----------------
-      if (lane == 0) {
-        const uint32_t qk_desc = (1u << 4) | (1u << 7) | (1u << 10) | (negate ? 1u << 13 : 0u) |
-                                 (static_cast<uint32_t>(kWideTile >> 3) << 17) | (128u >> 4 << 24);
-        const uint32_t pv_desc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
-                                 (static_cast<uint32_t>(HD >> 3) << 17) | (128u >> 4 << 24);
-        auto qk = [&](int tile, int st) {
-#pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) {
-            const uint32_t off = (ks >> 2) * L::kPiece + (ks & 3) * 32;
-            tc_mma_ss(tmem + tile * 128, tc_desc(base + L::kQ + tile * L::kTileB + off, 16),
-                      tc_desc(base + L::kK + st * L::kTileB + off, 16), qk_desc, ks > 0 ? 1u : 0u);
-          }
-          tc_commit(&w.s_full[tile]);
-        };
-        auto pv = [&](int tile, int st, bool first) {
-#pragma unroll
-          for (int ks = 0; ks < kWideTile / 16; ++ks) {
-            tc_mma_ts(tmem + 256 + tile * 128, tmem + tile * 128 + ks * 8,
-                      tc_desc(base + L::kV + st * L::kTileB + ks * 16 * 128, L::kPiece), pv_desc,
-                      (!first || ks > 0) ? 1u : 0u);
-          }
-          tc_commit(&w.pv_done[tile]);
-        };
-        auto wait_p = [&](int tile) {
-          ok = ok && bar_wait(w, &w.p_full[tile], n_p[tile] & 1, 4);
-          ++n_p[tile];
-          tc_fence_after();
-        };
+  // The roles part here for good, each with its own loop over the batches of segments, so that
+  // the registers can be split: 384 threads x 168 at launch = 2 x 128 x 208 + 128 x 88.
+  auto next_batch = [&]() {
+    block_sync();
+    if (tid == 0) n_segs = w.fail != 0 ? 0 : walk_fill(a, walk, cta, G, segs);
+    block_sync();
+    const int n = n_segs;
+    block_sync();
+    return n;
+  };
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    for (int n_now = n_segs; n_now != 0; n_now = next_batch()) {
+      bool ok = true;
+      if (warp == 9) {
+        // ---------------- copies ----------------
         for (int si = 0; si < n_now && ok; ++si) {
-          const int t0 = segs[si].t0, t1 = segs[si].t1, kv_end = segs[si].kv_end;
-          const bool two = segs[si].rows > 128;
-          for (int t = t0; t < t1 && ok; ++t, ++n_kv) {
+          const Seg g = segs[si];
+          const int32_t *table = a.c.table + g.b * a.c.table_stride;
+          for (int t = g.t0; t < g.t1 && ok; ++t, ++n_kv) {
             const int st = n_kv & 1;
             const uint32_t ph = (n_kv >> 1) & 1;
-            if (t == t0) ok = bar_wait(w, &w.q_full[0], n_q[0]++ & 1, 5);
-            ok = ok && bar_wait(w, &w.k_full[st], ph, 6);
+            // a page per lane; one past the item's rows, or that is none, is read as zeros
+            const int row = t * kWideTile + lane * box;
+            int id = a.c.n_pages;
+            bool none = false;
+            if (lane < boxes && row < g.kv_end) {
+              id = __ldg(table + (row >> shift));
+              none = id < 0 || id >= a.c.n_pages;
+              if (none) id = a.c.n_pages;
+            }
+            const uint32_t bad = __ballot_sync(0xffffffffu, none);
+            const int in_page = row & ((1 << shift) - 1);
+            if (n_kv >= 2) ok = bar_wait(w, &w.k_empty[st], ph ^ 1, 1);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            tc_fence_after();
-            qk(0, st);
-            if (two) {
-              if (t > t0) {
-                wait_p(1);
-                if (!ok) break;
-                pv(1, st ^ 1, t == t0 + 1);
-                tc_commit(&w.v_empty[st ^ 1]);
-              } else {
-                ok = bar_wait(w, &w.q_full[1], n_q[1]++ & 1, 5);
-                if (!ok) break;
-                tc_fence_after();
+            if (lane == 0) {
+              *reinterpret_cast<volatile uint32_t *>(&w.bad[n_kv & 3]) = bad;
+              bar_expect(&w.k_full[st], L::kTileB);
+            }
+            ++n_k;
+            __syncwarp();
+            if (lane < boxes) {
+  #pragma unroll
+              for (int h = 0; h < L::kHalves; ++h) {
+                tma_page(base + L::kK + st * L::kTileB + h * L::kPiece + lane * box * 128, &k_map, &w.k_full[st], h * 64,
+                         g.kvh, in_page, id);
               }
-              qk(1, st);
             }
-            tc_commit(&w.k_empty[st]);
-            ok = bar_wait(w, &w.v_full[st], ph, 7);
-            if (ok && (t + 1) * kWideTile > kv_end) {
-              ok = bar_wait(w, &w.v_fixed[st], (fixed >> st) & 1u, 8);
-              fixed ^= 1u << st;
+            if (n_kv >= 2) ok = bar_wait(w, &w.v_empty[st], ph ^ 1, 2);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (lane == 0) bar_expect(&w.v_full[st], L::kTileB);
+            ++n_v;
+            __syncwarp();
+            if (lane < boxes) {
+  #pragma unroll
+              for (int h = 0; h < L::kHalves; ++h) {
+                tma_page(base + L::kV + st * L::kTileB + h * L::kPiece + lane * box * 128, &v_map, &w.v_full[st], h * 64,
+                         g.kvh, in_page, id);
+              }
             }
-            if (!ok) break;
-            wait_p(0);
-            if (!ok) break;
-            pv(0, st, t == t0);
-            if (!two) tc_commit(&w.v_empty[st]);
-          }
-          if (ok && two) {
-            wait_p(1);
-            if (!ok) break;
-            const int st = (n_kv - 1) & 1;
-            pv(1, st, t1 == t0 + 1);
-            tc_commit(&w.v_empty[st]);
+            if ((t + 1) * kWideTile > g.kv_end) {
+              // rows behind the last may hold anything (0 x NaN): zeros for the second product
+              ok = __all_sync(0xffffffffu, bar_wait(w, &w.v_full[st], ph, 3));
+              if (!ok) break;
+              const int first = max(g.kv_end - t * kWideTile, 0);
+              for (int i = lane; i < (kWideTile - first) * 8 * L::kHalves; i += 32) {
+                const int r = first + (i >> 3) / L::kHalves, h = (i >> 3) % L::kHalves;
+                *reinterpret_cast<uint4 *>(sm + L::kV + st * L::kTileB + h * L::kPiece + r * 128 + (i & 7) * 16) =
+                    make_uint4(0, 0, 0, 0);
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) bar_arrive(&w.v_fixed[st]);
+            }
           }
         }
+        if (!ok) {
+          // a role gave up: the copies in flight land before the CTA leaves
+          for (uint32_t i = n_k >= 2 ? n_k - 2 : 0; i < n_k; ++i) bar_poll(&w.k_full[i & 1], (i >> 1) & 1);
+          for (uint32_t i = n_v >= 2 ? n_v - 2 : 0; i < n_v; ++i) bar_poll(&w.v_full[i & 1], (i >> 1) & 1);
+        }
+      } else if (warp == 8) {
+        // ---------------- products ----------------
+        if (lane == 0) {
+          const uint32_t qk_desc = (1u << 4) | (1u << 7) | (1u << 10) | (negate ? 1u << 13 : 0u) |
+                                   (static_cast<uint32_t>(kWideTile >> 3) << 17) | (128u >> 4 << 24);
+          const uint32_t pv_desc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
+                                   (static_cast<uint32_t>(HD >> 3) << 17) | (128u >> 4 << 24);
+          // operand descriptors by stage; a step of 16 elements adds a constant
+          const uint64_t q_desc = tc_desc(base + L::kQ, 16), k_desc = tc_desc(base + L::kK, 16);
+          const uint64_t v_desc = tc_desc(base + L::kV, L::kPiece);
+          auto qk = [&](int tile, int st) {
+            const uint64_t qd = q_desc + (tile * L::kTileB >> 4), kd = k_desc + (st * L::kTileB >> 4);
+  #pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks) {
+              const uint32_t off = ((ks >> 2) * L::kPiece + (ks & 3) * 32) >> 4;
+              tc_mma_ss(tmem + tile * 128, qd + off, kd + off, qk_desc, ks > 0 ? 1u : 0u);
+            }
+            tc_commit(&w.s_full[tile]);
+          };
+          auto pv = [&](int tile, int st, bool first) {
+            const uint64_t vd = v_desc + (st * L::kTileB >> 4);
+  #pragma unroll
+            for (int ks = 0; ks < kWideTile / 16; ++ks) {
+              tc_mma_ts(tmem + 256 + tile * 128, tmem + tile * 128 + ks * 8, vd + (ks * 16 * 128 >> 4), pv_desc,
+                        (!first || ks > 0) ? 1u : 0u);
+            }
+            tc_commit(&w.pv_done[tile]);
+          };
+          auto wait_p = [&](int tile) {
+            ok = ok && bar_wait(w, &w.p_full[tile], n_p[tile] & 1, 4);
+            ++n_p[tile];
+            tc_fence_after();
+          };
+          for (int si = 0; si < n_now && ok; ++si) {
+            const int t0 = segs[si].t0, t1 = segs[si].t1, kv_end = segs[si].kv_end;
+            const bool two = segs[si].rows > 128;
+            for (int t = t0; t < t1 && ok; ++t, ++n_kv) {
+              const int st = n_kv & 1;
+              const uint32_t ph = (n_kv >> 1) & 1;
+              if (t == t0) ok = bar_wait(w, &w.q_full[0], n_q[0]++ & 1, 5);
+              ok = ok && bar_wait(w, &w.k_full[st], ph, 6);
+              if (!ok) break;
+              tc_fence_after();
+              qk(0, st);
+              if (two) {
+                if (t > t0) {
+                  wait_p(1);
+                  if (!ok) break;
+                  pv(1, st ^ 1, t == t0 + 1);
+                  tc_commit(&w.v_empty[st ^ 1]);
+                } else {
+                  ok = bar_wait(w, &w.q_full[1], n_q[1]++ & 1, 5);
+                  if (!ok) break;
+                  tc_fence_after();
+                }
+                qk(1, st);
+              }
+              tc_commit(&w.k_empty[st]);
+              ok = bar_wait(w, &w.v_full[st], ph, 7);
+              if (ok && (t + 1) * kWideTile > kv_end) {
+                ok = bar_wait(w, &w.v_fixed[st], (fixed >> st) & 1u, 8);
+                fixed ^= 1u << st;
+              }
+              if (!ok) break;
+              wait_p(0);
+              if (!ok) break;
+              pv(0, st, t == t0);
+              if (!two) tc_commit(&w.v_empty[st]);
+            }
+            if (ok && two) {
+              wait_p(1);
+              if (!ok) break;
+              const int st = (n_kv - 1) & 1;
+              pv(1, st, t1 == t0 + 1);
+              tc_commit(&w.v_empty[st]);
+            }
+          }
+        }
+        __syncwarp();
       }
-      __syncwarp();
-    } else {
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    for (int n_now = n_segs; n_now != 0; n_now = next_batch()) {
+      bool ok = true;
       // ---------------- softmax: a thread per query row ----------------
       const int tile = warp >> 2;
       const int r = tid & 127;  // row of the tile, and lane of tensor memory
@@ -301,28 +323,47 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         if (g.rows <= first_row) continue;
         // the item's queries, K-major with the 128-byte swizzle, zeros past the last row
         {
-          constexpr int C = HD / 8;
-#pragma unroll 4
-          for (int i = r; i < 128 * C; i += 128) {
-            const int qr = i / C, c = i % C;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (first_row + qr < g.rows) {
-              const int token = token_of(a.p, g, first_row + qr);
-              const int head = head_of(a.p, g, first_row + qr, token);
-              v = ld_act16(a.q + (g.r0 + token) * a.q_stride + head * HD + c * 8);
+          // chunk c of rows qr0, qr0 + step, ...; eight requests before the first store
+          constexpr int C = HD / 8, step = 128 / C;
+          const int c = r % C, qr0 = r / C;
+          unsigned char *dst = sm + L::kQ + tile * L::kTileB + (c >> 3) * L::kPiece;
+#pragma unroll 1
+          for (int i0 = 0; i0 < C; i0 += 8) {
+            uint4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int qr = first_row + qr0 + (i0 + i) * step;
+              const int token = token_of(a.p, g, min(qr, g.rows - 1));
+              const int head = head_of(a.p, g, min(qr, g.rows - 1), token);
+              v[i] = ld_act16(a.q + (g.r0 + token) * a.q_stride + head * HD + c * 8);
+              if (qr >= g.rows) v[i] = make_uint4(0, 0, 0, 0);
             }
-            *reinterpret_cast<uint4 *>(sm + L::kQ + tile * L::kTileB + (c >> 3) * L::kPiece + qr * 128 +
-                                       (((c & 7) ^ (qr & 7)) << 4)) = v;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int qr = qr0 + (i0 + i) * step;
+              *reinterpret_cast<uint4 *>(dst + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = v[i];
+            }
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           bar_arrive(&w.q_full[tile]);
         }
         const bool mine = first_row + r < g.rows;
         const int token = token_of(a.p, g, min(first_row + r, g.rows - 1));
+        // cache rows that all of this warp's rows see: the older ones and, causally, the new ones
+        // up to its first row's token
+        const int seen_by_all =
+            a.tree != nullptr ? g.base : g.base + token_of(a.p, g, min(first_row + (warp & 3) * 32, g.rows - 1)) + 1;
         float m_run = -INFINITY, l_run = 0.f;
         const float c2 = a.c2;
 
         for (int t = g.t0; t < g.t1; ++t) {
+          // what the row sees of a tile that not all rows see whole, while the product runs
+          const bool masked = (t + 1) * kWideTile > seen_by_all;
+          uint32_t see[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+          if (masked) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) see[k] = seen32(a, g, token, t * kWideTile + k * 32);
+          }
           ok = __all_sync(0xffffffffu, bar_wait(w, &w.s_full[tile], n_s & 1, 9));
           if (!ok) break;
           tc_fence_after();
@@ -334,10 +375,10 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           tmem_wait_ld();
           const uint32_t bad =
               *reinterpret_cast<volatile uint32_t *>(&w.bad[(n_kv + tiles_before + (t - g.t0)) & 3]);
-          if ((t + 1) * kWideTile > g.base || bad != 0u) {
+          if (masked || bad != 0u) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              uint32_t m = seen32(a, g, token, t * kWideTile + k * 32);
+              uint32_t m = see[k];
               if (bad != 0u) {
                 for (int i = 0; i < 32; ++i) {
                   if ((bad >> ((k * 32 + i) / box)) & 1u) m &= ~(1u << i);
@@ -349,15 +390,13 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
               }
             }
           }
-          float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+          float mx0 = __uint_as_float(s[0]), mx1 = __uint_as_float(s[1]);
 #pragma unroll
-          for (int e = 0; e < 128; e += 4) {
-            mx0 = fmaxf(mx0, __uint_as_float(s[e]));
-            mx1 = fmaxf(mx1, __uint_as_float(s[e + 1]));
-            mx2 = fmaxf(mx2, __uint_as_float(s[e + 2]));
-            mx3 = fmaxf(mx3, __uint_as_float(s[e + 3]));
+          for (int e = 2; e < 126; e += 4) {
+            mx0 = max3(mx0, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+            mx1 = max3(mx1, __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
           }
-          const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c2;
+          const float mx = max3(fmaxf(mx0, mx1), __uint_as_float(s[126]), __uint_as_float(s[127])) * c2;
           // raise the subtracted maximum only when it is far behind
           const bool raise = mx > m_run + 8.f || m_run == -INFINITY;
           const float m_new = raise ? fmaxf(mx, m_run) : m_run;
@@ -366,18 +405,19 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           m_run = m_new;
           const float m_use = m_new == -INFINITY ? 0.f : m_new;
           const f32x2_t c22 = pack_f32x2(c2, c2), mm2 = pack_f32x2(-m_use, -m_use);
-          float sum0 = 0.f, sum1 = 0.f;
+          f32x2_t sum2 = pack_f32x2(0.f, 0.f);
 #pragma unroll
           for (int e = 0; e < 128; e += 2) {
             float p0, p1;
             unpack_f32x2(ffma2(pack_f32x2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c22, mm2), p0, p1);
             p0 = fast_exp2(p0);
             p1 = fast_exp2(p1);
-            sum0 += p0;
-            sum1 += p1;
+            sum2 = add2(sum2, pack_f32x2(p0, p1));
             const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);
             s[e >> 1] = *reinterpret_cast<const uint32_t *>(&v);
           }
+          float sum0, sum1;
+          unpack_f32x2(sum2, sum0, sum1);
           l_run = fmaf(l_run, alpha, sum0 + sum1);
           tmem_st32(s_addr, s);
           tmem_st32(s_addr + 32, s + 32);
@@ -443,14 +483,9 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
       n_kv += seg_tiles;
     }
-    __syncthreads();
-    if (tid == 0) n_segs = w.fail != 0 ? 0 : walk_fill(a, walk, cta, G, segs);
-    __syncthreads();
-    n_now = n_segs;
-    __syncthreads();
   }
   tc_fence_before();
-  __syncthreads();
+  block_sync();
   tc_fence_after();
   if (warp == 8) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
