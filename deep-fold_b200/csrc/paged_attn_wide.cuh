@@ -11,7 +11,10 @@
 // The order of issue is QK0(i) PV1(i-1) QK1(i) PV0(i): while one tile's softmax runs the
 // other's products do. Both sides need about 2048 clocks per key tile (4 products of
 // 128^3 at 4096 multiply-adds a clock; 32768 exp2 at 16 a clock), so overlap is what
-// counts. The running maximum a row subtracts is raised only when the new one is more than 8
+// counts: P goes over in halves, so that its product starts under the second half's exps,
+// and three exps of eight are taken on the FMA pipe (Cody and Waite's reduction to
+// |f| <= 1/2, a cubic fitted to 2^f for least relative error, 7.5e-5: a fiftieth of the rounding
+// of P to bf16 that follows). The running maximum a row subtracts is raised only when the new one is more than 8
 // (in log2) above it: P then stays below 2^8, which bf16 holds as exactly as 1, and the
 // accumulator in tensor memory is almost never rescaled.
 // P is rounded to bf16 for the second product, its sum is not; everything else is FP32.
@@ -47,7 +50,7 @@ struct WideLayout {
 
 struct WideBars {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], v_fixed[2];
-  uint64_t s_full[2], p_full[2], pv_done[2], q_full[2];
+  uint64_t s_full[2], p_half[2], p_full[2], pv_done[2], q_full[2];
   uint32_t bad[4];  // pages of the last tiles that are none, a bit per page
   uint32_t tmem;
   int fail;
@@ -76,6 +79,11 @@ __device__ __forceinline__ bool bar_wait(WideBars &w, uint64_t *b, uint32_t pari
 // A barrier of the whole block that the roles reach from different places.
 __device__ __forceinline__ void block_sync() { asm volatile("bar.sync 0;" ::: "memory"); }
 
+template <bool B>
+struct BoolC {
+  static constexpr bool value = B;
+};
+
 template <int HD>
 __global__ void __launch_bounds__(kWideThreads, 1)
 attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -99,6 +107,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       bar_init(&w.v_full[i], 1);
       bar_init(&w.v_empty[i], 1);
       bar_init(&w.s_full[i], 1);
+      bar_init(&w.p_half[i], 128);
       bar_init(&w.p_full[i], 128);
       bar_init(&w.pv_done[i], 1);
       bar_init(&w.q_full[i], 128);
@@ -224,84 +233,88 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           for (uint32_t i = n_v >= 2 ? n_v - 2 : 0; i < n_v; ++i) bar_poll(&w.v_full[i & 1], (i >> 1) & 1);
         }
       } else if (warp == 8) {
-        // ---------------- products ----------------
-        if (lane == 0) {
-          const uint32_t qk_desc = (1u << 4) | (1u << 7) | (1u << 10) | (negate ? 1u << 13 : 0u) |
-                                   (static_cast<uint32_t>(kWideTile >> 3) << 17) | (128u >> 4 << 24);
-          const uint32_t pv_desc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
-                                   (static_cast<uint32_t>(HD >> 3) << 17) | (128u >> 4 << 24);
-          // operand descriptors by stage; a step of 16 elements adds a constant
-          const uint64_t q_desc = tc_desc(base + L::kQ, 16), k_desc = tc_desc(base + L::kK, 16);
-          const uint64_t v_desc = tc_desc(base + L::kV, L::kPiece);
-          auto qk = [&](int tile, int st) {
-            const uint64_t qd = q_desc + (tile * L::kTileB >> 4), kd = k_desc + (st * L::kTileB >> 4);
-  #pragma unroll
+        // ---------------- products: a converged warp, one elected thread issues ----------------
+        const uint32_t qk_desc = (1u << 4) | (1u << 7) | (1u << 10) | (negate ? 1u << 13 : 0u) |
+                                 (static_cast<uint32_t>(kWideTile >> 3) << 17) | (128u >> 4 << 24);
+        const uint32_t pv_desc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
+                                 (static_cast<uint32_t>(HD >> 3) << 17) | (128u >> 4 << 24);
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        // operand descriptors of the first stage; a step of 16 elements adds a constant
+        const uint64_t q_desc = tc_desc(base + L::kQ, 16), k_desc = tc_desc(base + L::kK, 16);
+        const uint64_t v_desc = tc_desc(base + L::kV, L::kPiece);
+        auto wait = [&](uint64_t *bar, uint32_t parity, int who) {
+          ok = __all_sync(0xffffffffu, bar_wait(w, bar, parity, who));
+          tc_fence_after();
+        };
+        auto qk = [&](int tile, int st) {
+          const uint64_t qd = q_desc + (tile * L::kTileB >> 4), kd = k_desc + (st * L::kTileB >> 4);
+          if (elect_one()) {
+#pragma unroll
             for (int ks = 0; ks < HD / 16; ++ks) {
               const uint32_t off = ((ks >> 2) * L::kPiece + (ks & 3) * 32) >> 4;
-              tc_mma_ss(tmem + tile * 128, qd + off, kd + off, qk_desc, ks > 0 ? 1u : 0u);
+              tc_mma_ss(tm + tile * 128, qd + off, kd + off, qk_desc, ks > 0 ? 1u : 0u);
             }
             tc_commit(&w.s_full[tile]);
-          };
-          auto pv = [&](int tile, int st, bool first) {
-            const uint64_t vd = v_desc + (st * L::kTileB >> 4);
-  #pragma unroll
-            for (int ks = 0; ks < kWideTile / 16; ++ks) {
-              tc_mma_ts(tmem + 256 + tile * 128, tmem + tile * 128 + ks * 8, vd + (ks * 16 * 128 >> 4), pv_desc,
-                        (!first || ks > 0) ? 1u : 0u);
-            }
-            tc_commit(&w.pv_done[tile]);
-          };
-          auto wait_p = [&](int tile) {
-            ok = ok && bar_wait(w, &w.p_full[tile], n_p[tile] & 1, 4);
-            ++n_p[tile];
-            tc_fence_after();
-          };
-          for (int si = 0; si < n_now && ok; ++si) {
-            const int t0 = segs[si].t0, t1 = segs[si].t1, kv_end = segs[si].kv_end;
-            const bool two = segs[si].rows > 128;
-            for (int t = t0; t < t1 && ok; ++t, ++n_kv) {
-              const int st = n_kv & 1;
-              const uint32_t ph = (n_kv >> 1) & 1;
-              if (t == t0) ok = bar_wait(w, &w.q_full[0], n_q[0]++ & 1, 5);
-              ok = ok && bar_wait(w, &w.k_full[st], ph, 6);
-              if (!ok) break;
-              tc_fence_after();
-              qk(0, st);
-              if (two) {
-                if (t > t0) {
-                  wait_p(1);
-                  if (!ok) break;
-                  pv(1, st ^ 1, t == t0 + 1);
-                  tc_commit(&w.v_empty[st ^ 1]);
-                } else {
-                  ok = bar_wait(w, &w.q_full[1], n_q[1]++ & 1, 5);
-                  if (!ok) break;
-                  tc_fence_after();
-                }
-                qk(1, st);
-              }
-              tc_commit(&w.k_empty[st]);
-              ok = bar_wait(w, &w.v_full[st], ph, 7);
-              if (ok && (t + 1) * kWideTile > kv_end) {
-                ok = bar_wait(w, &w.v_fixed[st], (fixed >> st) & 1u, 8);
-                fixed ^= 1u << st;
-              }
-              if (!ok) break;
-              wait_p(0);
-              if (!ok) break;
-              pv(0, st, t == t0);
-              if (!two) tc_commit(&w.v_empty[st]);
-            }
-            if (ok && two) {
-              wait_p(1);
-              if (!ok) break;
-              const int st = (n_kv - 1) & 1;
-              pv(1, st, t1 == t0 + 1);
-              tc_commit(&w.v_empty[st]);
+          }
+          __syncwarp();
+        };
+        // O += P V once the halves of P are there; the V tile has been waited for. `last`: the
+        // stage's last product.
+        auto pv = [&](int tile, int st, bool first, bool last) {
+          const uint64_t vd = v_desc + (st * L::kTileB >> 4);
+          const uint32_t par = n_p[tile]++ & 1;
+          const uint32_t d = tm + 256 + tile * 128, p = tm + tile * 128;
+          wait(&w.p_half[tile], par, 4);
+          if (!ok) return;
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+              tc_mma_ts(d, p + ks * 8, vd + (ks * 16 * 128 >> 4), pv_desc, (!first || ks > 0) ? 1u : 0u);
             }
           }
+          __syncwarp();
+          wait(&w.p_full[tile], par, 5);
+          if (!ok) return;
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = 4; ks < 8; ++ks) tc_mma_ts(d, p + ks * 8, vd + (ks * 16 * 128 >> 4), pv_desc, 1u);
+            tc_commit(&w.pv_done[tile]);
+            if (last) tc_commit(&w.v_empty[st]);
+          }
+          __syncwarp();
+        };
+        for (int si = 0; si < n_now && ok; ++si) {
+          const int t0 = segs[si].t0, t1 = segs[si].t1, kv_end = segs[si].kv_end;
+          const bool two = segs[si].rows > 128;
+          for (int t = t0; t < t1; ++t, ++n_kv) {
+            const int st = n_kv & 1;
+            const uint32_t ph = (n_kv >> 1) & 1;
+            if (t == t0) wait(&w.q_full[0], n_q[0]++ & 1, 6);
+            if (ok) wait(&w.k_full[st], ph, 7);
+            if (!ok) break;
+            qk(0, st);
+            if (two) {
+              if (t > t0) {
+                pv(1, st ^ 1, t == t0 + 1, true);
+              } else {
+                wait(&w.q_full[1], n_q[1]++ & 1, 6);
+              }
+              if (!ok) break;
+              qk(1, st);
+            }
+            if (elect_one()) tc_commit(&w.k_empty[st]);
+            __syncwarp();
+            wait(&w.v_full[st], ph, 8);
+            if (ok && (t + 1) * kWideTile > kv_end) {
+              wait(&w.v_fixed[st], (fixed >> st) & 1u, 9);
+              fixed ^= 1u << st;
+            }
+            if (!ok) break;
+            pv(0, st, t == t0, !two);
+            if (!ok) break;
+          }
+          if (ok && two) pv(1, (n_kv - 1) & 1, t1 == t0 + 1, true);
         }
-        __syncwarp();
       }
     }
   } else {
@@ -315,38 +328,38 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       const uint32_t s_addr = tmem + quad + tile * 128;
       const uint32_t o_addr = tmem + quad + 256 + tile * 128;
       uint32_t seg_tiles = 0;  // key tiles of this batch before the segment
+      const int first_row = tile * 128;
+      // An item's queries to shared memory, K-major with the 128-byte swizzle, zeros past the last
+      // row: chunk c of rows qr0, qr0 + step, ...; all requests before the first store. The
+      // tile's last product with the queries before has been waited for (its scores are here).
+      bool q_ahead = false;  // the next segment's are there already
+      auto load_q = [&](const Seg &g) {
+        constexpr int C = HD / 8, step = 128 / C;
+        const int c = r % C, qr0 = r / C;
+        unsigned char *dst = sm + L::kQ + tile * L::kTileB + (c >> 3) * L::kPiece;
+        uint4 v[C];
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          const int qr = first_row + qr0 + i * step;
+          const int token = token_of(a.p, g, min(qr, g.rows - 1));
+          const int head = head_of(a.p, g, min(qr, g.rows - 1), token);
+          v[i] = ld_act16(a.q + (g.r0 + token) * a.q_stride + head * HD + c * 8);
+          if (qr >= g.rows) v[i] = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          const int qr = qr0 + i * step;
+          *reinterpret_cast<uint4 *>(dst + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = v[i];
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        bar_arrive(&w.q_full[tile]);
+      };
       for (int si = 0; si < n_now && ok; ++si) {
         const Seg g = segs[si];
-        const int first_row = tile * 128;
         const uint32_t tiles_before = seg_tiles;
         seg_tiles += g.t1 - g.t0;
         if (g.rows <= first_row) continue;
-        // the item's queries, K-major with the 128-byte swizzle, zeros past the last row
-        {
-          // chunk c of rows qr0, qr0 + step, ...; eight requests before the first store
-          constexpr int C = HD / 8, step = 128 / C;
-          const int c = r % C, qr0 = r / C;
-          unsigned char *dst = sm + L::kQ + tile * L::kTileB + (c >> 3) * L::kPiece;
-#pragma unroll 1
-          for (int i0 = 0; i0 < C; i0 += 8) {
-            uint4 v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int qr = first_row + qr0 + (i0 + i) * step;
-              const int token = token_of(a.p, g, min(qr, g.rows - 1));
-              const int head = head_of(a.p, g, min(qr, g.rows - 1), token);
-              v[i] = ld_act16(a.q + (g.r0 + token) * a.q_stride + head * HD + c * 8);
-              if (qr >= g.rows) v[i] = make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int qr = qr0 + (i0 + i) * step;
-              *reinterpret_cast<uint4 *>(dst + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = v[i];
-            }
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          bar_arrive(&w.q_full[tile]);
-        }
+        if (!q_ahead) load_q(g);
         const bool mine = first_row + r < g.rows;
         const int token = token_of(a.p, g, min(first_row + r, g.rows - 1));
         // cache rows that all of this warp's rows see: the older ones and, causally, the new ones
@@ -364,7 +377,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 #pragma unroll
             for (int k = 0; k < 4; ++k) see[k] = seen32(a, g, token, t * kWideTile + k * 32);
           }
-          ok = __all_sync(0xffffffffu, bar_wait(w, &w.s_full[tile], n_s & 1, 9));
+          ok = __all_sync(0xffffffffu, bar_wait(w, &w.s_full[tile], n_s & 1, 10));
           if (!ok) break;
           tc_fence_after();
           uint32_t s[128];
@@ -396,55 +409,77 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             mx0 = max3(mx0, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
             mx1 = max3(mx1, __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
           }
-          const float mx = max3(fmaxf(mx0, mx1), __uint_as_float(s[126]), __uint_as_float(s[127])) * c2;
+          const float mx = max3(max3(mx0, mx1, mx1), __uint_as_float(s[126]), __uint_as_float(s[127])) * c2;
           // raise the subtracted maximum only when it is far behind
           const bool raise = mx > m_run + 8.f || m_run == -INFINITY;
           const float m_new = raise ? fmaxf(mx, m_run) : m_run;
           const float alpha = raise ? (m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new)) : 1.f;
           const bool turn_down = raise && m_run != -INFINITY;
+          // scores of -inf (hidden), +inf or NaN: not for the exps on the FMA pipe
+          bool exact = masked || bad != 0u;
+          if (__any_sync(0xffffffffu, turn_down || !(mx < INFINITY))) {
+            exact = exact || __any_sync(0xffffffffu, !(mx < INFINITY));
+            // the accumulator is this thread's once the last product into it is done
+            ok = __all_sync(0xffffffffu, bar_wait(w, &w.pv_done[tile], (n_s & 1) ^ 1, 11));
+            if (!ok) break;
+            tc_fence_after();
+            const float by = turn_down ? alpha : 1.f;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(o_addr + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
+              tmem_st16(o_addr + c, o);
+            }
+            tmem_wait_st();
+          }
           m_run = m_new;
           const float m_use = m_new == -INFINITY ? 0.f : m_new;
           const f32x2_t c22 = pack_f32x2(c2, c2), mm2 = pack_f32x2(-m_use, -m_use);
           f32x2_t sum2 = pack_f32x2(0.f, 0.f);
+          // a half of the row's exps, in place as bf16 pairs, and over to the product
+          auto half = [&](int e0, auto on_fma) {
 #pragma unroll
-          for (int e = 0; e < 128; e += 2) {
-            float p0, p1;
-            unpack_f32x2(ffma2(pack_f32x2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c22, mm2), p0, p1);
-            p0 = fast_exp2(p0);
-            p1 = fast_exp2(p1);
-            sum2 = add2(sum2, pack_f32x2(p0, p1));
-            const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);
-            s[e >> 1] = *reinterpret_cast<const uint32_t *>(&v);
+            for (int i = 0; i < 64; i += 2) {
+              const int e = e0 + i;
+              f32x2_t x = ffma2(pack_f32x2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c22, mm2);
+              float p0, p1;
+              if (decltype(on_fma)::value && (i >> 1) % 8 < 3) {
+                exp2_fma(x, p0, p1);
+              } else {
+                unpack_f32x2(x, p0, p1);
+                p0 = fast_exp2(p0);
+                p1 = fast_exp2(p1);
+              }
+              sum2 = add2(sum2, pack_f32x2(p0, p1));
+              const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);
+              s[e >> 1] = *reinterpret_cast<const uint32_t *>(&v);
+            }
+            tmem_st32(s_addr + (e0 >> 1), s + (e0 >> 1));
+            tmem_wait_st();
+            tc_fence_before();
+            bar_arrive(e0 == 0 ? &w.p_half[tile] : &w.p_full[tile]);
+          };
+          if (exact) {
+            half(0, BoolC<false>());
+            half(64, BoolC<false>());
+          } else {
+            half(0, BoolC<true>());
+            half(64, BoolC<true>());
           }
           float sum0, sum1;
           unpack_f32x2(sum2, sum0, sum1);
           l_run = fmaf(l_run, alpha, sum0 + sum1);
-          tmem_st32(s_addr, s);
-          tmem_st32(s_addr + 32, s + 32);
-          if (__any_sync(0xffffffffu, turn_down)) {
-            // the accumulator is this thread's once the last product into it is done
-            ok = __all_sync(0xffffffffu, bar_wait(w, &w.pv_done[tile], (n_s & 1) ^ 1, 10));
-            if (!ok) break;
-            tc_fence_after();
-            const float by = turn_down ? alpha : 1.f;
-#pragma unroll
-            for (int c = 0; c < HD; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(o_addr + c, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
-              tmem_st32(o_addr + c, o);
-            }
-          }
-          tmem_wait_st();
-          tc_fence_before();
-          bar_arrive(&w.p_full[tile]);
           ++n_s;
         }
         if (!ok) break;
+        // the next segment's queries, so that its first products run under what follows
+        q_ahead = si + 1 < n_now && segs[si + 1].rows > first_row;
+        if (q_ahead) load_q(segs[si + 1]);
         // ---- the segment's result ----
-        ok = __all_sync(0xffffffffu, bar_wait(w, &w.pv_done[tile], (n_s & 1) ^ 1, 11));
+        ok = __all_sync(0xffffffffu, bar_wait(w, &w.pv_done[tile], (n_s & 1) ^ 1, 12));
         if (!ok) break;
         tc_fence_after();
         const bool whole = g.whole;
