@@ -126,35 +126,15 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
-// The largest of three, NaN if one is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 __device__ __forceinline__ f32x2_t add2(f32x2_t a, f32x2_t b) {
   f32x2_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
-}
-// 2^x of a pair without the special-function unit: x = n + f with n the nearest integer (from the
-// low bits of x + 1.5 2^23), 2^f by a cubic, n added to the exponent.
-// Below -125 it gives 2^-125; x is finite.
-__device__ __forceinline__ void exp2_fma(f32x2_t x, float &y0, float &y1) {
-  float x0, x1;
-  unpack_f32x2(x, x0, x1);
-  x = pack_f32x2(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
-  const f32x2_t t = add2(x, pack_f32x2(12582912.f, 12582912.f));
-  const f32x2_t n = add2(t, pack_f32x2(-12582912.f, -12582912.f));
-  const f32x2_t f = ffma2(n, pack_f32x2(-1.f, -1.f), x);
-  f32x2_t p = ffma2(f, pack_f32x2(0.0551716685f, 0.0551716685f), pack_f32x2(0.2426111251f, 0.2426111251f));
-  p = ffma2(p, f, pack_f32x2(0.6932609677f, 0.6932609677f));
-  p = ffma2(p, f, pack_f32x2(0.9999280572f, 0.9999280572f));
-  float t0, t1, p0, p1;
-  unpack_f32x2(t, t0, t1);
-  unpack_f32x2(p, p0, p1);
-  y0 = __uint_as_float((__float_as_uint(t0) << 23) + __float_as_uint(p0));
-  y1 = __uint_as_float((__float_as_uint(t1) << 23) + __float_as_uint(p1));
 }
 #undef CHR_R8
 #undef CHR_I8
