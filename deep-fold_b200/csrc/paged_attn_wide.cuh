@@ -5,14 +5,16 @@
 // 128-row tiles, so that a cache row crosses from L2 once per 256 query rows (two CTAs of
 // 128 rows each would need 64 bytes per clock and SM, more than L2 delivers to all SMs).
 //   warp 9      page look-up and TMA copies of K and V pages (two stages each)
-//   warp 8      issues tcgen05.mma: S_w = Q_w K^T (128 x 128, FP32, tensor memory) and
-//               O_w += P_w V, P_w read from tensor memory, where it lies over S_w
+//   warp 8      issues tcgen05.mma in steps of 64 cache rows: S_w = Q_w K^T (128 x 64, FP32, tensor
+//               memory) and O_w += P_w V, P_w read from tensor memory, where it lies over S_w
 //   warps 0-3   softmax of tile 0, warps 4-7 of tile 1: a thread owns a row
-// The order of issue is QK0(i) PV1(i-1) QK1(i) PV0(i): while one tile's softmax runs the
-// other's products do. Both sides need about 2048 clocks per key tile (4 products of
-// 128^3 at 4096 multiply-adds a clock; 32768 exp2 at 16 a clock), so overlap is what
-// counts: P goes over in halves, so that its product starts under the second half's exps.
-// The running maximum a row subtracts is raised only when the new one is more than 8
+// Each tile has two S buffers (2 x 2 x 64 columns; the accumulators take the other 256): the
+// order of issue is PV0(j) QK0(j+2) PV1(j) QK1(j+2), so the scores of the next step are there
+// when a softmax ends and neither side waits for the other's latency. Per 128 cache rows the
+// products take 2 x (2 x 8 x 48 + 8 x 64) = 2560 clocks - the 128 x 64 one is held up by the
+// 128 bytes a clock its operands are read at, hence 48 - and the exps 2048 (32768 at 16 a clock).
+// (With one S buffer of 128 columns per tile, products 2048 clocks, the chain of both was 4100.) The running
+// maximum a row subtracts is raised only when the new one is more than 8
 // (in log2) above it: P then stays below 2^8, which bf16 holds as exactly as 1, and the
 // accumulator in tensor memory is almost never rescaled.
 // P is rounded to bf16 for the second product, its sum is not; everything else is FP32.
@@ -29,9 +31,10 @@
 namespace chr {
 namespace {
 
-constexpr int kWideThreads = 384;  // ten warps at work; three warpgroups to split the registers
+constexpr int kWideThreads = 320;
 constexpr int kWideM = 256;
 constexpr int kWideTile = 128;
+constexpr int kWideStep = 64;   // cache rows of one product
 
 template <int HD>
 struct WideLayout {
@@ -48,7 +51,8 @@ struct WideLayout {
 
 struct WideBars {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], v_fixed[2];
-  uint64_t s_full[2], p_half[2], p_full[2], pv_done[2], q_full[2];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [query tile][buffer]
+  uint64_t q_full[2];
   uint32_t bad[4];  // pages of the last tiles that are none, a bit per page
   uint32_t tmem;
   int fail;
@@ -110,10 +114,11 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       bar_init(&w.k_empty[i], 1);
       bar_init(&w.v_full[i], 1);
       bar_init(&w.v_empty[i], 1);
-      bar_init(&w.s_full[i], 1);
-      bar_init(&w.p_half[i], 128);
-      bar_init(&w.p_full[i], 128);
-      bar_init(&w.pv_done[i], 1);
+      for (int j = 0; j < 2; ++j) {
+        bar_init(&w.s_full[i][j], 1);
+        bar_init(&w.p_full[i][j], 128);
+        bar_init(&w.pv_done[i][j], 1);
+      }
       bar_init(&w.q_full[i], 128);
       bar_init(&w.v_fixed[i], 1);
     }
@@ -150,11 +155,10 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   uint32_t n_k = 0, n_v = 0;  // copy role: tiles requested
   uint32_t fixed = 0;         // product role: parity of each stage's zeroed tails
   uint32_t n_q[2] = {0, 0};   // segments a query tile took part in
-  uint32_t n_s = 0;           // softmax role: its tiles
-  uint32_t n_p[2] = {0, 0};   // product role: P tiles consumed
+  uint32_t n_s = 0;           // softmax role: steps of its query tile; product role: pairs of tile 0
+  uint32_t n_s1 = 0;          // product role: pairs of steps of query tile 1
 
-  // The roles part here for good, each with its own loop over the batches of segments, so that
-  // the registers can be split: 384 threads x 168 at launch = 2 x 128 x 208 + 128 x 88.
+  // The roles part here for good, each with its own loop over the batches of segments.
   auto next_batch = [&]() {
     block_sync();
     if (tid == 0) n_segs = w.fail != 0 ? 0 : walk_fill(a, walk, cta, G, segs);
@@ -164,7 +168,6 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     return n;
   };
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     for (int n_now = n_segs; n_now != 0; n_now = next_batch()) {
       bool ok = true;
       if (warp == 9) {
@@ -239,7 +242,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       } else if (warp == 8) {
         // ---------------- products: a converged warp, one elected thread issues ----------------
         const uint32_t qk_desc = (1u << 4) | (1u << 7) | (1u << 10) | (negate ? 1u << 13 : 0u) |
-                                 (static_cast<uint32_t>(kWideTile >> 3) << 17) | (128u >> 4 << 24);
+                                 (static_cast<uint32_t>(kWideStep >> 3) << 17) | (128u >> 4 << 24);
         const uint32_t pv_desc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
                                  (static_cast<uint32_t>(HD >> 3) << 17) | (128u >> 4 << 24);
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
@@ -247,40 +250,34 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         const uint64_t q_desc = tc_desc(base + L::kQ, 16), k_desc = tc_desc(base + L::kK, 16);
         const uint64_t v_desc = tc_desc(base + L::kV, L::kPiece);
         auto wait = [&](uint64_t *bar, uint32_t parity, int who) { bar_wait(w, bar, parity, who); };
-        auto qk = [&](int tile, int st, bool last) {
-          const uint64_t qd = q_desc + (tile * L::kTileB >> 4), kd = k_desc + (st * L::kTileB >> 4);
+        // S = Q K^T for 64 rows of a K stage; `last`: the stage's last product
+        auto qk = [&](int tile, int buf, int st, int half, bool last) {
+          const uint64_t qd = q_desc + (tile * L::kTileB >> 4);
+          const uint64_t kd = k_desc + ((st * L::kTileB + half * kWideStep * 128) >> 4);
           if (elect_one()) {
 #pragma unroll
             for (int ks = 0; ks < HD / 16; ++ks) {
               const uint32_t off = ((ks >> 2) * L::kPiece + (ks & 3) * 32) >> 4;
-              tc_mma_ss(tm + tile * 128, qd + off, kd + off, qk_desc, ks > 0 ? 1u : 0u);
+              tc_mma_ss(tm + tile * 128 + buf * 64, qd + off, kd + off, qk_desc, ks > 0 ? 1u : 0u);
             }
-            tc_commit(&w.s_full[tile]);
+            tc_commit(&w.s_full[tile][buf]);
             if (last) tc_commit(&w.k_empty[st]);
           }
           __syncwarp();
         };
-        // O += P V once the halves of P are there; the V tile has been waited for. `last`: the
-        // stage's last product.
-        auto pv = [&](int tile, uint32_t count, int st, bool first, bool last) {
-          const uint64_t vd = v_desc + (st * L::kTileB >> 4);
-          const uint32_t par = count & 1;
-          const uint32_t d = tm + 256 + tile * 128, p = tm + tile * 128;
-          wait(&w.p_half[tile], par, 4);
+        // O += P V for 64 rows of a V stage, once P is there
+        auto pv = [&](int tile, int buf, uint32_t pair, int st, int half, bool first, bool last) {
+          if (!ok) return;
+          const uint64_t vd = v_desc + ((st * L::kTileB + half * kWideStep * 128) >> 4);
+          wait(&w.p_full[tile][buf], pair & 1, 5);
           tc_fence_after();  // P was stored by other threads
           if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-              tc_mma_ts(d, p + ks * 8, vd + (ks * 16 * 128 >> 4), pv_desc, (!first || ks > 0) ? 1u : 0u);
+            for (int ks = 0; ks < kWideStep / 16; ++ks) {
+              tc_mma_ts(tm + 256 + tile * 128, tm + tile * 128 + buf * 64 + ks * 8, vd + (ks * 16 * 128 >> 4), pv_desc,
+                        (!first || ks > 0) ? 1u : 0u);
             }
-          }
-          __syncwarp();
-          wait(&w.p_full[tile], par, 5);
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int ks = 4; ks < 8; ++ks) tc_mma_ts(d, p + ks * 8, vd + (ks * 16 * 128 >> 4), pv_desc, 1u);
-            tc_commit(&w.pv_done[tile]);
+            tc_commit(&w.pv_done[tile][buf]);
             if (last) tc_commit(&w.v_empty[st]);
           }
           __syncwarp();
@@ -295,8 +292,11 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           wait(&w.q_full[0], n_q[0]++ & 1, 6);
           if (two) wait(&w.q_full[1], n_q[1]++ & 1, 6);
           wait(&w.k_full[n_kv & 1], (n_kv >> 1) & 1, 7);
-          qk(0, n_kv & 1, !two);
-          if (two) qk(1, n_kv & 1, true);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            qk(0, half, n_kv & 1, half, !two && half == 1);
+            if (two) qk(1, half, n_kv & 1, half, half == 1);
+          }
 #pragma unroll 1
           for (int i = 0; i < tiles; ++i, ++n_kv) {
             const int st = n_kv & 1;
@@ -307,19 +307,23 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
               fixed ^= 1u << st;
             }
             if (more) wait(&w.k_full[st ^ 1], ((n_kv + 1) >> 1) & 1, 7);
-            pv(0, n_p[0]++, st, i == 0, !two);
-            if (more) qk(0, st ^ 1, !two);
-            if (two) {
-              pv(1, n_p[1]++, st, i == 0, true);
-              if (more) qk(1, st ^ 1, true);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              pv(0, half, n_s, st, half, i == 0 && half == 0, !two && half == 1);
+              if (more) qk(0, half, st ^ 1, half, !two && half == 1);
+              if (two) {
+                pv(1, half, n_s1, st, half, i == 0 && half == 0, half == 1);
+                if (more) qk(1, half, st ^ 1, half, half == 1);
+              }
             }
+            ++n_s;
+            if (two) ++n_s1;
           }
           ok = __all_sync(0xffffffffu, *reinterpret_cast<volatile int *>(&w.fail) == 0);
         }
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     for (int n_now = n_segs; n_now != 0; n_now = next_batch()) {
       bool ok = true;
       // ---------------- softmax: a thread per query row ----------------
@@ -370,32 +374,32 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         float m_run = -INFINITY, l_run = 0.f;
         const float c2 = a.c2;
 
-        for (int t = g.t0; t < g.t1; ++t) {
-          // what the row sees of a tile that not all rows see whole, while the product runs
-          const bool masked = (t + 1) * kWideTile > seen_by_all;
-          uint32_t see[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+#pragma unroll 1
+        for (int j = 0; j < 2 * (g.t1 - g.t0); ++j) {
+          const int key0 = g.t0 * kWideTile + j * kWideStep;
+          const uint32_t s_buf = s_addr + (n_s & 1) * 64;
+          // what the row sees of a step that not all rows see whole, while the product runs
+          const bool masked = key0 + kWideStep > seen_by_all;
+          uint32_t see[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
           if (masked) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) see[k] = seen32(a, g, token, t * kWideTile + k * 32);
+            see[0] = seen32(a, g, token, key0);
+            see[1] = seen32(a, g, token, key0 + 32);
           }
-          bar_wait(w, &w.s_full[tile], n_s & 1, 10);
+          bar_wait(w, &w.s_full[tile][n_s & 1], (n_s >> 1) & 1, 10);
           __syncwarp();
           tc_fence_after();
-          uint32_t s[128];
-          tmem_ld32(s_addr, s);
-          tmem_ld32(s_addr + 32, s + 32);
-          tmem_ld32(s_addr + 64, s + 64);
-          tmem_ld32(s_addr + 96, s + 96);
+          uint32_t s[64];
+          tmem_ld32(s_buf, s);
+          tmem_ld32(s_buf + 32, s + 32);
           tmem_wait_ld();
-          const uint32_t bad =
-              *reinterpret_cast<volatile uint32_t *>(&w.bad[(n_kv + tiles_before + (t - g.t0)) & 3]);
+          const uint32_t bad = *reinterpret_cast<volatile uint32_t *>(&w.bad[(n_kv + tiles_before + (j >> 1)) & 3]);
           if (masked || bad != 0u) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 2; ++k) {
               uint32_t m = see[k];
               if (bad != 0u) {
                 for (int i = 0; i < 32; ++i) {
-                  if ((bad >> ((k * 32 + i) / box)) & 1u) m &= ~(1u << i);
+                  if ((bad >> (((j & 1) * kWideStep + k * 32 + i) / box)) & 1u) m &= ~(1u << i);
                 }
               }
 #pragma unroll
@@ -409,22 +413,23 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           for (int c = 0; c < 4; ++c) {
             mx4[c] = fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 4]));
 #pragma unroll
-            for (int e = 8; e < 128; e += 8) {
+            for (int e = 8; e < 64; e += 8) {
               mx4[c] = max3(mx4[c], __uint_as_float(s[e + c]), __uint_as_float(s[e + c + 4]));
             }
           }
           const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * c2;
           // raise the subtracted maximum only when it is far behind
-          const bool raise = mx > m_run + 8.f || m_run == -INFINITY;
+          const bool raise = mx > m_run + kSlack || m_run == -INFINITY;
           const float m_new = raise ? fmaxf(mx, m_run) : m_run;
-          const float alpha = raise ? (m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new)) : 1.f;
           const bool turn_down = raise && m_run != -INFINITY;
           if (__any_sync(0xffffffffu, turn_down)) {
-            // the accumulator is this thread's once the last product into it is done
-            bar_wait(w, &w.pv_done[tile], (n_s & 1) ^ 1, 11);
+            // The accumulator is this thread's once the last product into it is done. (That of
+            // the step before, whose barrier this is too, ended before these scores began.)
+            bar_wait(w, &w.pv_done[tile][(n_s - 1) & 1], ((n_s - 1) >> 1) & 1, 11);
             __syncwarp();
             tc_fence_after();
-            const float by = turn_down ? alpha : 1.f;
+            const float by = turn_down ? fast_exp2(m_run - m_new) : 1.f;
+            l_run *= by;
 #pragma unroll 1
             for (int c = 0; c < HD; c += 16) {
               uint32_t o[16];
@@ -437,30 +442,26 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             tmem_wait_st();
           }
           m_run = m_new;
-          const float m_use = m_new == -INFINITY ? 0.f : m_new;
+          const float m_use = m_new == -INFINITY ? 0.f : m_new;  // nothing seen so far: all -inf
           const f32x2_t c22 = pack_f32x2(c2, c2), mm2 = pack_f32x2(-m_use, -m_use);
-          f32x2_t sum2 = pack_f32x2(0.f, 0.f);
+          f32x2_t sum2 = pack_f32x2(l_run, 0.f);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            // a half of the row's exps, in place as bf16 pairs, and over to the product
-#pragma unroll
-            for (int e = h * 64; e < h * 64 + 64; e += 2) {
-              float p0, p1;
-              unpack_f32x2(ffma2(pack_f32x2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c22, mm2), p0, p1);
-              p0 = fast_exp2(p0);
-              p1 = fast_exp2(p1);
-              sum2 = add2(sum2, pack_f32x2(p0, p1));
-              const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);
-              s[e >> 1] = *reinterpret_cast<const uint32_t *>(&v);
-            }
-            tmem_st32(s_addr + h * 32, s + h * 32);
-            tmem_wait_st();
-            tc_fence_before();
-            bar_arrive(h == 0 ? &w.p_half[tile] : &w.p_full[tile]);
+          for (int e = 0; e < 64; e += 2) {
+            float p0, p1;
+            unpack_f32x2(ffma2(pack_f32x2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c22, mm2), p0, p1);
+            p0 = fast_exp2(p0);
+            p1 = fast_exp2(p1);
+            sum2 = add2(sum2, pack_f32x2(p0, p1));
+            const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);
+            s[e >> 1] = *reinterpret_cast<const uint32_t *>(&v);
           }
+          tmem_st32(s_buf, s);
+          tmem_wait_st();
+          tc_fence_before();
+          bar_arrive(&w.p_full[tile][n_s & 1]);
           float sum0, sum1;
           unpack_f32x2(sum2, sum0, sum1);
-          l_run = fmaf(l_run, alpha, sum0 + sum1);
+          l_run = sum0 + sum1;
           ++n_s;
         }
         if (!ok) break;
@@ -468,7 +469,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         q_ahead = si + 1 < n_now && segs[si + 1].rows > first_row;
         if (q_ahead) load_q(segs[si + 1]);
         // ---- the segment's result ----
-        ok = __all_sync(0xffffffffu, bar_wait(w, &w.pv_done[tile], (n_s & 1) ^ 1, 12));
+        ok = __all_sync(0xffffffffu, bar_wait(w, &w.pv_done[tile][(n_s - 1) & 1], ((n_s - 1) >> 1) & 1, 12));
         if (!ok) break;
         tc_fence_after();
         const bool whole = g.whole;
