@@ -49,14 +49,18 @@ inline int paged_cache(const chr_nf4_pages_t *p, PagedCache &c) {
 // one kv head its queries are R = n * n_rep rows (token-major), cut into items of M
 // rows. Item j reads cache rows 0 .. kv_end(j), in tiles of `tile` rows. All items, in
 // the order (sequence, kv head, item), lie on one axis with a length that is what they
-// cost, and CTA c of G takes the piece [total c / G, total (c+1) / G) of it: every CTA
-// has the same amount of cache to read whatever the lengths, and the host needs to know
+// cost, and CTA c of G takes the piece between total c / G and total (c+1) / G of it: every
+// CTA has the same amount of cache to read whatever the lengths, and the host needs to know
 // none of them. A piece border inside an item falls on the tile border next to it; an
 // item that a border cuts is left as FP32 partials (at most two per CTA: of its first
 // and of its last item) that a second kernel joins.
 // The length of an item is its cache rows plus `extra` (what starting and ending it costs,
 // in rows), times n_rep; the causal part is counted exactly up to rounding - base n_rep
 // plus the rows up to its last - so that the axis has a closed form.
+// Places on the axis are whole numbers in binary64 (the host sees to it that they stay
+// below 2^53, where sums and products of them are exact): every CTA derives the same ones.
+// The walk runs once per CTA, from a cold instruction cache, where a kilobyte of code takes as
+// long as a cache tile; hence short loops and no wide integer division.
 struct PagedRows {
   const int32_t *q_start;  // [batch + 1], or null: row b is sequence b's only one
   const int32_t *kv_len;   // [batch]
@@ -70,41 +74,37 @@ struct PagedSeq {
   int r0, n, len;     // first row, rows, cache rows
   int base;           // len - n: cache rows older than the new ones (may be negative)
   int R, J;           // query rows under a kv head, items
-  bool stairs;        // causal with a cost that grows from item to item
+  int stairs;         // causal with a cost that grows from item to item
+  double flat;        // the part of an item's cost that does not
 };
 
 __device__ __forceinline__ PagedSeq paged_seq(const PagedRows &p, int b) {
   PagedSeq s;
+  s.r0 = b;
+  int end = b < p.T ? b + 1 : b;
   if (p.q_start != nullptr) {
-    const int lo = min(max(__ldg(p.q_start + b), 0), p.T);
-    const int hi = min(max(__ldg(p.q_start + b + 1), lo), p.T);
-    s.r0 = lo;
-    s.n = hi - lo;
-  } else {
-    s.r0 = b;
-    s.n = b < p.T ? 1 : 0;
+    s.r0 = min(max(__ldg(p.q_start + b), 0), p.T);
+    end = min(max(__ldg(p.q_start + b + 1), s.r0), p.T);
   }
+  s.n = end - s.r0;
   s.len = min(max(__ldg(p.kv_len + b), 0), p.cap);
   s.base = s.len - s.n;
   s.R = s.n * p.n_rep;
   s.J = (s.R + p.M - 1) / p.M;
   s.stairs = p.causal != 0 && s.base >= 0;
+  s.flat = (static_cast<double>(s.stairs ? s.base : s.len) + p.extra) * p.n_rep;
   return s;
 }
 
 // Length of items 0 .. j-1, and of item j.
-__device__ __forceinline__ long long paged_before(const PagedRows &p, const PagedSeq &s, int j) {
-  const long long jj = j;
-  if (!s.stairs) return jj * (static_cast<long long>(s.len) + p.extra) * p.n_rep;
-  long long v = jj * (static_cast<long long>(s.base) + p.extra) * p.n_rep + jj * (jj + 1) / 2 * p.M;
-  if (j >= s.J) v -= jj * p.M - s.R;  // the last item is not full
+__device__ __forceinline__ double paged_before(const PagedRows &p, const PagedSeq &s, int j) {
+  const double jj = j;
+  double v = jj * s.flat;
+  if (s.stairs) v += j < s.J ? 0.5 * jj * (jj + 1.0) * p.M : 0.5 * jj * (jj - 1.0) * p.M + s.R;
   return v;
 }
-__device__ __forceinline__ long long paged_cost(const PagedRows &p, const PagedSeq &s, int j) {
-  return paged_before(p, s, j + 1) - paged_before(p, s, j);
-}
-__device__ __forceinline__ long long paged_seq_cost(const PagedRows &p, const PagedSeq &s) {
-  return s.J == 0 ? 0 : paged_before(p, s, s.J) * p.n_kv;
+__device__ __forceinline__ double paged_cost(const PagedRows &p, const PagedSeq &s, int j) {
+  return s.flat + (s.stairs ? min((j + 1) * p.M, s.R) : 0);
 }
 
 // Cache rows item j can see: to its last token's own row when causal, else all.
@@ -117,41 +117,29 @@ __device__ __forceinline__ int paged_kv_end(const PagedRows &p, const PagedSeq &
 // Tile border that stands for place `off` of an item of cost `cost` and nt tiles: any
 // function of the three that does not fall as `off` grows will do, and each step of this
 // one is rounded monotonically.
-__device__ __forceinline__ int paged_border(long long off, long long cost, int nt) {
-  if (off <= 0) return 0;
+__device__ __forceinline__ int paged_border(double off, double cost, int nt) {
+  if (off <= 0.0) return 0;
   if (off >= cost) return nt;
-  const float f = __fdiv_rn(__ll2float_rn(off), __ll2float_rn(cost));
+  const float f = __fdiv_rn(__double2float_rn(off), __double2float_rn(cost));
   return min(__float2int_rn(__fmul_rn(f, __int2float_rn(nt))), nt);
 }
 
-// floor(a / b) for 0 <= a < 2^62, b > 0, quotient below 2^52. The axis of most batches fits 32
-// bits; else a guess in binary64 is put right.
-__device__ __forceinline__ long long floor_div(long long a, long long b) {
-  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-  long long q = static_cast<long long>(__ddiv_rn(static_cast<double>(a), static_cast<double>(b)));
+// floor(a / b) for whole a >= 0, b > 0 and a small quotient: a guess, put right.
+__device__ __forceinline__ int floor_div(double a, double b) {
+  int q = __float2int_rz(__fdividef(__double2float_rn(a), __double2float_rn(b)));
   while (q * b > a) --q;
   while ((q + 1) * b <= a) ++q;
   return q;
 }
 
-// The axis: its length, the pieces it is cut into (no more than the grid has CTAs, and none
-// shorter than a tile), and where piece c starts.
+// The axis: its length and the pieces it is cut into (no more than the grid has CTAs, and none
+// shorter than a tile). Piece c starts at floor(total (c / G)).
 struct PagedAxis {
-  long long total, whole;  // whole = total / G
-  int G, rest;             // rest = total % G
+  double total, per;  // per = 1 / G
+  int G;
 };
-__device__ __forceinline__ PagedAxis paged_axis(const PagedRows &p, long long total, int ctas) {
-  PagedAxis x;
-  x.total = total;
-  const long long unit = static_cast<long long>(p.tile) * p.n_rep;
-  x.G = ctas;
-  if (total < unit * ctas) x.G = max(static_cast<int>(floor_div(total, unit)), 1);
-  x.whole = floor_div(total, x.G);
-  x.rest = static_cast<int>(total - x.whole * x.G);
-  return x;
-}
-__device__ __forceinline__ long long paged_piece(const PagedAxis &x, int c) {
-  return x.whole * c + static_cast<unsigned>(x.rest) * static_cast<unsigned>(c) / static_cast<unsigned>(x.G);
+__device__ __forceinline__ double paged_piece(const PagedAxis &x, int c) {
+  return c >= x.G ? x.total : floor(x.total * (c * x.per));
 }
 
 // One piece of a CTA's share: tiles t0 .. t1-1 of an item.
@@ -163,16 +151,17 @@ struct Seg {
 };
 constexpr int kSegs = 32;   // segments described at a time
 
-// An item that borders cut, described by the CTA that holds its start: pieces first ..
-// first + n - 1 hold a partial each (the first in slot 1, the others in slot 0).
+// A CTA's note for the join: whether its two partials hold anything, and, if a cut item
+// starts in its piece, that item: pieces first .. first + n - 1 hold a partial each (the
+// first in slot 1, the others in slot 0).
 struct PagedCut {
-  int n, first;
-  int kvh, row0, rows, r0;
+  int live[2];
+  int n, kvh, row0, rows, r0, pad;
 };
 
 // The walk along a CTA's piece. One warp starts it, its first thread goes on.
 struct SegWalk {
-  long long x_hi, x_lo, start;  // the piece, and the item the walk is at
+  double x_hi, x_lo, start;  // the piece, and the item the walk is at
   PagedSeq s;
   int b, kvh, j;
   PagedAxis axis;
@@ -188,65 +177,74 @@ __device__ __forceinline__ int head_of(const PagedRows &p, const Seg &g, int r, 
   return g.kvh * p.n_rep + g.rem0 + r - (token - g.tok0) * p.n_rep;
 }
 
-// Called by a whole warp; false: nothing to do for CTA c. The walk's functions run once or
-// a few times per CTA: as calls, they leave the instruction cache to the loops.
+// Called by a whole warp; false: nothing to do for CTA c. A lane takes a run of sequences:
+// one pass adds them up, a second, by the lane that holds the piece's start, finds it.
 static __device__ __noinline__ bool walk_start(const PagedRows &p, SegWalk &w, int c, int ctas) {
   const int lane = threadIdx.x & 31;
   const int per = (p.batch + 31) / 32;
   const int b0 = min(lane * per, p.batch), b1 = min(b0 + per, p.batch);
-  long long mine = 0;
-#pragma unroll 4
-  for (int i = b0; i < b1; ++i) mine += paged_seq_cost(p, paged_seq(p, i));
-  long long incl = mine;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, incl, off);
-    if (lane >= off) incl += o;
-  }
-  const long long total = __shfl_sync(0xffffffffu, incl, 31);
-  if (total <= 0) return false;
-  const PagedAxis axis = paged_axis(p, total, ctas);
-  if (c >= axis.G) return false;
-  const long long x = paged_piece(axis, c);
-  const int from = __ffs(__ballot_sync(0xffffffffu, x < incl)) - 1;
-  if (lane == from) {
-    long long at = incl - mine;
+  PagedAxis axis;
+  double at = 0.0, x = 0.0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    double cost = 0.0;
+    PagedSeq s;
     int b = b0;
-    PagedSeq s = paged_seq(p, b);
-    for (;;) {
-      const long long cost = paged_seq_cost(p, s);
-      if (x < at + cost) break;
+#pragma unroll 1
+    for (; b < b1; ++b) {
+      s = paged_seq(p, b);
+      cost = paged_before(p, s, s.J) * p.n_kv;
+      if (pass == 1 && x < at + cost) break;
       at += cost;
-      s = paged_seq(p, ++b);
     }
-    const long long one = paged_before(p, s, s.J);
-    w.b = b;
-    w.kvh = static_cast<int>(floor_div(x - at, one));
-    at += w.kvh * one;
-    int lo = 0, hi = s.J - 1;  // the last item that starts at x or before
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (paged_before(p, s, mid) <= x - at) {
-        lo = mid;
-      } else {
-        hi = mid - 1;
+    if (pass == 1) {
+      const double one = paged_before(p, s, s.J);
+      const int kvh = floor_div(x - at, one);
+      at += kvh * one;
+      int lo = 0, hi = s.J - 1;  // the last item that starts at x or before
+#pragma unroll 1
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (at + paged_before(p, s, mid) <= x) {
+          lo = mid;
+        } else {
+          hi = mid - 1;
+        }
       }
+      w.b = b;
+      w.kvh = kvh;
+      w.j = lo;
+      w.start = at + paged_before(p, s, lo);
+      w.s = s;
+      w.x_lo = x;
+      w.x_hi = paged_piece(axis, c + 1);
+      w.axis = axis;
+      break;
     }
-    w.j = lo;
-    w.start = at + paged_before(p, s, lo);
-    w.s = s;
-    w.x_lo = x;
-    w.x_hi = paged_piece(axis, c + 1);
-    w.axis = axis;
+    double incl = at;
+#pragma unroll 1
+    for (int off = 1; off < 32; off <<= 1) {
+      const double o = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += o;
+    }
+    axis.total = __shfl_sync(0xffffffffu, incl, 31);
+    if (axis.total <= 0.0) return false;
+    const double unit = static_cast<double>(p.tile) * p.n_rep;
+    axis.G = axis.total < unit * ctas ? max(floor_div(axis.total, unit), 1) : ctas;
+    axis.per = 1.0 / axis.G;
+    if (c >= axis.G) return false;
+    x = paged_piece(axis, c);
+    const int from = __ffs(__ballot_sync(0xffffffffu, x < incl)) - 1;
+    if (lane != from) break;
+    at = incl - at;
   }
   __syncwarp();
   return true;
 }
 
 // The item at the walk's place as a segment of CTA c's piece, then on to the next one.
-// `cut` is filled when the piece holds the start but not the end of the item.
 __device__ __forceinline__ void walk_next(const PagedRows &p, SegWalk &w, int c, Seg &g, PagedCut &cut) {
-  const long long cost = paged_cost(p, w.s, w.j), end = w.start + cost;
+  const double cost = paged_cost(p, w.s, w.j), end = w.start + cost;
   g.b = w.b;
   g.kvh = w.kvh;
   g.row0 = w.j * p.M;
@@ -262,14 +260,16 @@ __device__ __forceinline__ void walk_next(const PagedRows &p, SegWalk &w, int c,
   g.t1 = paged_border(w.x_hi - w.start, cost, nt);
   g.whole = w.start >= w.x_lo && end <= w.x_hi;
   g.slot = w.start < w.x_lo ? 0 : 1;
+  if (g.whole == 0) cut.live[g.slot] = g.t0 < g.t1;
   if (g.slot == 1 && end > w.x_hi) {
     // the last piece that starts before the item's end
-    int last = static_cast<int>(floor_div(end, w.axis.whole + (w.axis.rest > 0 ? 1 : 0)));
-    last = min(max(last, c + 1), w.axis.G - 1);
-    while (last + 1 < w.axis.G && paged_piece(w.axis, last + 1) < end) ++last;
+    int last = c + 1 + __float2int_rz(__fdividef(__double2float_rn(end - w.x_hi) * w.axis.G, __double2float_rn(w.axis.total)));
+    last = min(last, w.axis.G - 1);
+#pragma unroll 1
     while (last > c + 1 && paged_piece(w.axis, last) >= end) --last;
+#pragma unroll 1
+    while (last + 1 < w.axis.G && paged_piece(w.axis, last + 1) < end) ++last;
     cut.n = last - c + 1;
-    cut.first = c;
     cut.kvh = g.kvh;
     cut.row0 = g.row0;
     cut.rows = g.rows;
@@ -280,6 +280,7 @@ __device__ __forceinline__ void walk_next(const PagedRows &p, SegWalk &w, int c,
     w.j = 0;
     if (++w.kvh == p.n_kv) {
       w.kvh = 0;
+#pragma unroll 1
       while (++w.b < p.batch) {
         w.s = paged_seq(p, w.b);
         if (w.s.J > 0) break;

@@ -48,46 +48,64 @@ __device__ __forceinline__ void ldm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
                : "r"(addr));
 }
 
-// The workspace: [G] descriptions of cut items, then the partials, [G][2][M] each: the
-// running maximum (log2 units) and sum of a row, and its HD unnormalised outputs.
+// The workspace: [G] notes of the CTAs, then the partials, [G][2][M] each: the running
+// maximum (log2 units) and sum of a row, and its HD unnormalised outputs.
 struct PagedWs {
   PagedCut *cut;
   float2 *ml;
   float *o;
 };
 __host__ __device__ __forceinline__ long long ws_floats_of(int ctas, int M, int hd) {
-  return (static_cast<long long>(ctas) * static_cast<int>(sizeof(PagedCut)) + 15) / 16 * 4 +
+  return static_cast<long long>(ctas) * static_cast<int>(sizeof(PagedCut) / 4) +
          static_cast<long long>(ctas) * 2 * M * (hd + 2);
 }
 __device__ __forceinline__ PagedWs ws_of(const PagedAttnArgs &a, int ctas) {
+  static_assert(sizeof(PagedCut) == 32, "two 16-byte loads");
   PagedWs w;
   w.cut = reinterpret_cast<PagedCut *>(a.ws);
-  w.o = a.ws + (static_cast<long long>(ctas) * static_cast<int>(sizeof(PagedCut)) + 15) / 16 * 4;
+  w.o = a.ws + static_cast<long long>(ctas) * static_cast<int>(sizeof(PagedCut) / 4);
   w.ml = reinterpret_cast<float2 *>(w.o + static_cast<long long>(ctas) * 2 * a.p.M * a.c.hd);
   return w;
 }
 
 // Describes up to kSegs segments of CTA c's piece from the walk's place on: their number.
-// One thread. An empty piece of a cut item is noted as such, and so is a cut item that
-// starts in the piece (at most its last).
-__device__ __noinline__ int walk_fill(const PagedAttnArgs &a, SegWalk &w, int c, int ctas, Seg *segs) {
+// One thread; `cut` is the CTA's note, complete once there are no more.
+__device__ __noinline__ int walk_fill(const PagedAttnArgs &a, SegWalk &at, PagedCut &note, int c, int ctas, Seg *segs) {
+  SegWalk w = at;  // in registers
+  PagedCut cut = note;
   int n = 0;
-  PagedCut cut;
-  cut.n = 0;
-  const PagedWs ws = ws_of(a, ctas);
+#pragma unroll 1
   while (n < kSegs && w.start < w.x_hi && w.b < a.p.batch) {
     Seg g;
     walk_next(a.p, w, c, g, cut);
-    if (g.t0 < g.t1) {
-      segs[n++] = g;
-    } else if (!g.whole) {
-      for (int r = 0; r < g.rows; ++r) {
-        ws.ml[(static_cast<long long>(c) * 2 + g.slot) * a.p.M + r] = make_float2(-INFINITY, 0.f);
-      }
-    }
+    if (g.t0 < g.t1) segs[n++] = g;
   }
-  if (cut.n != 0) ws.cut[c] = cut;
+  at = w;
+  note = cut;
+  ws_of(a, ctas).cut[c] = cut;
   return n;
+}
+
+// The walk of a CTA, in shared memory: thread 0's, and not worth the registers of a thread.
+struct PagedWalk {
+  SegWalk at;
+  PagedCut note;
+  int n_segs;
+};
+// The first segments; all threads of the block call it.
+__device__ __forceinline__ int walk_begin(const PagedAttnArgs &a, PagedWalk &w, Seg *segs) {
+  if (threadIdx.x < 32) {
+    const int ctas = gridDim.x, c = blockIdx.x;
+    if (threadIdx.x == 0) {
+      w.at.start = w.at.x_hi = 0.0;
+      w.note.live[0] = w.note.live[1] = w.note.n = 0;
+    }
+    __syncwarp();
+    walk_start(a.p, w.at, c, ctas);
+    if (threadIdx.x == 0) w.n_segs = walk_fill(a, w.at, w.note, c, ctas, segs);
+  }
+  __syncthreads();
+  return w.n_segs;
 }
 
 // Which of the 32 cache rows that begin `older` rows before the new ones a drafted row sees.
@@ -204,8 +222,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   Seg *segs = reinterpret_cast<Seg *>(at);
   at += L::kSegB;
   uint64_t *bars = reinterpret_cast<uint64_t *>(at);  // [warp][stage]
-  __shared__ int n_segs;
-  __shared__ SegWalk walk;  // thread 0's: not worth the registers of a thread
+  __shared__ PagedWalk walk;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g8 = lane >> 2, t4 = lane & 3;
@@ -218,13 +235,8 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   }
   pdl_wait();
   pdl_trigger();
-  if (warp == 0) {
-    if (lane == 0) ws_of(a, G).cut[cta].n = 0;
-    const bool some = walk_start(a.p, walk, cta, G);
-    if (lane == 0) n_segs = some ? walk_fill(a, walk, cta, G, segs) : 0;
-  }
   zero_tail_rows<HD>(a, cta, G);
-  __syncthreads();
+  int n_now = walk_begin(a, walk, segs);
 
   const uint32_t ring = smem_u32(smem) + warp * S * L::kHalf;
   uint64_t *bar = bars + warp * S;
@@ -235,7 +247,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   int ahead = 0;        // ring slot requested next
   uint32_t phase = 0;   // parity of each slot's next completed copy
 
-  for (int n_now = n_segs; n_now != 0;) {
+  while (n_now != 0) {
     // A segment's queries (where they fit registers next to the running ones) and the pages of
     // its first 32 tiles (lane i: this warp's block of tile t0 + i) are fetched one segment early.
     uint32_t qn[KEEP ? KS : 1][2];
@@ -561,9 +573,10 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
     }
     __syncthreads();
-    if (tid == 0) n_segs = walk_fill(a, walk, cta, G, segs);
+    if (n_now < kSegs) break;  // there are no more
+    if (tid == 0) walk.n_segs = walk_fill(a, walk.at, walk.note, cta, G, segs);
     __syncthreads();
-    n_now = n_segs;
+    n_now = walk.n_segs;
     __syncthreads();
   }
   if (!ok) {
@@ -614,23 +627,27 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Pag
   PagedCut cut;
   cut.n = 0;
   if (c < G) {
-    static_assert(sizeof(PagedCut) == 24, "three 8-byte loads");
-    const int2 *src = reinterpret_cast<const int2 *>(ws.cut + c);
-    const int2 d0 = __ldcg(src), d1 = __ldcg(src + 1), d2 = __ldcg(src + 2);
-    cut.n = d0.x;
-    cut.first = d0.y;
-    cut.kvh = d1.x;
-    cut.row0 = d1.y;
-    cut.rows = d2.x;
-    cut.r0 = d2.y;
+    const int4 *src = reinterpret_cast<const int4 *>(ws.cut + c);
+    const int4 d0 = __ldcg(src), d1 = __ldcg(src + 1);
+    cut.n = d0.z;
+    cut.kvh = d0.w;
+    cut.row0 = d1.x;
+    cut.rows = d1.y;
+    cut.r0 = d1.z;
+    cut.pad = c;  // its first piece
   }
   if (lane == 0) cuts[warp] = cut;
   // row r's partial in piece i: slot 1 of the first CTA, slot 0 of the others
   auto part = [&](const PagedCut &t, int i, int r) {
-    return ((t.first + i) * 2ll + (i == 0 ? 1 : 0)) * a.p.M + r;
+    return ((t.pad + i) * 2ll + (i == 0 ? 1 : 0)) * a.p.M + r;
+  };
+  // ... and its maximum and sum; a piece that was rounded away wrote none
+  auto ml_of = [&](const PagedCut &t, int i, int r) {
+    const int live = i < t.n ? __ldcg(&ws.cut[t.pad + i].live[i == 0 ? 1 : 0]) : 0;
+    return live != 0 ? __ldcg(ws.ml + part(t, i, r)) : make_float2(-INFINITY, 0.f);
   };
   auto add = [&](float4 &acc, float w, long long at) {
-    if (w != 0.f && lane * 4 < hd) {  // an empty piece wrote no outputs
+    if (w != 0.f && lane * 4 < hd) {
       const float4 v = __ldcg(reinterpret_cast<const float4 *>(ws.o + at * hd) + lane);
       acc.x = fmaf(w, v.x, acc.x);
       acc.y = fmaf(w, v.y, acc.y);
@@ -640,7 +657,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Pag
   };
   if (cut.n > 0 && cut.n <= kJoinFew) {
     for (int r = blockIdx.y; r < cut.rows; r += gridDim.y) {
-      const float2 ml = lane < cut.n ? __ldcg(ws.ml + part(cut, lane, r)) : make_float2(-INFINITY, 0.f);
+      const float2 ml = ml_of(cut, lane, r);
       const float mm = warp_max_xor(ml.x);
       const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mm);
       const float l = warp_sum_xor(w * ml.y);
@@ -657,7 +674,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Pag
     for (int r = blockIdx.y; r < t.rows; r += gridDim.y) {
       // pieces warp * 32 + lane, + 256, ... for the maximum and the sum
       float mm = -INFINITY;
-      for (int i = tid; i < t.n; i += kJoinThreads) mm = fmaxf(mm, __ldcg(ws.ml + part(t, i, r)).x);
+      for (int i = tid; i < t.n; i += kJoinThreads) mm = fmaxf(mm, ml_of(t, i, r).x);
       mm = warp_max_xor(mm);
       if (lane == 0) red[0][warp] = mm;
       __syncthreads();
@@ -667,7 +684,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Pag
       float l = 0.f;
       for (int i0 = warp * 8; i0 < t.n; i0 += kJoinThreads / 4) {
         // eight pieces of this warp at a time: their weights in lanes, then their outputs
-        const float2 ml = lane < 8 && i0 + lane < t.n ? __ldcg(ws.ml + part(t, i0 + lane, r)) : make_float2(-INFINITY, 0.f);
+        const float2 ml = lane < 8 ? ml_of(t, i0 + lane, r) : make_float2(-INFINITY, 0.f);
         const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mm);
         l = fmaf(w, ml.y, l);
 #pragma unroll
@@ -849,7 +866,7 @@ extern "C" int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, i
   a.p.extra = f.extra;
   a.p.per_rep = 1.f / static_cast<float>(n_rep);
   a.p.causal = tree == nullptr;
-  // the axis is measured in 64-bit integers that binary64 holds exactly
+  // places on the axis are whole numbers that binary64 holds exactly
   const double items = static_cast<double>(T) * n_q / f.M + static_cast<double>(a.c.batch) * a.c.n_kv;
   if (items * (static_cast<double>(a.p.cap) + f.extra) * n_rep > 4.0e15) return kDims;
   a.q = static_cast<const __nv_bfloat16 *>(q);

@@ -103,8 +103,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   const uint32_t base = smem_u32(sm);
   WideBars &w = *reinterpret_cast<WideBars *>(sm + L::kBars);
   Seg *segs = reinterpret_cast<Seg *>(sm + L::kSegOff);
-  __shared__ int n_segs;
-  __shared__ SegWalk walk;  // thread 0's: not worth the registers of a thread
+  __shared__ PagedWalk walk;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int G = gridDim.x, cta = blockIdx.x;
@@ -138,13 +137,8 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 
   pdl_wait();
   pdl_trigger();
-  if (warp == 0) {
-    if (lane == 0) ws_of(a, G).cut[cta].n = 0;
-    const bool some = walk_start(a.p, walk, cta, G);
-    if (lane == 0) n_segs = some ? walk_fill(a, walk, cta, G, segs) : 0;
-  }
   zero_tail_rows<HD>(a, cta, G);
-  __syncthreads();
+  const int n_first = walk_begin(a, walk, segs);
 
   const int shift = a.c.page_shift;
   const int box = min(1 << shift, kWideTile);  // rows of one copy
@@ -159,16 +153,17 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   uint32_t n_s1 = 0;          // product role: pairs of steps of query tile 1
 
   // The roles part here for good, each with its own loop over the batches of segments.
-  auto next_batch = [&]() {
+  auto next_batch = [&](int n) {
+    if (n < kSegs) return 0;  // there are no more
     block_sync();
-    if (tid == 0) n_segs = w.fail != 0 ? 0 : walk_fill(a, walk, cta, G, segs);
+    if (tid == 0) walk.n_segs = w.fail != 0 ? 0 : walk_fill(a, walk.at, walk.note, cta, G, segs);
     block_sync();
-    const int n = n_segs;
+    n = walk.n_segs;
     block_sync();
     return n;
   };
   if (warp >= 8) {
-    for (int n_now = n_segs; n_now != 0; n_now = next_batch()) {
+    for (int n_now = n_first; n_now != 0; n_now = next_batch(n_now)) {
       bool ok = true;
       if (warp == 9) {
         // ---------------- copies ----------------
@@ -324,7 +319,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
     }
   } else {
-    for (int n_now = n_segs; n_now != 0; n_now = next_batch()) {
+    for (int n_now = n_first; n_now != 0; n_now = next_batch(n_now)) {
       bool ok = true;
       // ---------------- softmax: a thread per query row ----------------
       const int tile = warp >> 2;
