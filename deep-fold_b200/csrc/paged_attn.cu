@@ -725,7 +725,7 @@ AttnForm form_of(int T, int batch, int n_rep, int n_kv, int hd, long long cap) {
   if (rows > 32 && (hd == 64 || hd == 128)) {
     f.M = kWideM;
     f.tile = kWideTile;
-    f.extra = kWideTile;
+    f.extra = 2 * kWideTile;  // queries in, result out (measured)
     f.ctas = static_cast<int>(sms);  // one resident CTA per SM
     return f;
   }
