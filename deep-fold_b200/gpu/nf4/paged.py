@@ -34,16 +34,16 @@ def _fail(msg: str):
     raise RuntimeError(msg)
 
 
-# The host's share of a small call is longer than the kernel's: the raw forms of "current device"
-# and "current stream" take a tenth of what the public ones do.
-_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+# A small call takes longer on the host than on the device, so the checks are kept lean: device
+# indices instead of device objects, each attribute read once, and the raw forms of "current
+# device" and "current stream", which take a tenth of what the public ones do.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _call(name: str, device: torch.device, *args) -> None:
-    """``name(*args, stream)`` with ``device`` current, on its current stream."""
-    index = device.index
+def _call(name: str, index: int, *args) -> None:
+    """``name(*args, stream)`` with device ``index`` current, on its current stream."""
     fn = getattr(_lib.load(), name)
     if index == _current_device():
         rc = fn(*args, _raw_stream(index))
@@ -54,69 +54,72 @@ def _call(name: str, device: torch.device, *args) -> None:
         _lib.check(rc, name)
 
 
-def _on(t: torch.Tensor, device: torch.device, dtype: torch.dtype, what: str) -> None:
-    if t.dtype is not dtype or t.device != device:
-        _fail(f"{what} must be {str(dtype)[6:]} on {device}")
-
-
-def _vector(t: torch.Tensor | None, n: int, device: torch.device, dtype: torch.dtype, what: str) -> int:
+def _vector(t: torch.Tensor | None, n: int, index: int, dtype: torch.dtype, what: str) -> int:
     """Address of a contiguous vector of ``n`` elements; 0 for ``None``."""
     if t is None:
         return 0
-    if t.dtype is not dtype or t.device != device or t.numel() != n or not t.is_contiguous():
-        _fail(f"{what} must be contiguous {str(dtype)[6:]} of {n} elements on {device}")
+    if t.dtype is not dtype or t.get_device() != index or t.numel() != n or not t.is_contiguous():
+        _fail(f"{what} must be contiguous {str(dtype)[6:]} of {n} elements on cuda:{index}")
     return t.data_ptr()
 
 
-def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor) -> tuple[ChrNf4Pages, torch.device]:
-    if not k_pages.is_cuda or k_pages.dtype is not _BF16 or k_pages.dim() != 4:
-        _fail("k_pages must be a CUDA bfloat16 [n_pages, page, n_kv, hd]")
-    device = k_pages.device
+def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor) -> tuple[ChrNf4Pages, int]:
+    """The C description of a paged cache, and its device's index."""
+    index = k_pages.get_device()
     shape = k_pages.shape
+    if index < 0 or k_pages.dtype is not _BF16 or len(shape) != 4:
+        _fail("k_pages must be a CUDA bfloat16 [n_pages, page, n_kv, hd]")
+    if v_pages.dtype is not _BF16 or v_pages.get_device() != index or v_pages.shape != shape:
+        _fail(f"v_pages must be bfloat16 {list(shape)} on cuda:{index}, as k_pages")
     n_pages, page, n_kv, hd = shape
-    _on(v_pages, device, _BF16, "v_pages")
-    if v_pages.shape != shape:
-        _fail("k_pages and v_pages differ in shape")
-    inner = (n_kv * hd, hd, 1)
-    ks, vs = k_pages.stride(), v_pages.stride()
-    if ks[1:] != inner or vs[1:] != inner:
+    one = page * n_kv * hd
+    ks, k_row, k_head, k_el = k_pages.stride()
+    vs, v_row, v_head, v_el = v_pages.stride()
+    row = n_kv * hd
+    if k_row != row or v_row != row or k_head != hd or v_head != hd or k_el != 1 or v_el != 1:
         _fail("the pages of a pool must each be contiguous")
     if page < 16 or page & (page - 1) or page > 65536:
         _fail(f"page must be a power of two in 16..65536, got {page}")
-    _on(table, device, _I32, "page_table")
-    if table.dim() != 2 or table.stride(1) != 1:
-        _fail("page_table must be int32 [batch, max_pages] with contiguous rows")
+    if table.dtype is not _I32 or table.get_device() != index or table.dim() != 2:
+        _fail(f"page_table must be int32 [batch, max_pages] on cuda:{index}")
     batch, max_pages = table.shape
-    if n_pages < 1 or batch < 1 or max_pages < 1:
+    t_row, t_el = table.stride()
+    if n_pages < 1 or batch < 1 or max_pages < 1 or one < 1:
         _fail("the pools and page_table must not be empty")
-    one = page * n_kv * hd
-    t_stride = table.stride(0)
-    if (n_pages > 1 and (ks[0] < one or vs[0] < one)) or (batch > 1 and t_stride < max_pages):
-        _fail("pages or table rows overlap")
-    return ChrNf4Pages(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), max(ks[0], one), max(vs[0], one),
-                       max(t_stride, max_pages), n_pages, page, n_kv, hd, batch, max_pages), device
+    if t_el != 1 and max_pages > 1:
+        _fail("page_table must have contiguous rows")
+    if ks < one or vs < one or t_row < max_pages:  # strides of an axis of one mean nothing
+        if (n_pages > 1 and (ks < one or vs < one)) or (batch > 1 and t_row < max_pages):
+            _fail("pages or table rows overlap")
+        ks, vs, t_row = max(ks, one), max(vs, one), max(t_row, max_pages)
+    return ChrNf4Pages(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), ks, vs, t_row, n_pages, page, n_kv,
+                       hd, batch, max_pages), index
 
 
-def _head_rows(t: torch.Tensor, hd: int, device: torch.device, what: str) -> tuple[int, int, int]:
+def _head_rows(t: torch.Tensor, hd: int, index: int, what: str) -> tuple[int, int, int]:
     """(rows, heads, row stride) of a bf16 ``[T, heads, hd]`` or ``[T, heads*hd]`` view whose rows
     are contiguous."""
-    _on(t, device, _BF16, what)
     shape, stride = t.shape, t.stride()
-    if len(shape) == 3:
-        rows, heads, width = shape
-        if width != hd or stride[2] != 1 or (heads > 1 and stride[1] != hd):
-            _fail(f"{what} must be [T, heads, {hd}] with contiguous rows")
-        row = heads * hd
-    elif len(shape) == 2:
+    if t.dtype is not _BF16 or t.get_device() != index:
+        _fail(f"{what} must be bfloat16 on cuda:{index}")
+    if len(shape) == 2:
         rows, row = shape
-        if row % hd or stride[1] != 1:
+        heads, left = divmod(row, hd)
+        if left or (stride[1] != 1 and row > 1):
             _fail(f"{what} must be [T, heads*{hd}] with contiguous rows")
-        heads = row // hd
+    elif len(shape) == 3:
+        rows, heads, width = shape
+        row = heads * hd
+        if width != hd or stride[2] != 1 or (stride[1] != hd and heads > 1):
+            _fail(f"{what} must be [T, heads, {hd}] with contiguous rows")
     else:
         _fail(f"{what} must be [T, heads, hd] or [T, heads*hd]")
-    if rows > 1 and stride[0] < row:
-        _fail(f"{what} rows overlap")
-    return rows, heads, max(stride[0], row)
+    step = stride[0]
+    if step < row:
+        if rows > 1:
+            _fail(f"{what} rows overlap")
+        step = row
+    return rows, heads, step
 
 
 def nf4_rope_kv_paged(
@@ -159,14 +162,16 @@ def nf4_rope_kv_paged(
         _fail("k must have rows")
     if seq is None and rows > pages.batch:
         _fail(f"{rows} rows for {pages.batch} sequences need seq")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.stride() != sin.stride() or cos.stride(1) != 1:
+    f32 = cos.dtype is _F32
+    tab = cos.shape
+    step = cos.stride()
+    if (not f32 and cos.dtype is not _BF16) or sin.dtype is not cos.dtype or cos.get_device() != device \
+            or sin.get_device() != device:
+        _fail(f"cos and sin must be float32 or bfloat16, both on cuda:{device}")
+    if len(tab) != 2 or sin.shape != tab or sin.stride() != step or (step[1] != 1 and tab[1] > 1):
         _fail("cos and sin must be [positions, rot/2] of one layout with contiguous rows")
-    if cos.dtype is not _F32 and cos.dtype is not _BF16:
-        _fail("cos and sin must be float32 or bfloat16")
-    _on(cos, device, cos.dtype, "cos")
-    _on(sin, device, cos.dtype, "sin")
-    tab_rows, half = cos.shape
-    tab_stride = cos.stride(0)
+    tab_rows, half = tab
+    tab_stride = step[0]
     if tab_rows < 1 or half < 1 or 2 * half > hd or (tab_rows > 1 and tab_stride < half):
         _fail(f"cos and sin must have 1..{hd // 2} columns and positions")
     n_q = qs = os_ = 0
@@ -176,7 +181,7 @@ def nf4_rope_kv_paged(
         if q_rows != rows or n_q < 1:
             _fail("q must have k's rows")
         if q_out is None:
-            q_out = torch.empty((rows, n_q, hd), dtype=_BF16, device=device)
+            q_out = torch.empty((rows, n_q, hd), dtype=_BF16, device=q.device)
             os_, zero = n_q * hd, 1
         else:
             o_rows, o_heads, os_ = _head_rows(q_out, hd, device, "q_out")
@@ -186,7 +191,7 @@ def nf4_rope_kv_paged(
         _fail("q_out goes with q")
     _call("chr_nf4_rope_kv_paged", device, pages, 0 if q is None else q.data_ptr(), qs, k.data_ptr(), ks,
           v.data_ptr(), vs, 0 if q is None else q_out.data_ptr(), os_, cos.data_ptr(), sin.data_ptr(),
-          max(tab_stride, half), tab_rows, 1 if cos.dtype is _F32 else 0, 2 * half, 1 if interleaved else 0,
+          max(tab_stride, half), tab_rows, 1 if f32 else 0, 2 * half, 1 if interleaved else 0,
           _vector(seq, rows, device, _I32, "seq"), _vector(slot, rows, device, _I64, "slot"),
           _vector(position, rows, device, _I64, "position"), rows, n_q, zero)
     return q_out
@@ -225,20 +230,21 @@ def nf4_attn_paged(
         _fail("q must have rows and a multiple of the pools' n_kv heads")
     words = 0
     if tree is not None:
-        if tree.dtype is not _I64 or tree.device != device or tree.dim() != 2 or tree.size(0) != rows \
+        if tree.dtype is not _I64 or tree.get_device() != device or tree.dim() != 2 or tree.size(0) != rows \
                 or tree.size(1) < 1 or not tree.is_contiguous():
-            _fail(f"tree must be contiguous int64 [{rows}, words] on {device}")
+            _fail(f"tree must be contiguous int64 [{rows}, words] on cuda:{device}")
         words = tree.size(1)
     if q_start is None and rows != batch:
         _fail(f"{rows} rows for {batch} sequences need q_start")
     zero = 0
     if out is None:
-        out = torch.empty((rows, n_q * hd), dtype=_BF16, device=device)
+        out = torch.empty((rows, n_q * hd), dtype=_BF16, device=q.device)
         zero = 1
-    elif out.dtype is not _BF16 or out.device != device or out.numel() != rows * n_q * hd or not out.is_contiguous():
-        _fail(f"out must be contiguous bfloat16 [{rows}, {n_q * hd}] on {device}")
-    need = _ws_floats(device.index, rows, batch, n_q, pages.n_kv, hd, pages.max_pages * pages.page)
-    ws = torch.empty(need, dtype=_F32, device=device)
+    elif out.dtype is not _BF16 or out.get_device() != device or out.numel() != rows * n_q * hd \
+            or not out.is_contiguous():
+        _fail(f"out must be contiguous bfloat16 [{rows}, {n_q * hd}] on cuda:{device}")
+    need = _ws_floats(device, rows, batch, n_q, pages.n_kv, hd, pages.max_pages * pages.page)
+    ws = torch.empty(need, dtype=_F32, device=q.device)
     _call("chr_nf4_attn_paged", device, pages, q.data_ptr(), qs, out.data_ptr(),
           _vector(q_start, batch + 1, device, _I32, "q_start"), _vector(kv_len, batch, device, _I32, "kv_len"),
           0 if tree is None else tree.data_ptr(), words, rows, n_q, float(scale), ws.data_ptr(), need, zero)
@@ -276,14 +282,15 @@ def nf4_sample_commit_batch(
     A ``temperature`` (float32; default 1) of 0 picks greedily. ``prob`` (float32 ``[B]``) receives
     the probability the token was drawn with. The same inputs give the same tokens. See
     ``chr_nf4_sample_commit_batch``."""
-    if not logits.is_cuda or logits.dtype is not _BF16 or logits.dim() != 2 or logits.stride(1) != 1:
-        _fail("logits must be a CUDA bfloat16 [B, n] view with contiguous rows")
+    device = logits.get_device()
+    if device < 0 or logits.dtype is not _BF16 or logits.dim() != 2:
+        _fail("logits must be a CUDA bfloat16 [B, n]")
     b, n = logits.shape
+    stride, el = logits.stride()
     if b < 1 or not 1 <= n <= SAMPLE_MAX_VOCAB:
         _fail(f"logits must have rows of 1..{SAMPLE_MAX_VOCAB} tokens")
-    device, stride = logits.device, logits.stride(0)
-    if b > 1 and stride < n:
-        _fail("logits rows overlap")
+    if (el != 1 and n > 1) or (b > 1 and stride < n):
+        _fail("logits must have contiguous rows that do not overlap")
     if u is None or next_token is None:
         _fail("u and next_token are needed")
     _call("chr_nf4_sample_commit_batch", device, logits.data_ptr(), max(stride, n), n, b,
