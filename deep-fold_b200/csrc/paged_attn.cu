@@ -600,6 +600,7 @@ namespace {
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr int kJoinFew = 16;
+constexpr int kMaxCtas = 1024;   // pieces an item can lie in
 
 __device__ __forceinline__ void join_store(const PagedAttnArgs &a, const PagedCut &cut, int r, int lane, float4 acc,
                                            float l) {
@@ -618,6 +619,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Pag
   __shared__ PagedCut cuts[kJoinWarps];
   __shared__ float4 fold[kJoinWarps][32];
   __shared__ float red[2][kJoinWarps];
+  __shared__ float weight[kMaxCtas];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int hd = a.c.hd;
   pdl_trigger();
@@ -643,8 +645,10 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Pag
   };
   // ... and its maximum and sum; a piece that was rounded away wrote none
   auto ml_of = [&](const PagedCut &t, int i, int r) {
-    const int live = i < t.n ? __ldcg(&ws.cut[t.pad + i].live[i == 0 ? 1 : 0]) : 0;
-    return live != 0 ? __ldcg(ws.ml + part(t, i, r)) : make_float2(-INFINITY, 0.f);
+    const int at = min(i, t.n - 1);
+    const int live = __ldcg(&ws.cut[t.pad + at].live[at == 0 ? 1 : 0]);
+    const float2 ml = __ldcg(ws.ml + part(t, at, r));
+    return i < t.n && live != 0 ? ml : make_float2(-INFINITY, 0.f);
   };
   auto add = [&](float4 &acc, float w, long long at) {
     if (w != 0.f && lane * 4 < hd) {
@@ -672,9 +676,17 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Pag
     const PagedCut t = cuts[k];
     if (t.n <= kJoinFew) continue;
     for (int r = blockIdx.y; r < t.rows; r += gridDim.y) {
-      // pieces warp * 32 + lane, + 256, ... for the maximum and the sum
-      float mm = -INFINITY;
-      for (int i = tid; i < t.n; i += kJoinThreads) mm = fmaxf(mm, ml_of(t, i, r).x);
+      float mm = -INFINITY, mine[kMaxCtas / kJoinThreads][2];
+#pragma unroll
+      for (int k2 = 0; k2 < kMaxCtas / kJoinThreads; ++k2) {
+        const int i = tid + k2 * kJoinThreads;
+        if (k2 * kJoinThreads < t.n) {
+          const float2 ml = ml_of(t, i, r);
+          mine[k2][0] = ml.x;
+          mine[k2][1] = ml.y;
+          mm = fmaxf(mm, ml.x);
+        }
+      }
       mm = warp_max_xor(mm);
       if (lane == 0) red[0][warp] = mm;
       __syncthreads();
@@ -682,14 +694,18 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Pag
       for (int w = 0; w < kJoinWarps; ++w) mm = fmaxf(mm, red[0][w]);
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       float l = 0.f;
-      for (int i0 = warp * 8; i0 < t.n; i0 += kJoinThreads / 4) {
-        // eight pieces of this warp at a time: their weights in lanes, then their outputs
-        const float2 ml = lane < 8 ? ml_of(t, i0 + lane, r) : make_float2(-INFINITY, 0.f);
-        const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mm);
-        l = fmaf(w, ml.y, l);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) add(acc, __shfl_sync(0xffffffffu, w, i), part(t, min(i0 + i, t.n - 1), r));
+      for (int k2 = 0; k2 < kMaxCtas / kJoinThreads; ++k2) {
+        const int i = tid + k2 * kJoinThreads;
+        if (i < t.n) {
+          const float w = mine[k2][0] == -INFINITY ? 0.f : fast_exp2(mine[k2][0] - mm);
+          l = fmaf(w, mine[k2][1], l);
+          weight[i] = w;
+        }
       }
+      __syncthreads();
+#pragma unroll 4
+      for (int i = warp; i < t.n; i += kJoinWarps) add(acc, weight[i], part(t, i, r));
       l = warp_sum_xor(l);
       if (lane == 0) red[1][warp] = l;
       fold[warp][lane] = acc;
@@ -718,25 +734,23 @@ struct AttnForm {
 };
 // The form of a call: from the head layout and the mean number of new rows per sequence,
 // which the host knows, never from the lengths, which it does not.
-AttnForm form_of(int T, int batch, int n_rep, int n_kv, int hd, long long cap) {
+AttnForm form_of(int T, int batch, int n_rep, int hd) {
   const long long rows = (static_cast<long long>(T) + batch - 1) / batch * n_rep;
-  const long long sms = sm_count();
+  const int sms = std::min(sm_count(), kMaxCtas / 2);
   AttnForm f;
   if (rows > 32 && (hd == 64 || hd == 128)) {
     f.M = kWideM;
     f.tile = kWideTile;
     f.extra = 2 * kWideTile;  // queries in, result out (measured)
-    f.ctas = static_cast<int>(sms);  // one resident CTA per SM
+    f.ctas = sms;             // one resident CTA per SM
     return f;
   }
   f.M = rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
   f.tile = kThinTile;
   f.extra = 3 * kThinTile;  // what starting and folding a segment takes, in rows (measured)
-  // Two resident CTAs per SM, and up to eight in all, so that an SM that is served faster
-  // takes more of them; no more than one for every 512 cache rows the tables can hold.
-  const long long items = (rows + f.M - 1) / f.M * batch * n_kv;
-  const long long want = items * (cap + f.extra) / 512;
-  f.ctas = static_cast<int>(std::min(std::max(want, 2 * sms), 2 * sms));
+  // Two resident CTAs per SM. (Three to eight, so that an SM that is served faster takes more
+  // of them, cost more in starts than they balance: 64 sequences 110 us against 108.)
+  f.ctas = 2 * sms;
   return f;
 }
 
@@ -820,12 +834,9 @@ cudaError_t launch_wide(const PagedAttnArgs &a, int negate, int ctas, cudaStream
 using namespace chr;
 
 extern "C" int64_t chr_nf4_attn_paged_ws(int32_t T, int32_t batch, int32_t n_q, int32_t n_kv,
-                                         int32_t hd, int64_t cap) {
-  if (T < 1 || batch < 1 || n_q < 1 || n_kv < 1 || n_q % n_kv != 0 || !head_dim_ok(hd) || cap < 1 ||
-      cap > 0x7fffffffll) {
-    return 0;
-  }
-  const AttnForm f = form_of(T, batch, n_q / n_kv, n_kv, hd, cap);
+                                         int32_t hd) {
+  if (T < 1 || batch < 1 || n_q < 1 || n_kv < 1 || n_q % n_kv != 0 || !head_dim_ok(hd)) return 0;
+  const AttnForm f = form_of(T, batch, n_q / n_kv, hd);
   return ws_floats_of(f.ctas, f.M, hd);
 }
 
@@ -853,7 +864,7 @@ extern "C" int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, i
   }
   const int n_rep = n_q / a.c.n_kv;
   a.p.cap = static_cast<int>(static_cast<long long>(a.c.max_pages) << a.c.page_shift);
-  const AttnForm f = form_of(T, a.c.batch, n_rep, a.c.n_kv, hd, a.p.cap);
+  const AttnForm f = form_of(T, a.c.batch, n_rep, hd);
   if (ws_floats < ws_floats_of(f.ctas, f.M, hd)) return kWorkspace;
   a.p.q_start = static_cast<const int32_t *>(q_start);
   a.p.kv_len = static_cast<const int32_t *>(kv_len);

@@ -168,7 +168,7 @@ SIGNATURES = {
          c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_int32,
          c_int32, c_int32, c_void_p],
     ),
-    "chr_nf4_attn_paged_ws": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int64]),
+    "chr_nf4_attn_paged_ws": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
     "chr_nf4_attn_paged": (
         c_int,
         [_PAGES, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,

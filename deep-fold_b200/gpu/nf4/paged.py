@@ -243,7 +243,7 @@ def nf4_attn_paged(
     elif out.dtype is not _BF16 or out.get_device() != device or out.numel() != rows * n_q * hd \
             or not out.is_contiguous():
         _fail(f"out must be contiguous bfloat16 [{rows}, {n_q * hd}] on cuda:{device}")
-    need = _ws_floats(device, rows, batch, n_q, pages.n_kv, hd, pages.max_pages * pages.page)
+    need = _ws_floats(device, rows, batch, n_q, pages.n_kv, hd)
     ws = torch.empty(need, dtype=_F32, device=q.device)
     _call("chr_nf4_attn_paged", device, pages, q.data_ptr(), qs, out.data_ptr(),
           _vector(q_start, batch + 1, device, _I32, "q_start"), _vector(kv_len, batch, device, _I32, "kv_len"),
@@ -252,9 +252,9 @@ def nf4_attn_paged(
 
 
 @functools.lru_cache(maxsize=4096)
-def _ws_floats(index: int, rows: int, batch: int, n_q: int, n_kv: int, hd: int, cap: int) -> int:
+def _ws_floats(index: int, rows: int, batch: int, n_q: int, n_kv: int, hd: int) -> int:
     with torch.cuda.device(index):
-        return int(_lib.load().chr_nf4_attn_paged_ws(rows, batch, n_q, n_kv, hd, cap))
+        return int(_lib.load().chr_nf4_attn_paged_ws(rows, batch, n_q, n_kv, hd))
 
 
 def nf4_sample_commit_batch(

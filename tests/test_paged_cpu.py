@@ -94,9 +94,8 @@ def test_workspace_query_answers_zero_for_what_the_call_refuses():
     from gpu.nf4 import _lib
 
     ws = _lib.load().chr_nf4_attn_paged_ws
-    assert ws(3, 2, 8, 2, 64, 64) > 0
-    for bad in ((0, 2, 8, 2, 64, 64), (3, 0, 8, 2, 64, 64), (3, 2, 7, 2, 64, 64), (3, 2, 8, 0, 64, 64), (3, 2, 8, 2, 48, 64),
-                (3, 2, 8, 2, 64, 0), (3, 2, 8, 2, 64, 1 << 31)):
+    assert ws(3, 2, 8, 2, 64) > 0
+    for bad in ((0, 2, 8, 2, 64), (3, 0, 8, 2, 64), (3, 2, 7, 2, 64), (3, 2, 8, 0, 64), (3, 2, 8, 2, 48)):
         assert ws(*bad) == 0
 
 
