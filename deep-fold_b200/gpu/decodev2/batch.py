@@ -20,11 +20,12 @@ pass over the weights costs less than two GEMV launches. Single GPU only.
 from __future__ import annotations
 
 from collections.abc import Sequence
+from dataclasses import dataclass
 
 import torch
 
 from gpu.nf4 import (ATTN_SPLIT, GEMV_MAX_N, nf4_attn_batch, nf4_gemm_rows, nf4_gemv_n,
-                     nf4_pick_commit_batch, nf4_rms_rows, nf4_silu_mul)
+                     nf4_pick_commit_batch, nf4_rms_rows, nf4_sample_commit_batch, nf4_silu_mul)
 
 from .embed import PackedEmbed
 from .graph import capture_on_side_stream
@@ -32,10 +33,38 @@ from .linear import DeviceLinear, DeviceWeights
 from .runner import consume_prompt
 from .state import DecodeState, GraphSafeKV
 
-__all__ = ["BatchState", "BatchLoop", "batched_greedy_decode", "GEMV_ROWS"]
+__all__ = ["BatchState", "BatchLoop", "Sampling", "batched_greedy_decode", "batched_sampled_decode", "GEMV_ROWS"]
 
 #: sequences up to which the linears take the CUDA-core GEMV (one launch of four rows)
 GEMV_ROWS = min(4, GEMV_MAX_N)
+
+
+@dataclass
+class Sampling:
+    """How each of ``B`` sequences draws its tokens: device vectors of ``nf4_sample_commit_batch``,
+    ``None`` where a setting is off for all."""
+
+    temperature: torch.Tensor | None = None
+    top_k: torch.Tensor | None = None
+    top_p: torch.Tensor | None = None
+    min_p: torch.Tensor | None = None
+
+    @classmethod
+    def of(cls, batch: int, device="cuda", *, temperature=None, top_k=None, top_p=None, min_p=None) -> "Sampling":
+        """From a number for all sequences, or one per sequence."""
+        def vec(v, dtype):
+            if v is None:
+                return None
+            t = torch.as_tensor(v, dtype=dtype).reshape(-1)
+            if t.numel() not in (1, batch):
+                raise ValueError(f"{t.numel()} settings for {batch} sequences")
+            return t.expand(batch).contiguous().to(device)
+
+        return cls(vec(temperature, torch.float32), vec(top_k, torch.int32), vec(top_p, torch.float32),
+                   vec(min_p, torch.float32))
+
+    def settings(self) -> dict:
+        return dict(temperature=self.temperature, top_k=self.top_k, top_p=self.top_p, min_p=self.min_p)
 
 
 class BatchState:
@@ -168,6 +197,13 @@ def batched_greedy_decode(state: BatchState, weights: DeviceWeights) -> None:
                           state.position, state.finished, int(state.spec.eos_id))
 
 
+def batched_sampled_decode(state: BatchState, weights: DeviceWeights, sampling: Sampling, u: torch.Tensor) -> None:
+    """Forward for every sequence, then a draw with its uniform number ``u[b]`` + commit on the device."""
+    batched_forward(state, weights)
+    nf4_sample_commit_batch(state.logits, u, state.next_token, token=state.token, position=state.position,
+                            finished=state.finished, eos=int(state.spec.eos_id), **sampling.settings())
+
+
 class BatchLoop:
     """Prefill ``B`` prompts, then decode them together (optionally as one CUDA graph per step)."""
 
@@ -193,14 +229,25 @@ class BatchLoop:
 
     @torch.no_grad()
     def generate(self, prompts: Sequence[Sequence[int]], n_new: int,
-                 chunk: int | None = None) -> list[list[int]]:
-        """``n_new`` greedy ids per sequence (EOS ignored), read back once at the end."""
+                 chunk: int | None = None, *, sampling: Sampling | None = None,
+                 u: torch.Tensor | None = None) -> list[list[int]]:
+        """``n_new`` ids per sequence (EOS ignored), read back once at the end: greedy ones, or with
+        ``sampling`` drawn with the uniform numbers ``u [n_new, B]`` (step by step, not captured)."""
         st = self.state
+        if sampling is not None and (u is None or tuple(u.shape) != (max(1, int(n_new)), st.batch)):
+            raise ValueError(f"sampling needs u [{max(1, int(n_new))}, {st.batch}]")
         st.prefill(self.weights, prompts, chunk=chunk)
+        if sampling is not None:  # the first token too is drawn, from the prompts' last logits
+            for i, one in enumerate(st._seq):
+                st.logits[i].copy_(one.arena.logits.view(-1))
+            nf4_sample_commit_batch(st.logits, u[0], st.next_token, token=st.token, **sampling.settings())
         trace = torch.zeros((max(1, int(n_new)), st.batch), dtype=torch.int64, device=st.device)
         trace[0].copy_(st.next_token)
         for i in range(1, int(n_new)):
-            self.step()
+            if sampling is None:
+                self.step()
+            else:
+                batched_sampled_decode(st, self.weights, sampling, u[i])
             trace[i].copy_(st.token)
         torch.cuda.synchronize()
         return [[int(t) for t in trace[:, j].tolist()] for j in range(st.batch)]
