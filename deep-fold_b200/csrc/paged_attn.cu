@@ -133,6 +133,31 @@ __device__ __forceinline__ uint32_t seen32(const PagedAttnArgs &a, const Seg &g,
   return m;
 }
 
+// A masked value enters the second product with weight zero, and 0 x NaN is NaN. So where some of
+// an item's rows do not see all of a tile's cache rows, infinities and NaN among their values are
+// taken out before the product, and added to the rows that do see them.
+constexpr uint32_t kExp2 = 0x7F807F80u;  // the exponents of two bf16
+// Bits 15 and 31: whether the lower, the upper of two bf16 is an infinity or NaN (the sum carries
+// out of an exponent of ones alone).
+__device__ __forceinline__ uint32_t not_finite2(uint32_t x) { return (x & kExp2) + 0x00800080u; }
+__device__ __forceinline__ uint32_t not_finite8(const uint4 &x) {
+  return (not_finite2(x.x) | not_finite2(x.y) | not_finite2(x.z) | not_finite2(x.w)) & 0x80008000u;
+}
+__device__ __forceinline__ uint32_t finite2(uint32_t x) {
+  return x & ~(((not_finite2(x) >> 15) & 0x00010001u) * 0xFFFFu);
+}
+__device__ __forceinline__ uint4 finite8(const uint4 &x) {
+  return make_uint4(finite2(x.x), finite2(x.y), finite2(x.z), finite2(x.w));
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 x;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(addr) : "memory");
+  return x;
+}
+__device__ __forceinline__ void sts16(uint32_t addr, const uint4 &x) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+}
+
 // Zeros for the rows behind the last sequence's, when the call asks for them.
 template <int HD>
 __device__ __forceinline__ void zero_tail_rows(const PagedAttnArgs &a, int cta, int G) {
@@ -494,13 +519,52 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             // rows behind the last may hold anything (0 x NaN): zeros for the product
             for (int i = lane; i < 16 * C; i += 32) {
               const int r = i / C;
-              if (row + r >= g.kv_end) {
-                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(v_blk + chunk_at<HD>(r, i - r * C)), "r"(0)
-                             : "memory");
-              }
+              if (row + r >= g.kv_end) sts16(v_blk + chunk_at<HD>(r, i - r * C), make_uint4(0, 0, 0, 0));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
+          }
+          if (row + 16 > seen_by_all) {
+            uint32_t bad = 0;
+#pragma unroll
+            for (int k = 0; k < (C + 1) / 2; ++k) {
+              const int i = lane + k * 32;
+              bad |= not_finite8(lds16(v_blk + chunk_at<HD>(i / C, i % C)));
+            }
+            if (__any_sync(0xffffffffu, bad != 0u)) {
+#pragma unroll 1
+              for (int j = 0; j < 16; ++j) {
+                bool sees[NQ][2];
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) sees[n][e] = (seen32(a, g, token[n][e], row) >> j) & 1u;
+                }
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                  uint16_t u;
+                  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(v_blk + chunk_at<HD>(j, c) + g8 * 2) : "memory");
+                  const float x = __uint_as_float(static_cast<uint32_t>(u) << 16);
+                  if (not_finite2(u) & 0x8000u) {
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+                      for (int e = 0; e < 2; ++e) {
+                        if (sees[n][e]) o[n][c >> 1][e + 2 * (c & 1)] += x;
+                      }
+                    }
+                  }
+                }
+              }
+              __syncwarp();
+#pragma unroll 1
+              for (int i = lane; i < 16 * C; i += 32) {
+                const uint32_t at16 = v_blk + chunk_at<HD>(i / C, i % C);
+                sts16(at16, finite8(lds16(at16)));
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+            }
           }
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {

@@ -54,6 +54,7 @@ struct WideBars {
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [query tile][buffer]
   uint64_t q_full[2];
   uint32_t bad[4];  // pages of the last tiles that are none, a bit per page
+  uint32_t odd;     // segments with infinities or NaN among the values not all rows see, a bit each
   uint32_t tmem;
   int fail;
 };
@@ -89,6 +90,46 @@ __device__ __forceinline__ bool bar_wait(WideBars &w, uint64_t *b, uint32_t pari
   return false;
 }
 
+// First cache row that not all rows of an item see.
+__device__ __forceinline__ int not_all_see(const PagedAttnArgs &a, int base, int tok0) {
+  return max(a.tree != nullptr ? base : base + tok0 + 1, 0);
+}
+
+// Adds the infinities and NaN that the product was spared to the accumulator of this thread's
+// row, where it sees them: the segment's values are read once more, element by element. Rare.
+template <int HD>
+__device__ __noinline__ void add_not_finite(const PagedAttnArgs &a, const Seg &g, int token, bool mine, uint32_t o_addr) {
+  const int first = max(not_all_see(a, g.base, g.tok0), g.t0 * kWideTile), end = min(g.kv_end, g.t1 * kWideTile);
+#pragma unroll 1
+  for (int c = 0; c < HD; c += 16) {
+    uint32_t o[16];
+    tmem_ld16(o_addr + c, o);
+    tmem_wait_ld();
+#pragma unroll 1
+    for (int key = first; key < end; ++key) {
+      const int id = __ldg(a.c.table + g.b * a.c.table_stride + (key >> a.c.page_shift));
+      if (!mine || id < 0 || id >= a.c.n_pages || (seen32(a, g, token, key) & 1u) == 0u) continue;
+      const int in_page = key & ((1 << a.c.page_shift) - 1);
+      const uint4 *v = reinterpret_cast<const uint4 *>(
+          a.c.v + id * a.c.v_page_stride + (static_cast<long long>(in_page) * a.c.n_kv + g.kvh) * HD + c);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 x = __ldcg(v + h);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t f = not_finite2(xs[e]);
+          if (f & 0x8000u) o[h * 8 + 2 * e] = __float_as_uint(__uint_as_float(o[h * 8 + 2 * e]) + bf16_lo(xs[e]));
+          if (f >> 31) o[h * 8 + 2 * e + 1] = __float_as_uint(__uint_as_float(o[h * 8 + 2 * e + 1]) + bf16_hi(xs[e]));
+        }
+      }
+    }
+    __syncwarp();
+    tmem_st16(o_addr + c, o);
+    tmem_wait_st();
+  }
+}
+
 // A barrier of the whole block that the roles reach from different places.
 __device__ __forceinline__ void block_sync() { asm volatile("bar.sync 0;" ::: "memory"); }
 
@@ -122,6 +163,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       bar_init(&w.v_fixed[i], 1);
     }
     w.fail = 0;
+    w.odd = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_map(&k_map);
     prefetch_map(&v_map);
@@ -156,7 +198,10 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   auto next_batch = [&](int n) {
     if (n < kSegs) return 0;  // there are no more
     block_sync();
-    if (tid == 0) walk.n_segs = w.fail != 0 ? 0 : walk_fill(a, walk.at, walk.note, cta, G, segs);
+    if (tid == 0) {
+      w.odd = 0;
+      walk.n_segs = w.fail != 0 ? 0 : walk_fill(a, walk.at, walk.note, cta, G, segs);
+    }
     block_sync();
     n = walk.n_segs;
     block_sync();
@@ -213,15 +258,25 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
                          g.kvh, in_page, id);
               }
             }
-            if ((t + 1) * kWideTile > g.kv_end) {
-              // rows behind the last may hold anything (0 x NaN): zeros for the second product
+            const int unseen = max(not_all_see(a, g.base, g.tok0) - t * kWideTile, 0);
+            if (unseen < kWideTile) {
+              // made fit for the second product: rows behind the last, which may hold anything,
+              // become zeros, and so do infinities and NaN in those not all rows see
               ok = __all_sync(0xffffffffu, bar_wait(w, &w.v_full[st], ph, 3));
               if (!ok) break;
-              const int first = max(g.kv_end - t * kWideTile, 0);
-              for (int i = lane; i < (kWideTile - first) * 8 * L::kHalves; i += 32) {
-                const int r = first + (i >> 3) / L::kHalves, h = (i >> 3) % L::kHalves;
-                *reinterpret_cast<uint4 *>(sm + L::kV + st * L::kTileB + h * L::kPiece + r * 128 + (i & 7) * 16) =
-                    make_uint4(0, 0, 0, 0);
+              const int first = min(max(g.kv_end - t * kWideTile, 0), kWideTile);
+              auto piece = [&](int i) {  // 16 bytes
+                const int r = (i >> 3) / L::kHalves, h = (i >> 3) % L::kHalves;
+                return base + L::kV + st * L::kTileB + h * L::kPiece + r * 128 + (i & 7) * 16;
+              };
+              uint32_t odd = 0;
+#pragma unroll 8
+              for (int i = unseen * 8 * L::kHalves + lane; i < first * 8 * L::kHalves; i += 32) odd |= not_finite8(lds16(piece(i)));
+              for (int i = first * 8 * L::kHalves + lane; i < kWideTile * 8 * L::kHalves; i += 32) sts16(piece(i), make_uint4(0, 0, 0, 0));
+              if (__any_sync(0xffffffffu, odd != 0u)) {
+#pragma unroll 1
+                for (int i = unseen * 8 * L::kHalves + lane; i < first * 8 * L::kHalves; i += 32) sts16(piece(i), finite8(lds16(piece(i))));
+                if (lane == 0) *reinterpret_cast<volatile uint32_t *>(&w.odd) = w.odd | 1u << si;
               }
               asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
               __syncwarp();
@@ -282,7 +337,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         for (int si = 0; si < n_u && ok; ++si) {
           const int t0 = __shfl_sync(0xffffffffu, segs[si].t0, 0);
           const int tiles = __shfl_sync(0xffffffffu, segs[si].t1, 0) - t0;
-          const int tail = __shfl_sync(0xffffffffu, segs[si].kv_end, 0) < (t0 + tiles) * kWideTile ? tiles - 1 : -1;
+          const int fixed_from = __shfl_sync(0xffffffffu, not_all_see(a, segs[si].base, segs[si].tok0), 0) - t0 * kWideTile;
           const bool two = __shfl_sync(0xffffffffu, segs[si].rows, 0) > 128;
           wait(&w.q_full[0], n_q[0]++ & 1, 6);
           if (two) wait(&w.q_full[1], n_q[1]++ & 1, 6);
@@ -297,7 +352,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             const int st = n_kv & 1;
             const bool more = i + 1 < tiles;
             wait(&w.v_full[st], (n_kv >> 1) & 1, 8);
-            if (i == tail) {
+            if ((i + 1) * kWideTile > fixed_from) {
               wait(&w.v_fixed[st], (fixed >> st) & 1u, 9);
               fixed ^= 1u << st;
             }
@@ -467,6 +522,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         ok = __all_sync(0xffffffffu, bar_wait(w, &w.pv_done[tile][(n_s - 1) & 1], ((n_s - 1) >> 1) & 1, 12));
         if (!ok) break;
         tc_fence_after();
+        if ((*reinterpret_cast<volatile uint32_t *>(&w.odd) >> si) & 1u) add_not_finite<HD>(a, g, token, mine, o_addr);
         const bool whole = g.whole;
         const int head = head_of(a.p, g, first_row + r, token);
         const float by = l_run != 0.f ? 1.f / l_run : 0.f;

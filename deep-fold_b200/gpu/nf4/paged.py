@@ -122,6 +122,18 @@ def _head_rows(t: torch.Tensor, hd: int, index: int, what: str) -> tuple[int, in
     return rows, heads, step
 
 
+def _overlap(a: torch.Tensor, a_rows: int, a_step: int, a_row: int, b: torch.Tensor, b_rows: int, b_step: int,
+             b_row: int) -> bool:
+    """Whether two row views share memory; views of one stacked product (one step, side by side) do not."""
+    gap = (b.data_ptr() - a.data_ptr()) // 2
+    if gap >= (a_rows - 1) * a_step + a_row or -gap >= (b_rows - 1) * b_step + b_row:
+        return False
+    if a_step == b_step:
+        off = gap % a_step
+        return off < a_row or off + b_row > a_step
+    return True
+
+
 def nf4_rope_kv_paged(
     q: torch.Tensor | None,
     k: torch.Tensor,
@@ -187,6 +199,9 @@ def nf4_rope_kv_paged(
             o_rows, o_heads, os_ = _head_rows(q_out, hd, device, "q_out")
             if o_rows != rows or o_heads != n_q:
                 _fail("q_out must have q's shape")
+            if (q_out.data_ptr() != q.data_ptr() or (os_ != qs and rows > 1)) and \
+                    _overlap(q_out, rows, os_, n_q * hd, q, rows, qs, n_q * hd):
+                _fail("q_out must be q or not overlap it")
     elif q_out is not None:
         _fail("q_out goes with q")
     _call("chr_nf4_rope_kv_paged", device, pages, 0 if q is None else q.data_ptr(), qs, k.data_ptr(), ks,
@@ -243,6 +258,8 @@ def nf4_attn_paged(
     elif out.dtype is not _BF16 or out.get_device() != device or out.numel() != rows * n_q * hd \
             or not out.is_contiguous():
         _fail(f"out must be contiguous bfloat16 [{rows}, {n_q * hd}] on cuda:{device}")
+    elif _overlap(out, rows, n_q * hd, n_q * hd, q, rows, qs, n_q * hd):
+        _fail("out must not overlap q")
     need = _ws_floats(device, rows, batch, n_q, pages.n_kv, hd)
     ws = torch.empty(need, dtype=_F32, device=q.device)
     _call("chr_nf4_attn_paged", device, pages, q.data_ptr(), qs, out.data_ptr(),

@@ -437,10 +437,12 @@ int chr_nf4_rope_kv_paged(const chr_nf4_pages_t *pages, const void *q, int64_t q
  * [T, n_q * hd] contiguous. A row that sees nothing gives zeros; rows behind the last
  * sequence's are left alone (zero_tail = 0) or zeroed. FP32 scores, running softmax and
  * accumulation; probabilities are rounded to bf16 for the value product. Cache rows at
- * kv_len and beyond may hold anything; the new rows' own v must be finite, since a
- * masked one enters the product with weight zero.
- * ws: chr_nf4_attn_paged_ws(...) floats, 16-byte aligned, no initial contents needed; two calls that may overlap on the device need one each. Two launches. Capturable: lengths, tables and
- * masks are read on the device, and a replay follows what they hold then.
+ * kv_len and beyond may hold anything; infinities and NaN in a new row reach the rows
+ * that see it and no others. A cache row on a page outside the pool is seen by none.
+ * out must not overlap q. ws: chr_nf4_attn_paged_ws(...) floats, 16-byte aligned, no
+ * initial contents needed; two calls that may overlap on the device need one each. Two
+ * launches. Capturable: lengths, tables and masks are read on the device, and a replay
+ * follows what they hold then.
  * Returns 0, -1 (null), -3 (dims), -5 (alignment: q, out, ws, pools 16 bytes), -6, -7. */
 int64_t chr_nf4_attn_paged_ws(int32_t T, int32_t batch, int32_t n_q, int32_t n_kv, int32_t hd);
 int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, int64_t q_stride, void *out,

@@ -133,3 +133,17 @@ def test_pages_struct_matches_the_header(tmp_path):
     subprocess.run(["gcc", f"-I{ROOT / 'include'}", str(src), "-o", str(exe)], check=True)
     got = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
     assert got == [ctypes.sizeof(ChrNf4Pages)] + [getattr(ChrNf4Pages, f).offset for f in fields]
+
+
+def test_overlap_of_row_views():
+    from gpu.nf4.paged import _overlap
+
+    y = torch.empty((6, 100), dtype=torch.bfloat16)
+    q, k, late = y[:, :60], y[:, 60:], y[3:, :60]
+    flat = torch.empty(400, dtype=torch.bfloat16)
+    assert not _overlap(q, 6, 100, 60, k, 6, 100, 40) and not _overlap(k, 6, 100, 40, q, 6, 100, 60)
+    assert _overlap(q, 6, 100, 60, late, 3, 100, 60) and _overlap(late, 3, 100, 60, q, 6, 100, 60)
+    assert not _overlap(y[:3], 3, 100, 100, y[3:], 3, 100, 100)  # one behind the other
+    assert _overlap(q, 6, 100, 60, y[:, 30:90], 6, 100, 60) and _overlap(y[:, 30:90], 6, 100, 60, q, 6, 100, 60)
+    assert _overlap(flat, 4, 60, 60, flat, 3, 100, 60)           # steps that differ
+    assert not _overlap(flat[:200], 2, 100, 100, flat[200:], 2, 60, 60)

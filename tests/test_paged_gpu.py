@@ -339,3 +339,64 @@ def test_wide_missing_pages_and_more_rows_than_cache_rows():
     q = torch.randn((90, 8, 64), generator=gen, device="cuda").to(BF16)
     got = _check(q, kp, vp, table, kv, _starts(rows), 0.125)
     assert not got[40:60].any() and got[79].any()
+
+
+@pytest.mark.parametrize("n_q,n_kv,hd", [(8, 1, 128), (4, 2, 64), (4, 2, 16), (6, 3, 32), (16, 1, 128), (8, 1, 64)])
+@pytest.mark.parametrize("rows,kv,page", [([3, 2], [20, 90], 16), ([8, 7], [140, 7], 32), ([40, 21], [300, 30], 64),
+                                          ([150, 1], [150, 9], 256)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_what_is_not_finite_reaches_only_the_rows_that_see_it(n_q, n_kv, hd, rows, kv, page, tree):
+    """Infinities and NaN in new rows: a row that does not see them keeps every bit; one that does
+    has them where their element is, or everywhere if they are in the key."""
+    from gpu.nf4 import nf4_attn_paged
+
+    gen = _gen(sum(rows) + n_q)
+    kp, vp, table = ref.make_cache(len(kv), kv, page, n_kv, hd, gen)
+    starts = _starts(rows)
+    q = torch.randn((sum(rows), n_q, hd), generator=gen, device="cuda").to(BF16)
+    bits = _tree_bits(rows, 3, gen) if tree else None
+    if tree:
+        bits[1] = 0  # sees no draft, not even itself
+    call = lambda: nf4_attn_paged(q, kp, vp, table, _i32(kv), hd ** -0.5, q_start=_i32(starts), tree=bits).view(-1, n_q, hd)
+    clean = call()
+    want = clean.clone()
+    n_rep = n_q // n_kv
+    for b, draft, pool, head, el, value in ((0, 1, vp, 0, 3, float("nan")), (0, 2, vp, n_kv - 1, hd - 1, float("inf")),
+                                            (0, rows[0] // 2 + 1, vp, 0, hd // 2, -float("inf")),
+                                            (1, rows[1] - 1, kp, 0, 1, float("nan")),
+                                            (1, rows[1] - 1, vp, 0, 0, float("inf"))):
+        if draft >= rows[b]:
+            continue
+        at = kv[b] - rows[b] + draft
+        pool[int(table[b, at // page]), at % page, head, el] = value
+        for i in range(rows[b]):
+            r = starts[b] + i
+            sees = draft <= i if not tree else bool((int(bits[r, draft // 64]) >> (draft % 64)) & 1)
+            if sees:
+                mine = want[r, head * n_rep:(head + 1) * n_rep]
+                if pool is kp:
+                    mine[:] = float("nan")
+                else:
+                    mine[:, el] += value
+    got = call()
+    same = (got == want) | (torch.isnan(got) & torch.isnan(want))
+    assert same.all(), (~same).nonzero()[:5].tolist()
+    assert not torch.equal(clean, got) or tree
+
+
+def test_results_that_overlap_the_queries_are_refused():
+    from gpu.nf4 import nf4_attn_paged, nf4_rope_kv_paged
+
+    gen = _gen(1)
+    kp, vp, table = ref.make_cache(2, [20, 20], 16, 2, 64, gen)
+    y = torch.randn((3, 8 * 64), generator=gen, device="cuda").to(BF16)
+    q = y[:2]
+    with pytest.raises(RuntimeError, match="overlap"):
+        nf4_attn_paged(q, kp, vp, table, _i32([20, 20]), 0.1, out=y[:2])
+    with pytest.raises(RuntimeError, match="overlap"):
+        nf4_attn_paged(q, kp, vp, table, _i32([20, 20]), 0.1, out=y[1:])
+    cos, sin = _tables(32, 32, torch.float32, gen)
+    k = torch.randn((2, 2 * 64), generator=gen, device="cuda").to(BF16)
+    with pytest.raises(RuntimeError, match="overlap"):
+        nf4_rope_kv_paged(q, k, k, kp, vp, table, cos, sin, _i64([19, 19]), q_out=y[1:])
+    assert nf4_rope_kv_paged(q, k, k, kp, vp, table, cos, sin, _i64([19, 19]), q_out=q) is q
