@@ -11,16 +11,19 @@
 // floating point. No sort, no sum over the vocabulary, the same result in every run.
 //
 // A cluster of C CTAs owns a row. Each CTA counts its slice of the vocabulary in its own
-// shared memory (65536 16-bit counters, 128 KB; a slice is at most 65535 tokens) and marks which
+// shared memory (65536 16-bit counters, 128 KB) and marks which
 // of the 1024 chunks of 64 values occur. The chunks that do - under a hundred, values of a
 // row spanning a dozen binary orders - are dealt over the cluster's warps: a warp adds the
 // CTAs' counters through distributed shared memory, takes one exp per value, and hands
 // counts and weights to the row's first CTA, one warp of which walks the cuts and the draw.
 // The CTA whose slice holds the drawn token finds its index. One launch, no scratch memory.
-// Bound by latency: counting 19,000 tokens per CTA takes 3 us (shared-memory atomics, about 4 a
-// clock), the rest is a chain of cluster barriers and dependent steps.
+// Bound by latency: one row of 151936 tokens on eight CTAs takes 15.2 us, of which counting 2 (19,000
+// tokens a CTA) and finding the token 2.5, the rest is a chain of cluster barriers and dependent
+// steps. 64 such rows, two CTAs each, take 24.2 us: counting 7.5 (shared-memory atomics, about
+// 5 a clock), finding 5. (With four CTAs each, which queue for the SMs, 35.9 us.)
 
 #include <cooperative_groups.h>
+#include <cstddef>
 
 #include "nf4_common.cuh"
 
@@ -35,7 +38,12 @@ constexpr int kKeys = 65536;
 constexpr int kChunk = 64;                 // values per chunk
 constexpr int kChunks = kKeys / kChunk;
 constexpr int kSampleMaxCluster = 8;
-constexpr int kSliceMax = 65535;           // a 16-bit counter never wraps
+// A slice is counted in two parts, the first of at most kPart tokens. A value that holds 32768
+// of them - there is one at most - is then set aside and its counter starts again, so that no
+// 16-bit counter wraps in the second part, of at most 32768 tokens, either.
+constexpr int kPart = 65520;               // in whole 16-byte pieces; the first part takes the ends too
+constexpr int kHeavy = 32768;
+constexpr int kSliceMax = kPart + kHeavy;
 
 struct SampleArgs {
   const __nv_bfloat16 *logits;
@@ -49,13 +57,18 @@ struct SampleArgs {
   int64_t eos;
 };
 
+constexpr int kGroups = 12;                // 32-piece groups of a warp when it looks for the token
+static_assert(kSliceMax / 8 <= kGroups * 32 * kSampleWarps && kGroups % 4 == 0, "a bit per token");
+constexpr int kSampleMaxVocab = 524280;
+static_assert(kSampleMaxVocab <= kSliceMax * kSampleMaxCluster, "a slice per CTA");
 constexpr int kCache = 80;  // chunks whose counts and weights the first CTA keeps
 
 struct SampleShared {
-  uint32_t hist[kKeys / 2];          // counters 2i (low half) and 2i + 1 (high half)
+  alignas(16) uint32_t hist[kKeys / 2];  // counters 2i (low half) and 2i + 1 (high half)
   uint32_t map[kChunks / 32];        // chunks that occur in this CTA's slice; bit c % 32 of word c / 32
-  uint8_t four[kChunks / 4];         // the same, four chunks a byte
+  alignas(16) uint8_t four[kChunks / 4]; // the same, four chunks a byte
   uint32_t max_key;                  // of this CTA's slice
+  uint32_t heavy_key, heavy_n;       // the value set aside (none: kNoKey) and its tokens
   uint32_t found[kSampleWarps];
   // the draw, written by the first CTA into every one
   uint32_t pick_key, pick_rank;      // value and its pick_rank-th occurrence
@@ -64,9 +77,13 @@ struct SampleShared {
   uint32_t count[kChunks];           // tokens, then tokens before the chunk
   double mass[kChunks];              // their weight, likewise
   uint16_t chunk[kChunks];
-  double w[kCache][kChunk];          // values of a chunk, highest first
-  uint32_t n[kCache][kChunk];
+  alignas(16) double w[kCache][kChunk];  // values of a chunk, highest first
+  alignas(16) uint32_t n[kCache][kChunk];
 };
+
+// 16-byte accesses to hist and w, 8-byte ones to four and n
+static_assert(offsetof(SampleShared, hist) % 16 == 0 && offsetof(SampleShared, w) % 16 == 0 &&
+              offsetof(SampleShared, four) % 16 == 0 && offsetof(SampleShared, n) % 16 == 0, "aligned");
 
 // A value's key orders as the value does: the bits of a bf16 with the sign flipped, a
 // negative one with all bits flipped; -0 has +0's key, NaN the highest.
@@ -80,47 +97,52 @@ __device__ __forceinline__ double key_weight(uint32_t key, double m, double temp
   return exp((static_cast<double>(key_value(key)) - m) / temp);
 }
 
-// The 16-byte pieces of elements lo..hi of a row: piece v starts at element first + 8 v; the
-// ones at the ends are read element by element, and what lies outside is marked.
+// Elements lo..hi of a row: up to 7 of them, then whole aligned 16-byte pieces from element
+// `first` on, then up to 7 from element `last` on.
 struct Slice {
   const unsigned short *x;
-  int lo, hi, first, pieces;
+  int lo, hi, first, last, pieces;
 };
 __device__ __forceinline__ Slice slice_of(const __nv_bfloat16 *row, int lo, int hi) {
   Slice s;
   s.x = reinterpret_cast<const unsigned short *>(row);
   s.lo = lo;
   s.hi = hi;
-  s.first = lo - static_cast<int>((reinterpret_cast<uintptr_t>(s.x + lo) & 15) >> 1);
-  s.pieces = (hi - s.first + 7) / 8;
+  s.first = min(lo + static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(s.x + lo) & 15)) & 15) >> 1), hi);
+  s.pieces = (hi - s.first) / 8;
+  s.last = s.first + s.pieces * 8;
   return s;
 }
-constexpr uint32_t kNegInf = 0xFF80u, kNegInfKey = 0x007Fu;
-// Piece v; elements outside the slice read as -inf, `in` tells which are inside.
-__device__ __forceinline__ uint4 slice_piece(const Slice &s, int v, uint32_t &in) {
-  const int at = s.first + v * 8;
-  if (at >= s.lo && at + 8 <= s.hi) {
-    in = 0xFFu;
-    return __ldcg(reinterpret_cast<const uint4 *>(s.x + at));
-  }
-  uint32_t w[4] = {0u, 0u, 0u, 0u};
-  in = 0u;
+constexpr uint32_t kNegInf = 0xFF80u, kNegInfKey = 0x007Fu, kNoKey = 0xFFFFFFFFu;
+// Two pieces, `step` apart; what lies at `end` or beyond is not read.
+__device__ __forceinline__ void slice_pieces(const Slice &s, int v, int step, int end, uint4 (&x)[2]) {
+  const uint4 *src = reinterpret_cast<const uint4 *>(s.x + s.first);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const bool inside = at + e >= s.lo && at + e < s.hi;
-    const uint32_t b = inside ? __ldcg(s.x + at + e) : kNegInf;
-    if (inside) in |= 1u << e;
-    w[e >> 1] |= b << ((e & 1) * 16);
+  for (int k = 0; k < 2; ++k) {
+    x[k] = make_uint4(0u, 0u, 0u, 0u);
+    if (v + k * step < end) x[k] = __ldcg(src + v + k * step);
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Elements before the pieces (tail = false) and behind them, one per lane; -inf where there is none.
+__device__ __forceinline__ uint32_t slice_edge(const Slice &s, bool tail, int lane) {
+  const int at = (tail ? s.last : s.lo) + lane;
+  return at < (tail ? s.hi : s.first) ? __ldcg(s.x + at) : kNegInf;
 }
 // Two bf16 values as order keys, but for NaN and -0, which are put right afterwards.
 __device__ __forceinline__ uint32_t raw_keys(uint32_t two) {
   return two ^ (((two >> 15) & 0x00010001u) * 0xFFFFu | 0x80008000u);
 }
-// One token of key `key`; -inf is not counted (a masked vocabulary would queue up at its counter).
-__device__ __forceinline__ void count_key(SampleShared &sm, uint32_t key) {
-  if (key != kNegInfKey) atomicAdd(&sm.hist[key >> 1], (key & 1u) ? 65536u : 1u);
+// One token of key `key`, at bit kAt of `keys`; -inf is not counted (a masked vocabulary would
+// queue up at its counter).
+template <int kAt>
+__device__ __forceinline__ void count_key(uint32_t hist, uint32_t keys) {
+  const uint32_t key = kAt == 0 ? keys & 0xFFFFu : keys >> 16;
+  const uint32_t at = hist + ((kAt == 0 ? keys << 1 : keys >> 15) & 0x1FFFCu);
+  const uint32_t one = (key & 1u) * 65535u + 1u;  // the upper half counts odd keys
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %0, 127;\n\t"
+      "@p red.shared.add.u32 [%1], %2;\n\t}" ::"r"(key), "r"(at), "r"(one) : "memory");
 }
 
 // The counts of chunk c over the cluster, two values per lane in descending order: lane l
@@ -139,6 +161,17 @@ __device__ __forceinline__ void chunk_counts(cg::cluster_group &cluster, SampleS
   for (int r = 0; r < kSampleMaxCluster; ++r) {
     hi += v[r] >> 16;
     lo += v[r] & 0xFFFFu;
+  }
+}
+// Adds what the CTAs set aside of chunk c; `heavy`: the value that CTA l did.
+__device__ __forceinline__ void add_heavy(cg::cluster_group &cluster, SampleShared &sm, int c, int lane, uint32_t heavy,
+                                          uint32_t &hi, uint32_t &lo) {
+  for (unsigned some = __ballot_sync(0xffffffffu, heavy >> 6 == static_cast<uint32_t>(c)); some != 0u; some &= some - 1u) {
+    const int r = __ffs(some) - 1;
+    const uint32_t n = *cluster.map_shared_rank(&sm.heavy_n, r);
+    const uint32_t at = 63u - (__shfl_sync(0xffffffffu, heavy, r) & 63u);
+    if (at == 2u * lane) hi += n;
+    if (at == 2u * lane + 1u) lo += n;
   }
 }
 
@@ -164,7 +197,9 @@ __device__ __noinline__ ChunkView view_chunk(SampleShared &sm, int i, double m, 
     v.w_hi = w.x;
     v.w_lo = w.y;
   } else {
+    const uint32_t heavy = lane < static_cast<int>(cluster.num_blocks()) ? *cluster.map_shared_rank(&sm.heavy_key, lane) : kNoKey;
     chunk_counts(cluster, sm, c, lane, v.n_hi, v.n_lo);
+    add_heavy(cluster, sm, c, lane, heavy, v.n_hi, v.n_lo);
     v.w_hi = key_weight(v.key, m, temp);
     v.w_lo = key_weight(v.key - 1u, m, temp);
   }
@@ -242,6 +277,10 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
   for (int i = tid; i < kKeys / 8; i += kSampleThreads) {
     reinterpret_cast<uint4 *>(sm.hist)[i] = make_uint4(0, 0, 0, 0);
   }
+  if (tid == 0) {
+    sm.heavy_key = kNoKey;
+    sm.heavy_n = 0u;
+  }
   __syncthreads();
   pdl_wait();
   const __nv_bfloat16 *row = a.logits + b * a.row_stride;
@@ -249,18 +288,48 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
   const Slice slice = slice_of(row, lo, hi);
 
   // ---- the slice's histogram ----
-#pragma unroll 4
-  for (int v = tid; v < slice.pieces; v += kSampleThreads) {
-    uint32_t in;
-    const uint4 x = slice_piece(slice, v, in);
-    const uint32_t two[4] = {raw_keys(x.x), raw_keys(x.y), raw_keys(x.z), raw_keys(x.w)};
+  static_assert(kNegInfKey == 127, "not counted");
+  const uint32_t hist = static_cast<uint32_t>(__cvta_generic_to_shared(sm.hist));
+  if (warp < 2) count_key<0>(hist, raw_keys(slice_edge(slice, warp == 1, lane)));
+#pragma unroll 1
+  for (int from = 0; from < max(slice.pieces, 1); from += kPart / 8) {
+    const int to = min(from + kPart / 8, slice.pieces);
+    uint4 x[2], next[2];
+    slice_pieces(slice, from + tid, kSampleThreads, to, x);
+#pragma unroll 1
+    for (int v = from + tid; v < to; v += 2 * kSampleThreads) {
+      slice_pieces(slice, v + 2 * kSampleThreads, kSampleThreads, to, next);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      count_key(sm, two[e] & 0xFFFFu);
-      count_key(sm, two[e] >> 16);
+      for (int k = 0; k < 2; ++k) {
+        if (v + k * kSampleThreads < to) {
+          const uint32_t two[4] = {raw_keys(x[k].x), raw_keys(x[k].y), raw_keys(x[k].z), raw_keys(x[k].w)};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            count_key<0>(hist, two[e]);
+            count_key<16>(hist, two[e]);
+          }
+        }
+        x[k] = next[k];
+      }
+    }
+    __syncthreads();
+    if (to < slice.pieces) {
+      for (int i = tid; i < kKeys / 8; i += kSampleThreads) {
+        const uint4 x = reinterpret_cast<const uint4 *>(sm.hist)[i];
+        if (((x.x | x.y | x.z | x.w) & 0x80008000u) == 0u) continue;
+        const uint32_t n[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if ((n[e] & 0x80008000u) == 0u) continue;
+          const bool high = (n[e] >> 31) != 0u;
+          sm.heavy_key = static_cast<uint32_t>((i * 4 + e) * 2 + (high ? 1 : 0));
+          sm.heavy_n = high ? n[e] >> 16 : n[e] & 0xFFFFu;
+          sm.hist[i * 4 + e] = high ? n[e] & 0xFFFFu : n[e] & 0xFFFF0000u;
+        }
+      }
+      __syncthreads();
     }
   }
-  __syncthreads();
   // NaN of either sign to the highest key, -0 to +0
   if (warp == 0) {
     uint32_t nans = 0u;
@@ -278,10 +347,23 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
     nans = __reduce_add_sync(0xffffffffu, nans);
     __syncwarp();
     if (lane == 0) {
-      if (nans != 0u) sm.hist[kKeys / 2 - 1] += nans << 16;
+      // a row with a NaN picks the first one, so only whether a slice has some matters
+      if (nans != 0u) sm.hist[kKeys / 2 - 1] += min(nans, 65535u) << 16;
       const uint32_t minus = sm.hist[0x7FFF >> 1] >> 16;  // -0: the high half of word 0x3FFF
+      const uint32_t plus = sm.hist[0x8000 >> 1];
       sm.hist[0x7FFF >> 1] &= 0xFFFFu;
-      sm.hist[0x8000 >> 1] += minus;
+      const uint32_t key = sm.heavy_key;
+      if (key == 0x7FFFu) {
+        sm.heavy_key = 0x8000u;
+      } else if (key != kNoKey && (key < kNegInfKey || key > 0xFF80u)) {
+        sm.heavy_key = 0xFFFFu;
+      }
+      if ((plus & 0xFFFFu) + minus < 65536u) {
+        sm.hist[0x8000 >> 1] = plus + minus;
+      } else {  // too many for the counter, so no other value was set aside
+        sm.heavy_key = 0x8000u;
+        sm.heavy_n += minus;
+      }
     }
   }
   __syncthreads();
@@ -300,6 +382,8 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
     uint32_t w = 0u;
 #pragma unroll
     for (int e = 0; e < 4; ++e) w |= ((v.x >> (8 * e)) & 15u) << (4 * e) | ((v.y >> (8 * e)) & 15u) << (16 + 4 * e);
+    const uint32_t heavy = sm.heavy_key;
+    if (heavy != kNoKey && static_cast<int>(heavy >> 11) == lane) w |= 1u << ((heavy >> 6) & 31u);
     sm.map[lane] = w;
     // the slice's maximum: the highest value of its highest chunk
     const unsigned words = __ballot_sync(0xffffffffu, w != 0u);
@@ -311,10 +395,12 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
       const uint32_t key = static_cast<uint32_t>(c * kChunk + 2 * lane) + ((n >> 16) != 0u ? 1u : 0u);
       best = __reduce_max_sync(0xffffffffu, n != 0u ? key : 0u);
     }
+    if (heavy != kNoKey) best = max(best, heavy);
     if (lane == 0) sm.max_key = best;
   }
   cluster.sync();
 
+  const uint32_t heavy = lane < C ? *cluster.map_shared_rank(&sm.heavy_key, lane) : kNoKey;
   uint32_t max_key = 0u;
 #pragma unroll
   for (int r = 0; r < kSampleMaxCluster; ++r) {
@@ -357,6 +443,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
       chunk_counts(cluster, sm, c, lane, n_hi, n_lo);
       const uint32_t key = static_cast<uint32_t>(c * kChunk + 63 - 2 * lane);
       const double w_hi = key_weight(key, m, temp), w_lo = key_weight(key - 1u, m, temp);
+      add_heavy(cluster, sm, c, lane, heavy, n_hi, n_lo);
       // a value that does not occur may have no finite weight
       double mass = (n_hi != 0u ? n_hi * w_hi : 0.0) + (n_lo != 0u ? n_lo * w_lo : 0.0);
       if (i < kCache) {
@@ -500,58 +587,99 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
       if (r < rank) before += n;
       if (r == rank) here = n;
     }
+    for (unsigned some = __ballot_sync(0xffffffffu, heavy == pick_key && lane <= rank); some != 0u; some &= some - 1u) {
+      const int r = __ffs(some) - 1;
+      const uint32_t n = *cluster.map_shared_rank(&sm.heavy_n, r);
+      if (r < rank) {
+        before += n;
+      } else {
+        here += n;
+      }
+    }
     if (pick_rank >= before && pick_rank < before + here) {
       uint32_t want = pick_rank - before;  // occurrence within the slice
       // its bits: one pattern, but for zero (either sign) and NaN (many)
       const uint32_t bits = (pick_key & 0x8000u) ? (pick_key & 0x7FFFu) : (~pick_key & 0xFFFFu);
-      const uint32_t mask = bits == 0u ? 0x7FFFu : 0xFFFFu;
+      const uint32_t mask = bits == 0u ? 0x7FFF7FFFu : 0xFFFFFFFFu, twice = bits * 0x10001u;
       const bool nan = pick_key == 0xFFFFu;
-      auto is = [&](uint32_t x) { return nan ? (x & 0x7FFFu) > 0x7F80u : (x & mask) == bits; };
-      auto matches = [&](int v) {
-        uint32_t in;
-        const uint4 x = slice_piece(slice, v, in);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-        uint32_t hit = 0u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) hit |= (is(w[e] & 0xFFFFu) ? 1u << (2 * e) : 0u) | (is(w[e] >> 16) ? 2u << (2 * e) : 0u);
-        return hit & in;
+      // bits 15 and 31: whether the lower, the upper of two elements is the value
+      auto is = [&](uint32_t two) {
+        if (nan) return ((two & 0x7FFF7FFFu) + 0x007F007Fu) & 0x80008000u;  // above 0x7F80
+        const uint32_t off = (two ^ twice) & mask;
+        return ~(((off & 0x7FFF7FFFu) + 0x7FFF7FFFu) | off) & 0x80008000u;
       };
-      // a warp's part of the slice, in order of index
+      auto matches = [&](const uint4 &x) {  // bit e: element e of a piece
+        const uint32_t c = is(x.x) >> 15 | is(x.y) >> 13 | is(x.z) >> 11 | is(x.w) >> 9;
+        return (c & 0x55u) | ((c >> 15) & 0xAAu);
+      };
+      // a warp's part of the slice, in order of index: up to kGroups groups of 32 pieces, whose
+      // matches a lane keeps, eight bits a piece; the ends go with the first and last warp's
       const int per = (slice.pieces + kSampleWarps - 1) / kSampleWarps;
       const int w0 = min(warp * per, slice.pieces), w1 = min(w0 + per, slice.pieces);
-      if (here == 1u) {
-#pragma unroll 4
-        for (int v = w0 + lane; v < w1; v += 32) {
-          const uint32_t hit = matches(v);
-          if (hit != 0u) commit(slice.first + v * 8 + __ffs(hit) - 1);
-        }
-      } else {
-        uint32_t mine = 0u;
-#pragma unroll 4
-        for (int v = w0 + lane; v < w1; v += 32) mine += __popc(matches(v));
-        mine = __reduce_add_sync(0xffffffffu, mine);
-        if (lane == 0) sm.found[warp] = mine;
-        __syncthreads();
-        uint32_t skip = 0u;
-        for (int w = 0; w < warp; ++w) skip += sm.found[w];
-        if (want >= skip && want < skip + mine) {
-          want -= skip;
-          for (int v0 = w0; v0 < w1; v0 += 32) {
-            uint32_t hit = v0 + lane < w1 ? matches(v0 + lane) : 0u;
-            uint32_t incl = __popc(hit);
-            const uint32_t own = incl;
+      uint32_t hits[kGroups / 4], mine = 0u;
 #pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-              const uint32_t o = __shfl_up_sync(0xffffffffu, incl, off);
-              if (lane >= off) incl += o;
+      for (int q = 0; q < kGroups / 4; ++q) hits[q] = 0u;
+      // (-inf, which pads the pieces and the ends, is never looked for)
+      uint32_t ends = 0u;
+      if (warp == 0 || warp == kSampleWarps - 1) ends = __ballot_sync(0xffffffffu, (is(slice_edge(slice, warp != 0, lane)) & 0x8000u) != 0u);
+      uint4 x[2], next[2];
+      slice_pieces(slice, w0 + lane, 32, w1, x);
+#pragma unroll 1
+      for (int q = 0; w0 + q * 64 < w1; ++q) {
+        const int v = w0 + q * 64 + lane;
+        slice_pieces(slice, v + 64, 32, w1, next);
+        uint32_t h = 0u;
+        if (v < w1) h = matches(x[0]);
+        if (v + 32 < w1) h |= matches(x[1]) << 8;
+        x[0] = next[0];
+        x[1] = next[1];
+        mine += __popc(h);
+        h <<= 16 * (q & 1);
+#pragma unroll
+        for (int i = 0; i < kGroups / 4; ++i) hits[i] |= i == q >> 1 ? h : 0u;
+      }
+      mine = __reduce_add_sync(0xffffffffu, mine) + __popc(ends);
+      if (lane == 0) sm.found[warp] = mine;
+      __syncthreads();
+      const uint32_t skip = __reduce_add_sync(0xffffffffu, lane < warp ? sm.found[lane] : 0u);
+      if (want >= skip && want < skip + mine) {
+        want -= skip;
+        const uint32_t in_front = warp == 0 ? __popc(ends) : 0u, behind = warp == 0 ? 0u : __popc(ends);
+        const uint32_t in_pieces = mine - in_front - behind;
+        if (want < in_front || want >= in_front + in_pieces) {
+          const uint32_t nth = want < in_front ? want : want - in_pieces;
+          if (((ends >> lane) & 1u) != 0u && __popc(ends & ((1u << lane) - 1u)) == nth) commit((warp == 0 ? slice.lo : slice.last) + lane);
+        } else if (in_pieces == 1u) {
+#pragma unroll
+          for (int i = 0; i < kGroups / 4; ++i) {
+            const int bit = __ffs(hits[i]) - 1;
+            if (bit >= 0) commit(slice.first + (w0 + (i * 4 + (bit >> 3)) * 32 + lane) * 8 + (bit & 7));
+          }
+        } else {
+          want -= in_front;
+          uint32_t hit = 0u, left = want, at = 0u;
+          bool found = false;
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) {
+            const uint32_t h = (hits[g / 4] >> (8 * (g & 3))) & 0xFFu;
+            const uint32_t all = __reduce_add_sync(0xffffffffu, __popc(h));
+            if (!found && left < all) {
+              found = true;
+              hit = h;
+              at = g;
             }
-            if (want >= incl - own && want < incl) {
-              for (uint32_t j = incl - own; j < want; ++j) hit &= hit - 1u;
-              commit(slice.first + (v0 + lane) * 8 + __ffs(hit) - 1);
-            }
-            const uint32_t all = __shfl_sync(0xffffffffu, incl, 31);
-            if (want < all) break;
-            want -= all;
+            if (!found) left -= all;
+          }
+          uint32_t incl = __popc(hit);
+          const uint32_t own = incl;
+#pragma unroll
+          for (int off = 1; off < 32; off <<= 1) {
+            const uint32_t o = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += o;
+          }
+          if (left >= incl - own && left < incl) {
+            for (uint32_t j = incl - own; j < left; ++j) hit &= hit - 1u;
+            commit(slice.first + (w0 + static_cast<int>(at) * 32 + lane) * 8 + __ffs(hit) - 1);
           }
         }
       }
@@ -572,7 +700,7 @@ extern "C" int chr_nf4_sample_commit_batch(const void *logits, int64_t row_strid
                                            void *position, void *finished, int64_t eos,
                                            void *stream) {
   if (logits == nullptr || u == nullptr || next_token == nullptr) return kNull;
-  if (n < 1 || n > kSliceMax * kSampleMaxCluster || batch < 1 || batch > 65535 || row_stride < n) {
+  if (n < 1 || n > kSampleMaxVocab || batch < 1 || batch > 65535 || row_stride < n) {
     return kDims;
   }
   // CTAs per row: slices of 4096 tokens are enough, and more CTAs than SMs would only queue,

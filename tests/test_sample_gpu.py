@@ -146,3 +146,48 @@ def test_captured_draw_follows_its_inputs():
         graph.replay()
         got = nxt.tolist()
         assert got == [ref.sample(r, float(v))[0] for r, v in zip(x.double().cpu().numpy(), u.cpu())]
+
+
+def test_slices_longer_than_a_counter_counts():
+    """So many rows that two blocks share a row of 151936 tokens: one value may then occur more often in
+    a block's half than 16 bits count - all equal, a lowest-value mask, zeros of both signs, NaN."""
+    n, b = 151936, 90
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    logits = (2 * torch.randn((b, n), generator=gen, device="cuda")).to(BF16)
+    low = torch.finfo(BF16).min
+    for i in range(b):
+        row = logits[i]
+        kind = i % 9
+        if kind == 0:
+            row[:] = 1.5
+        elif kind == 1:  # all masked but a few
+            keep = row[::5000].clone()
+            row[:] = low
+            row[::5000] = keep
+        elif kind == 2:  # masked behind some place in the row
+            row[100 + 800 * i:] = low
+        elif kind == 3:
+            row[:] = 0.0
+            row[::2] = -0.0
+        elif kind == 4:
+            row[:] = 0.0
+            row[:33000] = -0.0
+            row[40000:140000] = -0.0
+            row[-5:] = 1.0
+        elif kind == 5:
+            row[: 70000 + i] = 3.0
+        elif kind == 6:  # two values that take most of a half each
+            row[:37000] = 2.0
+            row[37000:76000] = 2.015625
+            row[76000:] = -1.0
+        elif kind == 7:
+            row[7:] = -math.inf
+    u = torch.rand(b, generator=gen, device="cuda").tolist()
+    _check(logits, u)
+    _check(logits, u, temperature=[0.7] * b, top_k=[(0, 40, 40000, 75000, 120000)[i % 5] for i in range(b)],
+           top_p=[(1.0, 0.9, 0.5)[i % 3] for i in range(b)], min_p=[(0.0, 0.01)[i % 2] for i in range(b)])
+    nans = logits.clone()
+    nans[::2, 5:] = math.nan
+    nans[1::2, 80000:] = -math.nan
+    tokens, _ = _run(nans, u)
+    assert tokens == [5 if i % 2 == 0 else 80000 for i in range(b)]
