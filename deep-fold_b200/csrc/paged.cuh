@@ -149,7 +149,7 @@ struct Seg {
   int t0, t1, whole, slot;  // whole: no border cuts it; slot: which of the CTA's partials else
   int tok0, rem0;           // token and head (of the group) of row0
 };
-constexpr int kSegs = 32;   // segments described at a time
+constexpr int kSegs = 24;   // segments described at a time
 
 // A CTA's note for the join: whether its two partials hold anything, and, if a cut item
 // starts in its piece, that item: pieces first .. first + n - 1 hold a partial each (the

@@ -679,6 +679,7 @@ __device__ __forceinline__ void join_store(const PagedAttnArgs &a, const PagedCu
       make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
 }
 
+template <int kRows>
 __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const PagedAttnArgs a, int G) {
   __shared__ PagedCut cuts[kJoinWarps];
   __shared__ float4 fold[kJoinWarps][32];
@@ -724,15 +725,35 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Pag
     }
   };
   if (cut.n > 0 && cut.n <= kJoinFew) {
-    for (int r = blockIdx.y; r < cut.rows; r += gridDim.y) {
-      const float2 ml = ml_of(cut, lane, r);
-      const float mm = warp_max_xor(ml.x);
-      const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mm);
-      const float l = warp_sum_xor(w * ml.y);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int i = 0; i < cut.n; ++i) add(acc, __shfl_sync(0xffffffffu, w, i), part(cut, i, r));
-      join_store(a, cut, r, lane, acc, l);
+    // kRows rows at a time, so that their chains of loads run side by side
+    for (int r0 = blockIdx.y; r0 < cut.rows; r0 += kRows * gridDim.y) {
+      float w[kRows], l[kRows];
+      float4 acc[kRows];
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        const float2 ml = ml_of(cut, lane, min(r0 + k * static_cast<int>(gridDim.y), cut.rows - 1));
+        w[k] = ml.x;
+        l[k] = ml.y;
+      }
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        const float mm = warp_max_xor(w[k]);
+        w[k] = w[k] == -INFINITY ? 0.f : fast_exp2(w[k] - mm);
+        l[k] = warp_sum_xor(w[k] * l[k]);
+        acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll(4 / kRows)
+      for (int i = 0; i < cut.n; ++i) {
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+          add(acc[k], __shfl_sync(0xffffffffu, w[k], i), part(cut, i, min(r0 + k * static_cast<int>(gridDim.y), cut.rows - 1)));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        const int r = r0 + k * static_cast<int>(gridDim.y);
+        if (r < cut.rows) join_store(a, cut, r, lane, acc[k], l[k]);
+      }
     }
   }
   __syncthreads();
@@ -969,9 +990,13 @@ extern "C" int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, i
     }
   }
   if (e != cudaSuccess) return kLaunch;
-  e = launch_chain(attn_paged_join_kernel,
-                   dim3(static_cast<unsigned>((f.ctas + kJoinWarps - 1) / kJoinWarps), f.M == kWideM ? 64 : f.M),
-                   dim3(kJoinThreads), 0, st, a, f.ctas);
+  // a row per warp, or four where items have many
+  const unsigned eights = static_cast<unsigned>((f.ctas + kJoinWarps - 1) / kJoinWarps);
+  if (f.M == kWideM) {
+    e = launch_chain(attn_paged_join_kernel<4>, dim3(eights, kWideM / 4), dim3(kJoinThreads), 0, st, a, f.ctas);
+  } else {
+    e = launch_chain(attn_paged_join_kernel<1>, dim3(eights, f.M), dim3(kJoinThreads), 0, st, a, f.ctas);
+  }
   return e == cudaSuccess ? kOk : kLaunch;
 }
 

@@ -46,7 +46,8 @@ struct WideLayout {
   static constexpr int kV = 4 * kTileB;                     // two stages
   static constexpr int kBars = 6 * kTileB;
   static constexpr int kSegOff = kBars + 256;
-  static constexpr int kBytes = kSegOff + kSegs * static_cast<int>(sizeof(Seg)) + 1024;
+  static constexpr int kStage = (kSegOff + kSegs * static_cast<int>(sizeof(Seg)) + 127) / 128 * 128;
+  static constexpr int kBytes = kStage + 8 * 4096 + 1024;   // results on their way out, 4 KB a warp
 };
 
 struct WideBars {
@@ -416,6 +417,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         if (g.rows <= first_row) continue;
         if (!q_ahead) load_q(g);
         const bool mine = first_row + r < g.rows;
+        const bool idle = first_row + (warp & 3) * 32 >= g.rows;  // no row of this warp's is one of the item's
         const int token = token_of(a.p, g, min(first_row + r, g.rows - 1));
         // cache rows that all of this warp's rows see: the older ones and, causally, the new ones
         // up to its first row's token
@@ -438,6 +440,11 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           bar_wait(w, &w.s_full[tile][n_s & 1], (n_s >> 1) & 1, 10);
           __syncwarp();
           tc_fence_after();
+          if (idle) {  // what the product makes of these rows is not used
+            bar_arrive(&w.p_full[tile][n_s & 1]);
+            ++n_s;
+            continue;
+          }
           uint32_t s[64];
           tmem_ld32(s_buf, s);
           tmem_ld32(s_buf + 32, s + 32);
@@ -523,38 +530,61 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         if (!ok) break;
         tc_fence_after();
         if ((*reinterpret_cast<volatile uint32_t *>(&w.odd) >> si) & 1u) add_not_finite<HD>(a, g, token, mine, o_addr);
+        // A warp's 32 rows go out 128 bytes of each at a time, through shared memory (chunk c of row
+        // r at c ^ (r & 7)), so that a store covers four whole lines and not 32 pieces of 16 bytes.
         const bool whole = g.whole;
-        const int head = head_of(a.p, g, first_row + r, token);
         const float by = l_run != 0.f ? 1.f / l_run : 0.f;
         const PagedWs ws = ws_of(a, G);
-        const long long at = (static_cast<long long>(cta) * 2 + g.slot) * kWideM + first_row + r;
-        float *part = ws.o + at * HD;
-        __nv_bfloat16 *dst = a.out + (static_cast<long long>(g.r0 + token) * a.p.n_kv * a.p.n_rep + head) * HD;
-#pragma unroll
-        for (int c = 0; c < HD; c += 32) {
+        const int wrow = first_row + (warp & 3) * 32;  // the warp's first row
+        const long long at = (static_cast<long long>(cta) * 2 + g.slot) * kWideM + wrow;
+        const int to = (g.r0 + token) * (a.p.n_kv * a.p.n_rep) + head_of(a.p, g, first_row + r, token);
+        unsigned char *stage = sm + L::kStage + warp * 4096;
+        const int rr = lane >> 3, cc = lane & 7;
+#pragma unroll 1
+        for (int c = 0; c < HD; c += whole ? 64 : 32) {
           uint32_t o[32];
-          tmem_ld32(o_addr + c, o);
-          tmem_wait_ld();
-          if (mine && whole) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint32_t v[4];
+          for (int h = 0; h < 2; ++h) {
+            if (h == 1 && !whole) break;
+            tmem_ld32(o_addr + c + h * 32, o);
+            tmem_wait_ld();
+            if (whole) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(o[e + 2 * i]) * by,
-                                                               __uint_as_float(o[e + 2 * i + 1]) * by);
-                v[i] = *reinterpret_cast<const uint32_t *>(&y);
+              for (int e = 0; e < 4; ++e) {
+                uint32_t v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(o[e * 8 + 2 * i]) * by,
+                                                                 __uint_as_float(o[e * 8 + 2 * i + 1]) * by);
+                  v[i] = *reinterpret_cast<const uint32_t *>(&y);
+                }
+                *reinterpret_cast<uint4 *>(stage + lane * 128 + (((h * 4 + e) ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
               }
-              *reinterpret_cast<uint4 *>(dst + c + e) = make_uint4(v[0], v[1], v[2], v[3]);
-            }
-          } else if (mine) {
+            } else {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              *reinterpret_cast<uint4 *>(part + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              for (int e = 0; e < 8; ++e) {
+                *reinterpret_cast<uint4 *>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                    make_uint4(o[e * 4], o[e * 4 + 1], o[e * 4 + 2], o[e * 4 + 3]);
+              }
             }
           }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int row = i * 4 + rr;
+            const uint4 v = *reinterpret_cast<const uint4 *>(stage + row * 128 + ((cc ^ (row & 7)) << 4));
+            const long long dst = __shfl_sync(0xffffffffu, to, row);
+            if (wrow + row < g.rows) {
+              if (whole) {
+                *reinterpret_cast<uint4 *>(a.out + dst * HD + c + cc * 8) = v;
+              } else {
+                *reinterpret_cast<uint4 *>(ws.o + (at + row) * HD + c + cc * 4) = v;
+              }
+            }
+          }
+          __syncwarp();
         }
-        if (mine && !whole) ws.ml[at] = make_float2(m_run, l_run);
+        if (mine && !whole) ws.ml[at + lane] = make_float2(m_run, l_run);
         tc_fence_before();
       }
       n_kv += seg_tiles;
