@@ -159,7 +159,7 @@ struct PagedCut {
   int n, kvh, row0, rows, r0, pad;
 };
 
-// The walk along a CTA's piece. One warp starts it, its first thread goes on.
+// The walk along a CTA's piece: the place a warp is at.
 struct SegWalk {
   double x_hi, x_lo, start;  // the piece, and the item the walk is at
   PagedSeq s;
@@ -242,51 +242,90 @@ static __device__ __noinline__ bool walk_start(const PagedRows &p, SegWalk &w, i
   return true;
 }
 
-// The item at the walk's place as a segment of CTA c's piece, then on to the next one.
-__device__ __forceinline__ void walk_next(const PagedRows &p, SegWalk &w, int c, Seg &g, PagedCut &cut) {
-  const double cost = paged_cost(p, w.s, w.j), end = w.start + cost;
-  g.b = w.b;
-  g.kvh = w.kvh;
-  g.row0 = w.j * p.M;
-  g.tok0 = g.row0 / p.n_rep;
-  g.rem0 = g.row0 - g.tok0 * p.n_rep;
-  g.rows = min(p.M, w.s.R - g.row0);
-  g.r0 = w.s.r0;
-  g.base = w.s.base;
-  g.len = w.s.len;
-  g.kv_end = paged_kv_end(p, w.s, w.j);
-  const int nt = max((g.kv_end + p.tile - 1) / p.tile, 1);
-  g.t0 = paged_border(w.x_lo - w.start, cost, nt);
-  g.t1 = paged_border(w.x_hi - w.start, cost, nt);
-  g.whole = w.start >= w.x_lo && end <= w.x_hi;
-  g.slot = w.start < w.x_lo ? 0 : 1;
-  if (g.whole == 0) cut.live[g.slot] = g.t0 < g.t1;
-  if (g.slot == 1 && end > w.x_hi) {
-    // the last piece that starts before the item's end
-    int last = c + 1 + __float2int_rz(__fdividef(__double2float_rn(end - w.x_hi) * w.axis.G, __double2float_rn(w.axis.total)));
-    last = min(last, w.axis.G - 1);
+// Describes up to kSegs segments of CTA c's piece from the walk's place on, and moves it past
+// them: their number, with kMore set if there are others. Called by a whole warp: lane i takes
+// the i-th item from the walk's place, for which it steps over groups (a kv head of a sequence) of
+// J items each. One thread that went from item to item took 0.8 us for each.
+constexpr int kMore = 256;
+static __device__ __noinline__ int walk_fill(const PagedRows &p, SegWalk &w, PagedCut &cut, int c, Seg *segs) {
+  static_assert(kSegs < 32, "a lane looks at the first item of the next call");
+  const int lane = threadIdx.x & 31;
+  const double x_lo = w.x_lo, x_hi = w.x_hi;
+  PagedSeq s = w.s;
+  int b = w.b, kvh = w.kvh, j = w.j + lane;
+  bool in = w.start < x_hi;
+  double start = w.start - paged_before(p, s, w.j);  // of the group
 #pragma unroll 1
-    while (last > c + 1 && paged_piece(w.axis, last) >= end) --last;
-#pragma unroll 1
-    while (last + 1 < w.axis.G && paged_piece(w.axis, last + 1) < end) ++last;
-    cut.n = last - c + 1;
-    cut.kvh = g.kvh;
-    cut.row0 = g.row0;
-    cut.rows = g.rows;
-    cut.r0 = g.r0;
-  }
-  w.start = end;
-  if (++w.j == w.s.J) {
-    w.j = 0;
-    if (++w.kvh == p.n_kv) {
-      w.kvh = 0;
-#pragma unroll 1
-      while (++w.b < p.batch) {
-        w.s = paged_seq(p, w.b);
-        if (w.s.J > 0) break;
+  while (in && j >= s.J) {
+    const int groups = min(j / s.J, p.n_kv - kvh);
+    j -= groups * s.J;
+    start += groups * paged_before(p, s, s.J);
+    kvh += groups;
+    in = start < x_hi;
+    if (in && kvh == p.n_kv) {
+      kvh = 0;
+      s.J = 0;
+      while (in && s.J == 0) {
+        if (++b < p.batch) {
+          s = paged_seq(p, b);
+        } else {
+          in = false;
+        }
       }
     }
   }
+  __syncwarp();  // all have read the walk's place
+  start += paged_before(p, s, j);
+  in = in && start < x_hi;
+  Seg g;
+  bool some = false;
+  if (in && lane < kSegs) {
+    const double cost = paged_cost(p, s, j), end = start + cost;
+    g.b = b;
+    g.kvh = kvh;
+    g.row0 = j * p.M;
+    g.tok0 = g.row0 / p.n_rep;
+    g.rem0 = g.row0 - g.tok0 * p.n_rep;
+    g.rows = min(p.M, s.R - g.row0);
+    g.r0 = s.r0;
+    g.base = s.base;
+    g.len = s.len;
+    g.kv_end = paged_kv_end(p, s, j);
+    const int nt = max((g.kv_end + p.tile - 1) / p.tile, 1);
+    g.t0 = paged_border(x_lo - start, cost, nt);
+    g.t1 = paged_border(x_hi - start, cost, nt);
+    g.whole = start >= x_lo && end <= x_hi;
+    g.slot = start < x_lo ? 0 : 1;
+    some = g.t0 < g.t1;
+    if (g.whole == 0) cut.live[g.slot] = some;
+    if (g.slot == 1 && end > x_hi) {
+      // the last piece that starts before the item's end
+      const PagedAxis axis = w.axis;
+      int last = c + 1 + __float2int_rz(__fdividef(__double2float_rn(end - x_hi) * axis.G, __double2float_rn(axis.total)));
+      last = min(last, axis.G - 1);
+#pragma unroll 1
+      while (last > c + 1 && paged_piece(axis, last) >= end) --last;
+#pragma unroll 1
+      while (last + 1 < axis.G && paged_piece(axis, last + 1) < end) ++last;
+      cut.n = last - c + 1;
+      cut.kvh = g.kvh;
+      cut.row0 = g.row0;
+      cut.rows = g.rows;
+      cut.r0 = g.r0;
+    }
+  }
+  const unsigned described = __ballot_sync(0xffffffffu, some);
+  if (some) segs[__popc(described & ((1u << lane) - 1u))] = g;
+  const bool more = __shfl_sync(0xffffffffu, in, kSegs);
+  if (lane == kSegs) {
+    w.start = in ? start : x_hi;
+    w.s = s;
+    w.b = b;
+    w.kvh = kvh;
+    w.j = j;
+  }
+  __syncwarp();
+  return __popc(described) + (more ? kMore : 0);
 }
 
 }  // namespace chr

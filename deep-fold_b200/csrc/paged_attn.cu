@@ -68,41 +68,32 @@ __device__ __forceinline__ PagedWs ws_of(const PagedAttnArgs &a, int ctas) {
   return w;
 }
 
-// Describes up to kSegs segments of CTA c's piece from the walk's place on: their number.
-// One thread; `cut` is the CTA's note, complete once there are no more.
-__device__ __noinline__ int walk_fill(const PagedAttnArgs &a, SegWalk &at, PagedCut &note, int c, int ctas, Seg *segs) {
-  SegWalk w = at;  // in registers
-  PagedCut cut = note;
-  int n = 0;
-#pragma unroll 1
-  while (n < kSegs && w.start < w.x_hi && w.b < a.p.batch) {
-    Seg g;
-    walk_next(a.p, w, c, g, cut);
-    if (g.t0 < g.t1) segs[n++] = g;
-  }
-  at = w;
-  note = cut;
-  ws_of(a, ctas).cut[c] = cut;
-  return n;
-}
-
-// The walk of a CTA, in shared memory: thread 0's, and not worth the registers of a thread.
+// The walk of a CTA, in shared memory, as the first warp's it is not worth the registers of all.
 struct PagedWalk {
   SegWalk at;
   PagedCut note;
-  int n_segs;
+  int n_segs;  // described now, and kMore
 };
+// Describes the next segments; called by the first warp. The CTA's note is complete once there
+// are no more.
+__device__ __forceinline__ void walk_on(const PagedAttnArgs &a, PagedWalk &w, Seg *segs) {
+  const int lane = threadIdx.x & 31, ctas = gridDim.x, c = blockIdx.x;
+  const int n = walk_fill(a.p, w.at, w.note, c, segs);
+  if (lane == 0) w.n_segs = n;
+  if (lane < static_cast<int>(sizeof(PagedCut) / 4)) {
+    reinterpret_cast<int *>(ws_of(a, ctas).cut + c)[lane] = reinterpret_cast<const int *>(&w.note)[lane];
+  }
+}
 // The first segments; all threads of the block call it.
 __device__ __forceinline__ int walk_begin(const PagedAttnArgs &a, PagedWalk &w, Seg *segs) {
   if (threadIdx.x < 32) {
-    const int ctas = gridDim.x, c = blockIdx.x;
     if (threadIdx.x == 0) {
       w.at.start = w.at.x_hi = 0.0;
       w.note.live[0] = w.note.live[1] = w.note.n = 0;
     }
     __syncwarp();
-    walk_start(a.p, w.at, c, ctas);
-    if (threadIdx.x == 0) w.n_segs = walk_fill(a, w.at, w.note, c, ctas, segs);
+    walk_start(a.p, w.at, blockIdx.x, gridDim.x);
+    walk_on(a, w, segs);
   }
   __syncthreads();
   return w.n_segs;
@@ -261,7 +252,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   pdl_wait();
   pdl_trigger();
   zero_tail_rows<HD>(a, cta, G);
-  int n_now = walk_begin(a, walk, segs);
+  int n_word = walk_begin(a, walk, segs);
 
   const uint32_t ring = smem_u32(smem) + warp * S * L::kHalf;
   uint64_t *bar = bars + warp * S;
@@ -272,7 +263,8 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   int ahead = 0;        // ring slot requested next
   uint32_t phase = 0;   // parity of each slot's next completed copy
 
-  while (n_now != 0) {
+  while (n_word != 0) {
+    const int n_now = n_word & (kMore - 1);
     // A segment's queries (where they fit registers next to the running ones) and the pages of
     // its first 32 tiles (lane i: this warp's block of tile t0 + i) are fetched one segment early.
     uint32_t qn[KEEP ? KS : 1][2];
@@ -637,10 +629,10 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
     }
     __syncthreads();
-    if (n_now < kSegs) break;  // there are no more
-    if (tid == 0) walk.n_segs = walk_fill(a, walk.at, walk.note, cta, G, segs);
+    if ((n_word & kMore) == 0) break;
+    if (warp == 0) walk_on(a, walk, segs);
     __syncthreads();
-    n_now = walk.n_segs;
+    n_word = walk.n_segs;
     __syncthreads();
   }
   if (!ok) {

@@ -197,11 +197,14 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 
   // The roles part here for good, each with its own loop over the batches of segments.
   auto next_batch = [&](int n) {
-    if (n < kSegs) return 0;  // there are no more
+    if ((n & kMore) == 0) return 0;
     block_sync();
-    if (tid == 0) {
-      w.odd = 0;
-      walk.n_segs = w.fail != 0 ? 0 : walk_fill(a, walk.at, walk.note, cta, G, segs);
+    if (warp == 0) {
+      walk_on(a, walk, segs);
+      if (lane == 0) {
+        w.odd = 0;
+        if (w.fail != 0) walk.n_segs = 0;
+      }
     }
     block_sync();
     n = walk.n_segs;
@@ -209,7 +212,8 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     return n;
   };
   if (warp >= 8) {
-    for (int n_now = n_first; n_now != 0; n_now = next_batch(n_now)) {
+    for (int n_word = n_first; n_word != 0; n_word = next_batch(n_word)) {
+      const int n_now = n_word & (kMore - 1);
       bool ok = true;
       if (warp == 9) {
         // ---------------- copies ----------------
@@ -375,7 +379,8 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
     }
   } else {
-    for (int n_now = n_first; n_now != 0; n_now = next_batch(n_now)) {
+    for (int n_word = n_first; n_word != 0; n_word = next_batch(n_word)) {
+      const int n_now = n_word & (kMore - 1);
       bool ok = true;
       // ---------------- softmax: a thread per query row ----------------
       const int tile = warp >> 2;
