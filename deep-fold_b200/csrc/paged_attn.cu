@@ -124,6 +124,51 @@ __device__ __forceinline__ uint32_t seen32(const PagedAttnArgs &a, const Seg &g,
   return m;
 }
 
+// Which of the 16 cache rows k0 .. k0+15 pairs of tokens see, two to a word. The masks' loads are
+// all under way before the first is used.
+template <int N>
+__device__ __forceinline__ void seen16(const PagedAttnArgs &a, const Seg &g, const int (&token)[N][2], int k0,
+                                       uint32_t (&see)[N]) {
+  const int d0 = k0 - g.base, from = max(d0, 0), older = from - d0;  // new row of the first key, keys before it
+  const int end = g.kv_end - k0;
+  const uint32_t there = end >= 16 ? 0xFFFFu : (end <= 0 ? 0u : (1u << end) - 1u);
+  if (a.tree == nullptr) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      uint32_t m[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int up_to = token[n][e] + 1 - d0;
+        m[e] = (up_to >= 16 ? 0xFFFFu : (up_to <= 0 ? 0u : (1u << up_to) - 1u)) & there;
+      }
+      see[n] = m[0] | m[1] << 16;
+    }
+    return;
+  }
+  const int words = 2 * a.tree_words, i = from >> 5, sh = from & 31;  // masks as 32-bit words
+  uint32_t lo[N][2], hi[N][2];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t *w = reinterpret_cast<const uint32_t *>(a.tree) + static_cast<long long>(g.r0 + token[n][e]) * words;
+      lo[n][e] = hi[n][e] = 0u;
+      if (i < words) lo[n][e] = __ldg(w + i);
+      if (sh > 16 && i + 1 < words) hi[n][e] = __ldg(w + i + 1);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    uint32_t m[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t v = __funnelshift_r(lo[n][e], hi[n][e], sh);
+      m[e] = (older >= 16 ? 0xFFFFu : (v << older) | ((1u << older) - 1u)) & there;
+    }
+    see[n] = m[0] | m[1] << 16;
+  }
+}
+
 // A masked value enters the second product with weight zero, and 0 x NaN is NaN. So where some of
 // an item's rows do not see all of a tile's cache rows, infinities and NaN among their values are
 // taken out before the product, and added to the rows that do see them.
@@ -420,6 +465,11 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         const int row = t * kThinTile + warp * 16;
         bool live = (has_rows >> (n_used & 31)) & 1u;
         ++n_used;
+        // a block that reaches beyond what all rows see is masked key by key: key j of queries 2 t4
+        // and 2 t4 + 1 in bits j and 16 + j
+        const bool masked = row + 16 > seen_by_all;
+        uint32_t see[NQ];
+        if (masked) seen16<NQ>(a, g, token, row, see);
         const uint32_t k_blk = ring + slot * L::kHalf;
         live = arrived(live);
         slot = slot + 1 == S ? 0 : slot + 1;
@@ -453,8 +503,6 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         request_k();  // into the slot freed a half block ago
         uint32_t p[NQ][2];
         if (live) {
-          // a block that reaches beyond what all rows see is masked key by key
-          const bool masked = row + 16 > seen_by_all;
           bool over = false;
 #pragma unroll
           for (int n = 0; n < NQ; ++n) {
@@ -463,7 +511,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
               s[n][e] *= a.c2;
               s[n][e + 2] *= a.c2;
               if (masked) {
-                const uint32_t m = seen32(a, g, token[n][e], row) >> g8;
+                const uint32_t m = see[n] >> (16 * e + g8);
                 if ((m & 1u) == 0u) s[n][e] = -INFINITY;
                 if ((m & 256u) == 0u) s[n][e + 2] = -INFINITY;
               }
@@ -516,7 +564,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
           }
-          if (row + 16 > seen_by_all) {
+          if (masked) {
             uint32_t bad = 0;
 #pragma unroll
             for (int k = 0; k < (C + 1) / 2; ++k) {
@@ -589,6 +637,10 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       const PagedWs ws = ws_of(a, G);
       const long long part = (static_cast<long long>(cta) * 2 + g.slot) * M;
       constexpr int FC = L::kFoldCols;
+      constexpr int kPerRow = FC / 4;                     // threads of a row, four columns each
+      constexpr int kPass = kThinThreads / kPerRow;       // rows at a time
+      constexpr int kPasses = (M + kPass - 1) / kPass;
+      float weight[kPasses][kThinWarps], sum[kPasses], top[kPasses];
 #pragma unroll
       for (int f = 0; f < HD / FC; ++f) {
         if (f > 0) __syncthreads();  // the last columns have been read
@@ -603,27 +655,47 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           }
         }
         __syncthreads();
-        for (int i = tid; i < g.rows * FC; i += kThinThreads) {
-          const int r = i / FC, d = i - r * FC;
-          float mm = -INFINITY;
+        if (f == 0) {
 #pragma unroll
-          for (int w = 0; w < kThinWarps; ++w) mm = fmaxf(mm, ml[(w * M + r) * 2]);
-          const float m_use = mm == -INFINITY ? 0.f : mm;
-          float ll = 0.f, oo = 0.f;
+          for (int i = 0; i < kPasses; ++i) {
+            const int r = min(tid / kPerRow + i * kPass, M - 1);
+            float2 x[kThinWarps];
+            top[i] = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kThinWarps; ++w) {
+              x[w] = *reinterpret_cast<const float2 *>(ml + (w * M + r) * 2);
+              top[i] = fmaxf(top[i], x[w].x);
+            }
+            sum[i] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kThinWarps; ++w) {
+              weight[i][w] = fast_exp2(x[w].x - (top[i] == -INFINITY ? 0.f : top[i]));
+              sum[i] = fmaf(weight[i][w], x[w].y, sum[i]);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+          const int r = tid / kPerRow + i * kPass, col = (tid % kPerRow) * 4;
+          if (r >= g.rows) continue;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int w = 0; w < kThinWarps; ++w) {
-            const float e = fast_exp2(ml[(w * M + r) * 2] - m_use);
-            ll = fmaf(e, ml[(w * M + r) * 2 + 1], ll);
-            oo = fmaf(e, fold[(w * M + r) * L::kFoldPitch + d], oo);
+            const float4 v = *reinterpret_cast<const float4 *>(fold + (w * M + r) * L::kFoldPitch + col);
+            acc.x = fmaf(weight[i][w], v.x, acc.x);
+            acc.y = fmaf(weight[i][w], v.y, acc.y);
+            acc.z = fmaf(weight[i][w], v.z, acc.z);
+            acc.w = fmaf(weight[i][w], v.w, acc.w);
           }
-          const int col = f * FC + d;
           if (g.whole) {
             const int tok = token_of(a.p, g, r), head = head_of(a.p, g, r, tok);
-            a.out[(static_cast<long long>(g.r0 + tok) * a.p.n_kv * a.p.n_rep + head) * HD + col] =
-                __float2bfloat16(ll != 0.f ? oo / ll : 0.f);
+            const float by = sum[i] != 0.f ? 1.f / sum[i] : 0.f;
+            __nv_bfloat16 *dst =
+                a.out + (static_cast<long long>(g.r0 + tok) * a.p.n_kv * a.p.n_rep + head) * HD + f * FC + col;
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(mma_pack(acc.x * by, acc.y * by), mma_pack(acc.z * by, acc.w * by));
           } else {
-            ws.o[(part + r) * HD + col] = oo;
-            if (col == 0) ws.ml[part + r] = make_float2(mm, ll);
+            *reinterpret_cast<float4 *>(ws.o + (part + r) * HD + f * FC + col) = acc;
+            if (f == 0 && col == 0) ws.ml[part + r] = make_float2(top[i], sum[i]);
           }
         }
       }
