@@ -1002,8 +1002,9 @@ extern "C" int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, i
   if (rc != kOk) return rc;
   const int hd = a.c.hd;
   if (T < 1 || n_q < 1 || n_q % a.c.n_kv != 0 || !head_dim_ok(hd) ||
-      q_stride < static_cast<int64_t>(n_q) * hd || (tree != nullptr && tree_words < 1) ||
-      !std::isfinite(scale) || (q_start == nullptr && T != a.c.batch) || static_cast<int64_t>(T) * n_q > 0x3fffffffll || n_q > 65536) {
+      q_stride < static_cast<int64_t>(n_q) * hd || (tree != nullptr && (tree_words < 1 || tree_words > (1 << 24))) ||
+      !std::isfinite(scale) || (q_start == nullptr && T != a.c.batch) ||
+      static_cast<int64_t>(T) * n_q > 0x3fffffffll || n_q > 65536) {
     return kDims;
   }
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(ws, 16) || q_stride % 8 != 0 || !aligned(a.c.k, 16) ||

@@ -19,8 +19,8 @@ import torch
 
 from . import _lib
 from ._lib import ChrNf4Dev, ChrNf4Plan
-from .paged import (PAGED_HEAD_DIMS, SAMPLE_MAX_VOCAB, nf4_attn_paged, nf4_rope_kv_paged,
-                    nf4_sample_commit_batch)
+from .paged import (PAGED_HEAD_DIMS, SAMPLE_MAX_VOCAB, nf4_attn_paged, nf4_attn_paged_status,
+                    nf4_rope_kv_paged, nf4_sample_commit_batch)
 from .plan import LIVE_MAX_N, PLAN_MAX_N, k_pad as _k_pad
 
 __all__ = [
@@ -31,6 +31,7 @@ __all__ = [
     "SAMPLE_MAX_VOCAB",
     "nf4_attn",
     "nf4_attn_paged",
+    "nf4_attn_paged_status",
     "nf4_embed_rows",
     "nf4_gemm",
     "nf4_gemm_rows",

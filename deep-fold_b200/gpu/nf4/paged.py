@@ -20,12 +20,15 @@ import torch
 from . import _lib
 from ._lib import ChrNf4Pages
 
-__all__ = ["nf4_attn_paged", "nf4_rope_kv_paged", "nf4_sample_commit_batch", "PAGED_HEAD_DIMS", "SAMPLE_MAX_VOCAB"]
+__all__ = ["nf4_attn_paged", "nf4_attn_paged_status", "nf4_rope_kv_paged",
+           "nf4_sample_commit_batch", "PAGED_HEAD_DIMS", "SAMPLE_MAX_VOCAB"]
 
 #: head dims the attention covers
 PAGED_HEAD_DIMS = (16, 32, 64, 128)
 #: widest row the sampled pick takes
 SAMPLE_MAX_VOCAB = 524280
+
+_MOST = 0x7FFFFFFF  # counts are passed in 32 bits
 
 _BF16, _F32, _I32, _I64, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.int64, torch.uint8
 
@@ -86,6 +89,8 @@ def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor) ->
     t_row, t_el = table.stride()
     if n_pages < 1 or batch < 1 or max_pages < 1 or one < 1:
         _fail("the pools and page_table must not be empty")
+    if batch > _MOST or max_pages * page > _MOST:
+        _fail("page_table is too large")
     if t_el != 1 and max_pages > 1:
         _fail("page_table must have contiguous rows")
     if ks < one or vs < one or t_row < max_pages:  # strides of an axis of one mean nothing
@@ -115,6 +120,8 @@ def _head_rows(t: torch.Tensor, hd: int, index: int, what: str) -> tuple[int, in
     else:
         _fail(f"{what} must be [T, heads, hd] or [T, heads*hd]")
     step = stride[0]
+    if rows > _MOST:
+        _fail(f"{what} has too many rows")
     if step < row:
         if rows > 1:
             _fail(f"{what} rows overlap")
@@ -184,7 +191,7 @@ def nf4_rope_kv_paged(
         _fail("cos and sin must be [positions, rot/2] of one layout with contiguous rows")
     tab_rows, half = tab
     tab_stride = step[0]
-    if tab_rows < 1 or half < 1 or 2 * half > hd or (tab_rows > 1 and tab_stride < half):
+    if not 1 <= tab_rows <= _MOST or half < 1 or 2 * half > hd or (tab_rows > 1 and tab_stride < half):
         _fail(f"cos and sin must have 1..{hd // 2} columns and positions")
     n_q = qs = os_ = 0
     zero = 0
@@ -274,6 +281,11 @@ def _ws_floats(index: int, rows: int, batch: int, n_q: int, n_kv: int, hd: int) 
         return int(_lib.load().chr_nf4_attn_paged_ws(rows, batch, n_q, n_kv, hd))
 
 
+def nf4_attn_paged_status() -> int:
+    """Read and clear the paged attention's status word (0 = healthy). Synchronises."""
+    return int(_lib.load().chr_nf4_attn_paged_status())
+
+
 def nf4_sample_commit_batch(
     logits: torch.Tensor,
     u: torch.Tensor,
@@ -304,8 +316,8 @@ def nf4_sample_commit_batch(
         _fail("logits must be a CUDA bfloat16 [B, n]")
     b, n = logits.shape
     stride, el = logits.stride()
-    if b < 1 or not 1 <= n <= SAMPLE_MAX_VOCAB:
-        _fail(f"logits must have rows of 1..{SAMPLE_MAX_VOCAB} tokens")
+    if not 1 <= b <= 65535 or not 1 <= n <= SAMPLE_MAX_VOCAB:
+        _fail(f"logits must be 1..65535 rows of 1..{SAMPLE_MAX_VOCAB} tokens")
     if (el != 1 and n > 1) or (b > 1 and stride < n):
         _fail("logits must have contiguous rows that do not overlap")
     if u is None or next_token is None:

@@ -72,7 +72,7 @@ def test_append_refusals(kw, rc):
 
 @pytest.mark.parametrize("kw,rc", [(dict(q=None), -1), (dict(out=None), -1), (dict(kv=None), -1), (dict(ws=None), -1),
                                    (dict(T=0), -3), (dict(n_q=0), -3), (dict(n_q=7), -3), (dict(qs=511), -3),
-                                   (dict(tree=P), -3), (dict(scale=float("nan")), -3),
+                                   (dict(tree=P), -3), (dict(tree=P, words=(1 << 24) + 1), -3), (dict(scale=float("nan")), -3),
                                    (dict(scale=float("inf")), -3), (dict(q_start=None), -3), (dict(T=1 << 30), -3),
                                    (dict(q=ctypes.c_void_p(4098)), -5), (dict(out=ctypes.c_void_p(4104)), -5),
                                    (dict(qs=516), -5), (dict(ws=ctypes.c_void_p(4104)), -5), (dict(tree=ctypes.c_void_p(4100), words=1), -5), (dict(floats=0), -7)])
