@@ -225,79 +225,74 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
 
 using namespace chr;
 
-extern "C" int chr_nf4_rope_kv_paged(const chr_nf4_pages_t *pages, const void *q, int64_t q_stride,
-                                     const void *k, int64_t k_stride, const void *v,
-                                     int64_t v_stride, void *q_out, int64_t q_out_stride,
-                                     const void *cos, const void *sin, int64_t tab_stride,
-                                     int32_t tab_rows, int32_t tab_f32, int32_t rot,
-                                     int32_t interleaved, const void *seq, const void *slot,
-                                     const void *position, int32_t T, int32_t n_q,
-                                     int32_t zero_skipped, void *stream) {
-  if (pages == nullptr || k == nullptr || v == nullptr || cos == nullptr || sin == nullptr ||
-      slot == nullptr || (n_q > 0 && (q == nullptr || q_out == nullptr))) {
+extern "C" int chr_nf4_rope_kv_paged(const chr_nf4_rope_kv_paged_t *args, void *stream) {
+  if (args == nullptr) return kNull;
+  const chr_nf4_rope_kv_paged_t &r = *args;
+  if (r.k == nullptr || r.v == nullptr || r.cos == nullptr || r.sin == nullptr ||
+      r.slot == nullptr || (r.n_q > 0 && (r.q == nullptr || r.q_out == nullptr))) {
     return kNull;
   }
   AppendArgs a{};
-  const int rc = paged_cache(pages, a.c);
+  const int rc = paged_cache(&r.pages, a.c);
   if (rc != kOk) return rc;
-  const long long q_row = static_cast<long long>(n_q) * a.c.hd;
+  const long long q_row = static_cast<long long>(r.n_q) * a.c.hd;
   const long long kv_row = static_cast<long long>(a.c.n_kv) * a.c.hd;
-  if (T < 1 || n_q < 0 || rot < 2 || (rot & 1) != 0 || rot > a.c.hd || tab_rows < 1 ||
-      tab_stride < rot / 2 || q_stride < q_row || q_out_stride < q_row || k_stride < kv_row ||
-      v_stride < kv_row || (n_q + 2ll * a.c.n_kv) * a.c.hd > (1 << 24) ||
-      (seq == nullptr && T > a.c.batch)) {
+  if (r.T < 1 || r.T > (1 << 30) || r.n_q < 0 || r.rot < 2 || (r.rot & 1) != 0 || r.rot > a.c.hd || r.tab_rows < 1 ||
+      r.tab_stride < r.rot / 2 || r.q_stride < q_row || r.q_out_stride < q_row || r.k_stride < kv_row ||
+      r.v_stride < kv_row || (r.n_q + 2ll * a.c.n_kv) * a.c.hd > (1 << 24) ||
+      (r.seq == nullptr && r.T > a.c.batch)) {
     return kDims;
   }
-  a.q = static_cast<const __nv_bfloat16 *>(q);
-  a.k = static_cast<const __nv_bfloat16 *>(k);
-  a.v = static_cast<const __nv_bfloat16 *>(v);
-  a.q_out = static_cast<__nv_bfloat16 *>(q_out);
-  a.q_stride = q_stride;
-  a.k_stride = k_stride;
-  a.v_stride = v_stride;
-  a.q_out_stride = q_out_stride;
-  a.cos = cos;
-  a.sin = sin;
-  a.tab_stride = tab_stride;
-  a.seq = static_cast<const int32_t *>(seq);
-  a.slot = static_cast<const int64_t *>(slot);
-  a.position = static_cast<const int64_t *>(position);
-  a.T = T;
-  a.n_q = n_q;
-  a.rot = rot;
-  a.tab_rows = tab_rows;
-  a.zero_skipped = zero_skipped != 0;
+  a.q = static_cast<const __nv_bfloat16 *>(r.q);
+  a.k = static_cast<const __nv_bfloat16 *>(r.k);
+  a.v = static_cast<const __nv_bfloat16 *>(r.v);
+  a.q_out = static_cast<__nv_bfloat16 *>(r.q_out);
+  a.q_stride = r.q_stride;
+  a.k_stride = r.k_stride;
+  a.v_stride = r.v_stride;
+  a.q_out_stride = r.q_out_stride;
+  a.cos = r.cos;
+  a.sin = r.sin;
+  a.tab_stride = r.tab_stride;
+  a.seq = static_cast<const int32_t *>(r.seq);
+  a.slot = static_cast<const int64_t *>(r.slot);
+  a.position = static_cast<const int64_t *>(r.position);
+  a.T = r.T;
+  a.n_q = r.n_q;
+  a.rot = r.rot;
+  a.tab_rows = r.tab_rows;
+  a.zero_skipped = r.zero_skipped != 0;
   // 16-byte pieces where every head, its rotated part and every row are made of them
-  const int tab_align = tab_f32 != 0 ? 16 : 8;
+  const int tab_align = r.tab_f32 != 0 ? 16 : 8;
   const bool vec =
-      a.c.hd % 8 == 0 && (interleaved != 0 ? rot % 8 == 0 : rot % 16 == 0) &&
-      (n_q == 0 || (aligned(q, 16) && aligned(q_out, 16) && q_stride % 8 == 0 && q_out_stride % 8 == 0)) &&
-      aligned(k, 16) && aligned(v, 16) && k_stride % 8 == 0 && v_stride % 8 == 0 &&
+      a.c.hd % 8 == 0 && (r.interleaved != 0 ? r.rot % 8 == 0 : r.rot % 16 == 0) &&
+      (r.n_q == 0 || (aligned(r.q, 16) && aligned(r.q_out, 16) && r.q_stride % 8 == 0 && r.q_out_stride % 8 == 0)) &&
+      aligned(r.k, 16) && aligned(r.v, 16) && r.k_stride % 8 == 0 && r.v_stride % 8 == 0 &&
       aligned(a.c.k, 16) && aligned(a.c.v, 16) && a.c.k_page_stride % 8 == 0 &&
-      a.c.v_page_stride % 8 == 0 && aligned(cos, tab_align) && aligned(sin, tab_align) &&
-      tab_stride % 4 == 0;
-  const int half = rot / 2;
-  const int per_head = vec ? (interleaved != 0 ? rot / 8 : half / 8) + (a.c.hd - rot) / 8 : a.c.hd - half;
-  const int units = (n_q + a.c.n_kv) * per_head + a.c.n_kv * (vec ? a.c.hd / 8 : a.c.hd);
+      a.c.v_page_stride % 8 == 0 && aligned(r.cos, tab_align) && aligned(r.sin, tab_align) &&
+      r.tab_stride % 4 == 0;
+  const int half = r.rot / 2;
+  const int per_head = vec ? (r.interleaved != 0 ? r.rot / 8 : half / 8) + (a.c.hd - r.rot) / 8 : a.c.hd - half;
+  const int units = (r.n_q + a.c.n_kv) * per_head + a.c.n_kv * (vec ? a.c.hd / 8 : a.c.hd);
   // few rows: a row is spread over CTAs until the SMs have one each
   int split = (units + kAppendThreads - 1) / kAppendThreads;
-  const int most = (2 * sm_count() + T - 1) / T;
+  const int most = (2 * sm_count() + r.T - 1) / r.T;
   split = split > most ? most : split;
-  const dim3 grid(static_cast<unsigned>(T), static_cast<unsigned>(split < 1 ? 1 : split));
+  const dim3 grid(static_cast<unsigned>(r.T), static_cast<unsigned>(split < 1 ? 1 : split));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
 #define CHR_APPEND(V, I, F) e = launch_chain(append_kernel<V, I, F>, grid, dim3(kAppendThreads), 0, st, a)
   if (vec) {
-    if (interleaved != 0) {
-      if (tab_f32 != 0) CHR_APPEND(true, true, true); else CHR_APPEND(true, true, false);
+    if (r.interleaved != 0) {
+      if (r.tab_f32 != 0) CHR_APPEND(true, true, true); else CHR_APPEND(true, true, false);
     } else {
-      if (tab_f32 != 0) CHR_APPEND(true, false, true); else CHR_APPEND(true, false, false);
+      if (r.tab_f32 != 0) CHR_APPEND(true, false, true); else CHR_APPEND(true, false, false);
     }
   } else {
-    if (interleaved != 0) {
-      if (tab_f32 != 0) CHR_APPEND(false, true, true); else CHR_APPEND(false, true, false);
+    if (r.interleaved != 0) {
+      if (r.tab_f32 != 0) CHR_APPEND(false, true, true); else CHR_APPEND(false, true, false);
     } else {
-      if (tab_f32 != 0) CHR_APPEND(false, false, true); else CHR_APPEND(false, false, false);
+      if (r.tab_f32 != 0) CHR_APPEND(false, false, true); else CHR_APPEND(false, false, false);
     }
   }
 #undef CHR_APPEND

@@ -989,36 +989,34 @@ extern "C" int64_t chr_nf4_attn_paged_ws(int32_t T, int32_t batch, int32_t n_q, 
   return ws_floats_of(f.ctas, f.M, hd);
 }
 
-extern "C" int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, int64_t q_stride,
-                                  void *out, const void *q_start, const void *kv_len,
-                                  const void *tree, int32_t tree_words, int32_t T, int32_t n_q,
-                                  float scale, float *ws, int64_t ws_floats, int32_t zero_tail,
-                                  void *stream) {
-  if (pages == nullptr || q == nullptr || out == nullptr || kv_len == nullptr || ws == nullptr) {
+extern "C" int chr_nf4_attn_paged(const chr_nf4_attn_paged_t *args, void *stream) {
+  if (args == nullptr) return kNull;
+  const chr_nf4_attn_paged_t &r = *args;
+  if (r.q == nullptr || r.out == nullptr || r.kv_len == nullptr || r.ws == nullptr) {
     return kNull;
   }
   PagedAttnArgs a{};
-  const int rc = paged_cache(pages, a.c);
+  const int rc = paged_cache(&r.pages, a.c);
   if (rc != kOk) return rc;
   const int hd = a.c.hd;
-  if (T < 1 || n_q < 1 || n_q % a.c.n_kv != 0 || !head_dim_ok(hd) ||
-      q_stride < static_cast<int64_t>(n_q) * hd || (tree != nullptr && (tree_words < 1 || tree_words > (1 << 24))) ||
-      !std::isfinite(scale) || (q_start == nullptr && T != a.c.batch) ||
-      static_cast<int64_t>(T) * n_q > 0x3fffffffll || n_q > 65536) {
+  if (r.T < 1 || r.n_q < 1 || r.n_q % a.c.n_kv != 0 || !head_dim_ok(hd) ||
+      r.q_stride < static_cast<int64_t>(r.n_q) * hd || (r.tree != nullptr && (r.tree_words < 1 || r.tree_words > (1 << 24))) ||
+      !std::isfinite(r.scale) || (r.q_start == nullptr && r.T != a.c.batch) ||
+      static_cast<int64_t>(r.T) * r.n_q > 0x3fffffffll || r.n_q > 65536) {
     return kDims;
   }
-  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(ws, 16) || q_stride % 8 != 0 || !aligned(a.c.k, 16) ||
+  if (!aligned(r.q, 16) || !aligned(r.out, 16) || !aligned(r.ws, 16) || r.q_stride % 8 != 0 || !aligned(a.c.k, 16) ||
       !aligned(a.c.v, 16) || a.c.k_page_stride % 8 != 0 || a.c.v_page_stride % 8 != 0 ||
-      (tree != nullptr && !aligned(tree, 8))) {
+      (r.tree != nullptr && !aligned(r.tree, 8))) {
     return kAlign;
   }
-  const int n_rep = n_q / a.c.n_kv;
+  const int n_rep = r.n_q / a.c.n_kv;
   a.p.cap = static_cast<int>(static_cast<long long>(a.c.max_pages) << a.c.page_shift);
-  const AttnForm f = form_of(T, a.c.batch, n_rep, hd);
-  if (ws_floats < ws_floats_of(f.ctas, f.M, hd)) return kWorkspace;
-  a.p.q_start = static_cast<const int32_t *>(q_start);
-  a.p.kv_len = static_cast<const int32_t *>(kv_len);
-  a.p.T = T;
+  const AttnForm f = form_of(r.T, a.c.batch, n_rep, hd);
+  if (r.ws_floats < ws_floats_of(f.ctas, f.M, hd)) return kWorkspace;
+  a.p.q_start = static_cast<const int32_t *>(r.q_start);
+  a.p.kv_len = static_cast<const int32_t *>(r.kv_len);
+  a.p.T = r.T;
   a.p.batch = a.c.batch;
   a.p.n_kv = a.c.n_kv;
   a.p.n_rep = n_rep;
@@ -1026,25 +1024,25 @@ extern "C" int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, i
   a.p.tile = f.tile;
   a.p.extra = f.extra;
   a.p.per_rep = 1.f / static_cast<float>(n_rep);
-  a.p.causal = tree == nullptr;
+  a.p.causal = r.tree == nullptr;
   // places on the axis are whole numbers that binary64 holds exactly
-  const double items = static_cast<double>(T) * n_q / f.M + static_cast<double>(a.c.batch) * a.c.n_kv;
+  const double items = static_cast<double>(r.T) * r.n_q / f.M + static_cast<double>(a.c.batch) * a.c.n_kv;
   if (items * (static_cast<double>(a.p.cap) + f.extra) * n_rep > 4.0e15) return kDims;
-  a.q = static_cast<const __nv_bfloat16 *>(q);
-  a.out = static_cast<__nv_bfloat16 *>(out);
-  a.tree = static_cast<const unsigned long long *>(tree);
-  a.ws = ws;
-  a.q_stride = q_stride;
-  a.tree_words = tree_words;
-  a.zero_tail = zero_tail != 0;
-  a.c2 = scale * 1.4426950408889634f;
+  a.q = static_cast<const __nv_bfloat16 *>(r.q);
+  a.out = static_cast<__nv_bfloat16 *>(r.out);
+  a.tree = static_cast<const unsigned long long *>(r.tree);
+  a.ws = r.ws;
+  a.q_stride = r.q_stride;
+  a.tree_words = r.tree_words;
+  a.zero_tail = r.zero_tail != 0;
+  a.c2 = r.scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (f.M == kWideM) {
     // the sign of the scale goes into the product, so that the maximum of the products is
     // that of the scores; no scale at all would make a hidden row 0 x -inf
     a.c2 = std::max(std::fabs(a.c2), 1e-30f);
-    const int negate = scale < 0.f;
+    const int negate = r.scale < 0.f;
     e = hd == 64 ? launch_wide<64>(a, negate, f.ctas, st) : launch_wide<128>(a, negate, f.ctas, st);
   } else {
     switch (hd) {

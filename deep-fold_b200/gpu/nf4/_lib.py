@@ -67,8 +67,27 @@ class ChrNf4Pages(Structure):
                 ("max_pages", c_int32)]
 
 
+class ChrNf4RopeKvPaged(Structure):
+    """Mirror of ``chr_nf4_rope_kv_paged_t``; ``gpu.nf4.paged`` packs it with ``struct``."""
+
+    _fields_ = [("pages", ChrNf4Pages), ("q", c_void_p), ("q_stride", c_int64), ("k", c_void_p),
+                ("k_stride", c_int64), ("v", c_void_p), ("v_stride", c_int64), ("q_out", c_void_p),
+                ("q_out_stride", c_int64), ("cos", c_void_p), ("sin", c_void_p), ("tab_stride", c_int64),
+                ("seq", c_void_p), ("slot", c_void_p), ("position", c_void_p), ("tab_rows", c_int32),
+                ("tab_f32", c_int32), ("rot", c_int32), ("interleaved", c_int32), ("T", c_int32),
+                ("n_q", c_int32), ("zero_skipped", c_int32), ("reserved", c_int32)]
+
+
+class ChrNf4AttnPaged(Structure):
+    """Mirror of ``chr_nf4_attn_paged_t``; ``gpu.nf4.paged`` packs it with ``struct``."""
+
+    _fields_ = [("pages", ChrNf4Pages), ("q", c_void_p), ("q_stride", c_int64), ("out", c_void_p),
+                ("q_start", c_void_p), ("kv_len", c_void_p), ("tree", c_void_p), ("ws", c_void_p),
+                ("ws_floats", c_int64), ("tree_words", c_int32), ("T", c_int32), ("n_q", c_int32),
+                ("zero_tail", c_int32), ("scale", c_float), ("reserved", c_int32)]
+
+
 _DEV = POINTER(ChrNf4Dev)
-_PAGES = POINTER(ChrNf4Pages)
 
 # name -> (restype, argtypes); every symbol include/chr_gpu.h declares.
 SIGNATURES = {
@@ -162,18 +181,9 @@ SIGNATURES = {
         [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
          c_int32, c_float, c_void_p],
     ),
-    "chr_nf4_rope_kv_paged": (
-        c_int,
-        [_PAGES, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
-         c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_int32,
-         c_int32, c_int32, c_void_p],
-    ),
+    "chr_nf4_rope_kv_paged": (c_int, [c_void_p, c_void_p]),  # a packed ChrNf4RopeKvPaged
     "chr_nf4_attn_paged_ws": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
-    "chr_nf4_attn_paged": (
-        c_int,
-        [_PAGES, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,
-         c_float, c_void_p, c_int64, c_int32, c_void_p],
-    ),
+    "chr_nf4_attn_paged": (c_int, [c_void_p, c_void_p]),  # a packed ChrNf4AttnPaged
     "chr_nf4_attn_paged_status": (c_int, []),
     "chr_nf4_sample_commit_batch": (
         c_int,

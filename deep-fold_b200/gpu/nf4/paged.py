@@ -14,11 +14,11 @@ follows what the tensors hold at replay.
 from __future__ import annotations
 
 import functools
+import struct
 
 import torch
 
 from . import _lib
-from ._lib import ChrNf4Pages
 
 __all__ = ["nf4_attn_paged", "nf4_attn_paged_status", "nf4_rope_kv_paged",
            "nf4_sample_commit_batch", "PAGED_HEAD_DIMS", "SAMPLE_MAX_VOCAB"]
@@ -37,9 +37,13 @@ def _fail(msg: str):
     raise RuntimeError(msg)
 
 
-# A small call takes longer on the host than on the device, so the checks are kept lean: device
-# indices instead of device objects, each attribute read once, and the raw forms of "current
-# device" and "current stream", which take a tenth of what the public ones do.
+# A small call takes longer on the host than on the device, so the host side is kept lean: device
+# indices instead of device objects, each attribute read once, the raw forms of "current device"
+# and "current stream", which take a tenth of what the public ones do, and the arguments packed into
+# one record (ctypes takes 0.2 us to convert each argument of a call).
+_PAGES = "6q6i"  # ChrNf4Pages
+_ROPE = struct.Struct(_PAGES + "14q8i").pack  # ChrNf4RopeKvPaged
+_ATTN = struct.Struct(_PAGES + "8q4ifi").pack  # ChrNf4AttnPaged
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -66,8 +70,8 @@ def _vector(t: torch.Tensor | None, n: int, index: int, dtype: torch.dtype, what
     return t.data_ptr()
 
 
-def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor) -> tuple[ChrNf4Pages, int]:
-    """The C description of a paged cache, and its device's index."""
+def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor) -> tuple[tuple, int]:
+    """The fields of ``ChrNf4Pages`` for a paged cache, and its device's index."""
     index = k_pages.get_device()
     shape = k_pages.shape
     if index < 0 or k_pages.dtype is not _BF16 or len(shape) != 4:
@@ -97,8 +101,8 @@ def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor) ->
         if (n_pages > 1 and (ks < one or vs < one)) or (batch > 1 and t_row < max_pages):
             _fail("pages or table rows overlap")
         ks, vs, t_row = max(ks, one), max(vs, one), max(t_row, max_pages)
-    return ChrNf4Pages(k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), ks, vs, t_row, n_pages, page, n_kv,
-                       hd, batch, max_pages), index
+    return (k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), ks, vs, t_row, n_pages, page, n_kv, hd, batch,
+            max_pages), index
 
 
 def _head_rows(t: torch.Tensor, hd: int, index: int, what: str) -> tuple[int, int, int]:
@@ -172,15 +176,15 @@ def nf4_rope_kv_paged(
     skipped: no cache row is written, its row of a given ``q_out`` is left alone, of a new one
     zero. Rows of one call must take different cache rows. See ``chr_nf4_rope_kv_paged``."""
     pages, device = _pages(k_pages, v_pages, page_table)
-    hd = pages.hd
+    n_kv, hd, batch = pages[8:11]
     rows, heads, ks = _head_rows(k, hd, device, "k")
     v_rows, v_heads, vs = _head_rows(v, hd, device, "v")
-    if heads != pages.n_kv or v_heads != heads or v_rows != rows:
+    if heads != n_kv or v_heads != heads or v_rows != rows:
         _fail("k and v must have the pools' n_kv heads and the same rows")
     if rows < 1:
         _fail("k must have rows")
-    if seq is None and rows > pages.batch:
-        _fail(f"{rows} rows for {pages.batch} sequences need seq")
+    if seq is None and rows > batch:
+        _fail(f"{rows} rows for {batch} sequences need seq")
     f32 = cos.dtype is _F32
     tab = cos.shape
     step = cos.stride()
@@ -200,7 +204,7 @@ def nf4_rope_kv_paged(
         if q_rows != rows or n_q < 1:
             _fail("q must have k's rows")
         if q_out is None:
-            q_out = torch.empty((rows, n_q, hd), dtype=_BF16, device=q.device)
+            q_out = q.new_empty((rows, n_q, hd))
             os_, zero = n_q * hd, 1
         else:
             o_rows, o_heads, os_ = _head_rows(q_out, hd, device, "q_out")
@@ -211,11 +215,12 @@ def nf4_rope_kv_paged(
                 _fail("q_out must be q or not overlap it")
     elif q_out is not None:
         _fail("q_out goes with q")
-    _call("chr_nf4_rope_kv_paged", device, pages, 0 if q is None else q.data_ptr(), qs, k.data_ptr(), ks,
-          v.data_ptr(), vs, 0 if q is None else q_out.data_ptr(), os_, cos.data_ptr(), sin.data_ptr(),
-          max(tab_stride, half), tab_rows, 1 if f32 else 0, 2 * half, 1 if interleaved else 0,
-          _vector(seq, rows, device, _I32, "seq"), _vector(slot, rows, device, _I64, "slot"),
-          _vector(position, rows, device, _I64, "position"), rows, n_q, zero)
+    _call("chr_nf4_rope_kv_paged", device, _ROPE(
+        *pages, 0 if q is None else q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+        0 if q is None else q_out.data_ptr(), os_, cos.data_ptr(), sin.data_ptr(), max(tab_stride, half),
+        _vector(seq, rows, device, _I32, "seq"), _vector(slot, rows, device, _I64, "slot"),
+        _vector(position, rows, device, _I64, "position"), tab_rows, f32, 2 * half, bool(interleaved), rows, n_q,
+        zero, 0))
     return q_out
 
 
@@ -244,11 +249,11 @@ def nf4_attn_paged(
     A row that sees nothing gives zeros. Rows of ``q`` behind the last sequence's are left alone in
     a given ``out`` (which must not overlap ``q``), zero in a new one. See ``chr_nf4_attn_paged``."""
     pages, device = _pages(k_pages, v_pages, page_table)
-    hd, batch = pages.hd, pages.batch
+    n_kv, hd, batch = pages[8:11]
     if hd not in PAGED_HEAD_DIMS:
         _fail(f"head_dim must be one of {PAGED_HEAD_DIMS}, got {hd}")
     rows, n_q, qs = _head_rows(q, hd, device, "q")
-    if rows < 1 or n_q < 1 or n_q % pages.n_kv:
+    if rows < 1 or n_q < 1 or n_q % n_kv:
         _fail("q must have rows and a multiple of the pools' n_kv heads")
     words = 0
     if tree is not None:
@@ -260,18 +265,22 @@ def nf4_attn_paged(
         _fail(f"{rows} rows for {batch} sequences need q_start")
     zero = 0
     if out is None:
-        out = torch.empty((rows, n_q * hd), dtype=_BF16, device=q.device)
+        out = q.new_empty((rows, n_q * hd))
         zero = 1
     elif out.dtype is not _BF16 or out.get_device() != device or out.numel() != rows * n_q * hd \
             or not out.is_contiguous():
         _fail(f"out must be contiguous bfloat16 [{rows}, {n_q * hd}] on cuda:{device}")
     elif _overlap(out, rows, n_q * hd, n_q * hd, q, rows, qs, n_q * hd):
         _fail("out must not overlap q")
-    need = _ws_floats(device, rows, batch, n_q, pages.n_kv, hd)
-    ws = torch.empty(need, dtype=_F32, device=q.device)
-    _call("chr_nf4_attn_paged", device, pages, q.data_ptr(), qs, out.data_ptr(),
-          _vector(q_start, batch + 1, device, _I32, "q_start"), _vector(kv_len, batch, device, _I32, "kv_len"),
-          0 if tree is None else tree.data_ptr(), words, rows, n_q, float(scale), ws.data_ptr(), need, zero)
+    scale = float(scale)
+    if not -3e38 < scale < 3e38:
+        _fail(f"scale must be finite, got {scale}")
+    need = _ws_floats(device, rows, batch, n_q, n_kv, hd)
+    ws = q.new_empty(need, dtype=_F32)
+    _call("chr_nf4_attn_paged", device, _ATTN(
+        *pages, q.data_ptr(), qs, out.data_ptr(), _vector(q_start, batch + 1, device, _I32, "q_start"),
+        _vector(kv_len, batch, device, _I32, "kv_len"), 0 if tree is None else tree.data_ptr(), ws.data_ptr(), need,
+        words, rows, n_q, zero, scale, 0))
     return out
 
 

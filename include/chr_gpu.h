@@ -397,7 +397,9 @@ int chr_nf4_silu_mul(const void *gate_up, void *out, int32_t N, int32_t I, void 
  * v_page_stride elements apart, each page is contiguous. Cache row a of sequence s is row
  * a % page of page table[s * table_stride + a / page]. page: a power of two, 16..65536.
  * Page ids may repeat between sequences (shared prefixes); an id outside [0, n_pages)
- * is no page: rows on it are neither written nor attended. */
+ * is no page: rows on it are neither written nor attended. The two entries take their
+ * arguments as one host record each (a binding fills it in one go), read before they
+ * return. */
 typedef struct {
   void *k, *v;
   const int32_t *table;   /* device int32 [batch, max_pages] */
@@ -417,13 +419,22 @@ typedef struct {
  * row, and its q_out row is left alone (zero_skipped = 0) or zeroed. Two rows of one call
  * must not take the same cache row, and no row a page that another sequence shares.
  * Returns 0, -1 (null), -3 (dims), -6 (launch). Capturable. */
-int chr_nf4_rope_kv_paged(const chr_nf4_pages_t *pages, const void *q, int64_t q_stride,
-                          const void *k, int64_t k_stride, const void *v, int64_t v_stride,
-                          void *q_out, int64_t q_out_stride, const void *cos, const void *sin,
-                          int64_t tab_stride, int32_t tab_rows, int32_t tab_f32, int32_t rot,
-                          int32_t interleaved, const void *seq, const void *slot,
-                          const void *position, int32_t T, int32_t n_q, int32_t zero_skipped,
-                          void *stream);
+typedef struct {
+  chr_nf4_pages_t pages;
+  const void *q;
+  int64_t q_stride;
+  const void *k;
+  int64_t k_stride;
+  const void *v;
+  int64_t v_stride;
+  void *q_out;
+  int64_t q_out_stride;
+  const void *cos, *sin;
+  int64_t tab_stride;
+  const void *seq, *slot, *position;
+  int32_t tab_rows, tab_f32, rot, interleaved, T, n_q, zero_skipped, reserved;
+} chr_nf4_rope_kv_paged_t;
+int chr_nf4_rope_kv_paged(const chr_nf4_rope_kv_paged_t *args, void *stream);
 
 /* Attention of T new rows over the paged cache. Sequence b owns rows q_start[b] ..
  * q_start[b+1]-1 of q (device int32 [batch + 1], not decreasing, within 0..T; NULL: T ==
@@ -445,10 +456,19 @@ int chr_nf4_rope_kv_paged(const chr_nf4_pages_t *pages, const void *q, int64_t q
  * follows what they hold then.
  * Returns 0, -1 (null), -3 (dims), -5 (alignment: q, out, ws, pools 16 bytes), -6, -7. */
 int64_t chr_nf4_attn_paged_ws(int32_t T, int32_t batch, int32_t n_q, int32_t n_kv, int32_t hd);
-int chr_nf4_attn_paged(const chr_nf4_pages_t *pages, const void *q, int64_t q_stride, void *out,
-                       const void *q_start, const void *kv_len, const void *tree,
-                       int32_t tree_words, int32_t T, int32_t n_q, float scale, float *ws,
-                       int64_t ws_floats, int32_t zero_tail, void *stream);
+typedef struct {
+  chr_nf4_pages_t pages;
+  const void *q;
+  int64_t q_stride;
+  void *out;
+  const void *q_start, *kv_len, *tree;
+  float *ws;
+  int64_t ws_floats;
+  int32_t tree_words, T, n_q, zero_tail;
+  float scale;
+  int32_t reserved;
+} chr_nf4_attn_paged_t;
+int chr_nf4_attn_paged(const chr_nf4_attn_paged_t *args, void *stream);
 
 /* Reads and clears the paged attention's device status word (synchronises the device): 0 =
  * every bounded wait of its tensor-core form completed; else the number of the wait that

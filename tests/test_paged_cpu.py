@@ -26,18 +26,20 @@ def _pages(**kw):
 def _append(pages=None, **kw):
     from gpu.nf4 import _lib
 
-    d = dict(q=P, qs=512, k=P, ks=128, v=P, vs=128, qo=P, qos=512, cos=P, sin=P, ts=32, rows=64, f32=1, rot=64, inter=0,
-             seq=P, slot=P, pos=None, T=3, n_q=8, zero=0)
+    d = dict(q=4096, q_stride=512, k=4096, k_stride=128, v=4096, v_stride=128, q_out=4096, q_out_stride=512, cos=4096,
+             sin=4096, tab_stride=32, tab_rows=64, tab_f32=1, rot=64, seq=4096, slot=4096, T=3, n_q=8)
     d.update(kw)
-    return _lib.load().chr_nf4_rope_kv_paged(_pages() if pages is None else pages, *d.values(), None)
+    args = _lib.ChrNf4RopeKvPaged(pages=_pages() if pages is None else pages, **d)
+    return _lib.load().chr_nf4_rope_kv_paged(ctypes.byref(args), None)
 
 
 def _attn(pages=None, **kw):
     from gpu.nf4 import _lib
 
-    d = dict(q=P, qs=512, out=P, q_start=P, kv=P, tree=None, words=0, T=3, n_q=8, scale=0.1, ws=P, floats=1 << 30, zero=0)
+    d = dict(q=4096, q_stride=512, out=4096, q_start=4096, kv_len=4096, T=3, n_q=8, scale=0.1, ws=4096, ws_floats=1 << 30)
     d.update(kw)
-    return _lib.load().chr_nf4_attn_paged(_pages() if pages is None else pages, *d.values(), None)
+    args = _lib.ChrNf4AttnPaged(pages=_pages() if pages is None else pages, **d)
+    return _lib.load().chr_nf4_attn_paged(ctypes.byref(args), None)
 
 
 def _sample(**kw):
@@ -61,28 +63,30 @@ def test_null_pools_are_refused(null):
     assert _append(_pages(**{null: None})) == -1 and _attn(_pages(**{null: None})) == -1
 
 
-@pytest.mark.parametrize("kw,rc", [(dict(k=None), -1), (dict(v=None), -1), (dict(q=None), -1), (dict(qo=None), -1),
+@pytest.mark.parametrize("kw,rc", [(dict(k=None), -1), (dict(v=None), -1), (dict(q=None), -1), (dict(q_out=None), -1),
                                    (dict(cos=None), -1), (dict(sin=None), -1), (dict(slot=None), -1), (dict(T=0), -3),
                                    (dict(n_q=-1), -3), (dict(rot=0), -3), (dict(rot=3), -3), (dict(rot=66), -3),
-                                   (dict(ts=31), -3), (dict(rows=0), -3), (dict(qs=511), -3), (dict(ks=127), -3),
-                                   (dict(vs=127), -3), (dict(qos=511), -3), (dict(seq=None), -3)])
+                                   (dict(tab_stride=31), -3), (dict(tab_rows=0), -3), (dict(q_stride=511), -3),
+                                   (dict(k_stride=127), -3), (dict(v_stride=127), -3), (dict(q_out_stride=511), -3),
+                                   (dict(seq=None), -3)])
 def test_append_refusals(kw, rc):
     assert _append(**kw) == rc
 
 
-@pytest.mark.parametrize("kw,rc", [(dict(q=None), -1), (dict(out=None), -1), (dict(kv=None), -1), (dict(ws=None), -1),
-                                   (dict(T=0), -3), (dict(n_q=0), -3), (dict(n_q=7), -3), (dict(qs=511), -3),
-                                   (dict(tree=P), -3), (dict(tree=P, words=(1 << 24) + 1), -3), (dict(scale=float("nan")), -3),
-                                   (dict(scale=float("inf")), -3), (dict(q_start=None), -3), (dict(T=1 << 30), -3),
-                                   (dict(q=ctypes.c_void_p(4098)), -5), (dict(out=ctypes.c_void_p(4104)), -5),
-                                   (dict(qs=516), -5), (dict(ws=ctypes.c_void_p(4104)), -5), (dict(tree=ctypes.c_void_p(4100), words=1), -5), (dict(floats=0), -7)])
+@pytest.mark.parametrize("kw,rc", [(dict(q=None), -1), (dict(out=None), -1), (dict(kv_len=None), -1), (dict(ws=None), -1),
+                                   (dict(T=0), -3), (dict(n_q=0), -3), (dict(n_q=7), -3), (dict(q_stride=511), -3),
+                                   (dict(tree=4096), -3), (dict(tree=4096, tree_words=(1 << 24) + 1), -3),
+                                   (dict(scale=float("nan")), -3), (dict(scale=float("inf")), -3),
+                                   (dict(q_start=None), -3), (dict(T=1 << 30), -3), (dict(q=4098), -5), (dict(out=4104), -5),
+                                   (dict(q_stride=516), -5), (dict(ws=4104), -5), (dict(tree=4100, tree_words=1), -5),
+                                   (dict(ws_floats=0), -7)])
 def test_attention_refusals(kw, rc):
     assert _attn(**kw) == rc
 
 
 @pytest.mark.parametrize("hd", [8, 24, 48, 96, 256])
 def test_attention_refuses_other_head_dims(hd):
-    assert _attn(_pages(hd=hd, k_page_stride=1 << 16, v_page_stride=1 << 16), qs=1 << 14) == -3
+    assert _attn(_pages(hd=hd, k_page_stride=1 << 16, v_page_stride=1 << 16), q_stride=1 << 14) == -3
 
 
 def test_attention_refuses_unaligned_pools():
@@ -121,18 +125,35 @@ def test_python_ops_refuse_cpu_tensors():
         nf4_sample_commit_batch(torch.zeros((2, 8), dtype=torch.bfloat16), torch.zeros(2), torch.zeros(2, dtype=torch.int64))
 
 
-def test_pages_struct_matches_the_header(tmp_path):
-    from gpu.nf4._lib import ChrNf4Pages
+@pytest.mark.parametrize("mirror,name", [("ChrNf4Pages", "chr_nf4_pages_t"), ("ChrNf4RopeKvPaged", "chr_nf4_rope_kv_paged_t"),
+                                         ("ChrNf4AttnPaged", "chr_nf4_attn_paged_t")])
+def test_records_match_the_header(mirror, name, tmp_path):
+    from gpu.nf4 import _lib
 
+    cls = getattr(_lib, mirror)
     src = tmp_path / "sz.c"
-    fields = [f[0] for f in ChrNf4Pages._fields_]
+    fields = [f[0] for f in cls._fields_]
     src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "chr_gpu.h"\nint main(void) { printf("%zu", '
-                   "sizeof(chr_nf4_pages_t));\n"
-                   + "".join(f'printf(" %zu", offsetof(chr_nf4_pages_t, {f}));\n' for f in fields) + "return 0; }\n")
+                   f"sizeof({name}));\n"
+                   + "".join(f'printf(" %zu", offsetof({name}, {f}));\n' for f in fields) + "return 0; }\n")
     exe = tmp_path / "sz"
     subprocess.run(["gcc", f"-I{ROOT / 'include'}", str(src), "-o", str(exe)], check=True)
     got = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
-    assert got == [ctypes.sizeof(ChrNf4Pages)] + [getattr(ChrNf4Pages, f).offset for f in fields]
+    assert got == [ctypes.sizeof(cls)] + [getattr(cls, f).offset for f in fields]
+
+
+def test_records_are_packed_in_the_order_of_their_fields():
+    from gpu.nf4 import _lib
+    from gpu.nf4.paged import _ATTN, _ROPE
+
+    def flat(record):
+        for name, _ in record._fields_:
+            v = getattr(record, name)
+            yield from flat(v) if isinstance(v, ctypes.Structure) else [v]
+
+    for pack, cls, n in ((_ROPE, _lib.ChrNf4RopeKvPaged, 34), (_ATTN, _lib.ChrNf4AttnPaged, 26)):
+        values = list(range(1, n + 1))
+        assert list(flat(cls.from_buffer_copy(pack(*values)))) == values
 
 
 def test_overlap_of_row_views():
