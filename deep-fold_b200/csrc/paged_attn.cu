@@ -220,7 +220,10 @@ __device__ __forceinline__ void zero_tail_rows(const PagedAttnArgs &a, int cta, 
 // and P^T comes out of S^T by one 8x8 transpose per tile.
 // Bound by HBM: a 16-row block costs about 100 + 60 NQ warp instructions, and two CTAs of four
 // warps with 4 x 4 KB requested each keep 128 KB in flight per SM (the latency-bandwidth
-// product needs about 55).
+// product needs about 55). 64 sequences of 150 to 3500 rows, 40 / 8 heads of 128 (480 MB): 89 us,
+// 5.4 TB/s; three of 90,000 to 131,071 rows, 16 / 2 heads (384 MB): 75 us, 5.1 TB/s. A short call
+// is a chain of latencies: one sequence of 1792 rows takes 12 us, of which finding the work 3,
+// the first pages 2.3, the products 1, fold and join 4.
 // The subtracted maximum follows a row's scores with a slack of 8 (in log2): it is raised, and
 // the accumulator rescaled, only when a score exceeds it by more, so that a block without
 // such a score costs one vote instead of a maximum over its lanes; P stays below 2^8.
@@ -725,6 +728,8 @@ namespace {
 // Block (x, y) looks at the descriptions of eight CTAs, a warp each, and joins every
 // gridDim.y-th row from y on of the items they hold the start of: a warp per item where it lies
 // in a few pieces, the whole block, its pieces dealt over the warps, where it lies in many.
+// Bound by latency, three dependent reads of L2: 3 to 4 us. Four rows of a wide item at a time
+// in a warp, their reads side by side, take 4.5 us; one after the other 6.5.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr int kJoinFew = 16;
@@ -884,19 +889,28 @@ struct AttnForm {
 // The form of a call: from the head layout and the mean number of new rows per sequence,
 // which the host knows, never from the lengths, which it does not.
 AttnForm form_of(int T, int batch, int n_rep, int hd) {
+  // Items as low as the rows allow: 64 sequences of 5 rows per kv head take 88 us with items of 8,
+  // 117 with 32. Above 32 rows the wide form: 16 trees of 35 rows take 70 us with it, 130 with thin
+  // items of 32; of 255 rows 102 and 455. From 17 to 32 rows it is a draw: 20 rows, 16 sequences of
+  // 2100 to 6000 cache rows 67 wide and 75 thin, two such 31.6 and 28.4, 32 of 100 to 900
+  // 42 and 37.
   const long long rows = (static_cast<long long>(T) + batch - 1) / batch * n_rep;
   const int sms = std::min(sm_count(), kMaxCtas / 2);
   AttnForm f;
   if (rows > 32 && (hd == 64 || hd == 128)) {
     f.M = kWideM;
     f.tile = kWideTile;
-    f.extra = 2 * kWideTile;  // queries in, result out (measured)
-    f.ctas = sms;             // one resident CTA per SM
+    // Queries in, result out, in rows: 16 trees of 32 drafts take 96.8 us with 4 tiles, 97.1 with 2,
+    // 98.8 with 1.
+    f.extra = 4 * kWideTile;
+    f.ctas = sms;  // one resident CTA per SM
     return f;
   }
   f.M = rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
   f.tile = kThinTile;
-  f.extra = 3 * kThinTile;  // what starting and folding a segment takes, in rows (measured)
+  // What starting and folding a segment takes, in rows: 64 sequences take 87.7 us with 3 tiles,
+  // 95.6 with 1, 87.9 with 6.
+  f.extra = 3 * kThinTile;
   // Two resident CTAs per SM. (Three to eight, so that an SM that is served faster takes more
   // of them, cost more in starts than they balance: 64 sequences 110 us against 108.)
   f.ctas = 2 * sms;
