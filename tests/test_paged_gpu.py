@@ -400,3 +400,76 @@ def test_results_that_overlap_the_queries_are_refused():
     with pytest.raises(RuntimeError, match="overlap"):
         nf4_rope_kv_paged(q, k, k, kp, vp, table, cos, sin, _i64([19, 19]), q_out=y[1:])
     assert nf4_rope_kv_paged(q, k, k, kp, vp, table, cos, sin, _i64([19, 19]), q_out=q) is q
+
+
+def test_pages_shared_between_sequences():
+    """Two sequences with one prefix: the same page ids in both rows of the table."""
+    from gpu.nf4 import nf4_attn_paged
+
+    gen = _gen(11)
+    kp, vp, table = ref.make_cache(2, [100, 100], 16, 2, 64, gen)
+    table[1, :4] = table[0, :4]
+    for rows in ([1, 1], [40, 40]):
+        q = torch.randn((sum(rows), 8, 64), generator=gen, device="cuda").to(BF16)
+        _check(q, kp, vp, table, [100, 90], _starts(rows), 0.125)
+    q[40:] = q[:40]
+    table[1] = table[0]
+    out = nf4_attn_paged(q, kp, vp, table, _i32([100, 100]), 0.125, q_start=_i32([0, 40, 80]))
+    assert torch.equal(out[:40], out[40:])
+
+
+def test_two_calls_at_once_on_two_streams():
+    from gpu.nf4 import nf4_attn_paged, nf4_rope_kv_paged
+
+    gen = _gen(12)
+    jobs = []
+    for rows, kv in (([1] * 6, [900, 33, 1500, 7, 64, 2000]), ([60, 3], [700, 1200])):
+        kp, vp, table = ref.make_cache(len(kv), kv, 16, 2, 128, gen)
+        q = torch.randn((sum(rows), 10, 128), generator=gen, device="cuda").to(BF16)
+        args = (q, kp, vp, table, _i32(kv), 0.09)
+        jobs.append((args, dict(q_start=_i32(_starts(rows))), nf4_attn_paged(*args, q_start=_i32(_starts(rows)))))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    outs = [[], []]
+    for _ in range(10):
+        for i, (args, kw, _) in enumerate(jobs):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(nf4_attn_paged(*args, **kw))
+    torch.cuda.synchronize()
+    for i, (_, _, want) in enumerate(jobs):
+        assert all(torch.equal(o, want) for o in outs[i])
+    # the append, on a stream that fills its input first
+    kp, vp, table = ref.make_cache(1, [64], 16, 2, 64, gen)
+    cos, sin = _tables(64, 32, torch.float32, gen)
+    with torch.cuda.stream(streams[0]):
+        k = torch.ones((1 << 12, 1 << 12), device="cuda").matmul(torch.ones((1 << 12, 1 << 12), device="cuda"))[:1, :128].to(BF16)
+        nf4_rope_kv_paged(None, k, k, kp, vp, table, cos, sin, _i64([5]))
+    streams[0].synchronize()
+    assert (vp[int(table[0, 0]), 5] == 4096).all()
+
+
+def test_offsets_past_32_bits():
+    """Pools of more than 2^31 elements: the pages used lie at their ends."""
+    from gpu.nf4 import nf4_attn_paged, nf4_rope_kv_paged
+
+    page, n_kv, hd = 64, 2, 128
+    n_pages = (1 << 31) // (page * n_kv * hd) + 40
+    gen = _gen(13)
+    kp = torch.empty((n_pages, page, n_kv, hd), dtype=BF16, device="cuda")
+    vp = torch.empty((n_pages, page, n_kv, hd), dtype=BF16, device="cuda")
+    rows = [130, 70]
+    table = torch.arange(n_pages - 1, n_pages - 9, -1, dtype=torch.int32, device="cuda").view(2, 4).contiguous()
+    cos, sin = _tables(256, 64, torch.float32, gen)
+    k, v = (torch.randn((200, n_kv * hd), generator=gen, device="cuda").to(BF16) for _ in range(2))
+    seq = _i32([0] * 130 + [1] * 70)
+    slot = _i64(list(range(130)) + list(range(70)))
+    nf4_rope_kv_paged(None, k, v, kp, vp, table, cos, sin, slot, seq=seq)
+    small_k, small_v = kp[-8:].clone(), vp[-8:].clone()
+    small_table = table - (n_pages - 8)
+    for new in ([1, 1], [100, 60]):
+        q = torch.randn((sum(new), 8, hd), generator=gen, device="cuda").to(BF16)
+        kw = dict(q_start=_i32(_starts(new)))
+        got = nf4_attn_paged(q, kp, vp, table, _i32(rows), 0.09, **kw)
+        assert torch.equal(got, nf4_attn_paged(q, small_k, small_v, small_table, _i32(rows), 0.09, **kw))
+        want, mag = ref.attention(q, small_k, small_v, small_table, rows, _starts(new), 0.09)
+        assert ((got.view_as(q).double().cpu() - want).abs() <= ref.attention_tolerance(want, mag)).all()
