@@ -14,8 +14,8 @@
 // takes one 16-byte piece of a head (two for the half layout, whose partner elements
 // sit r/2 further on), so all of a row's accesses are 16 bytes wide; rows share nothing
 // but the table row, which stays in L1. q and k are requested before the chain
-// seq -> page table -> destination is resolved, so the two latencies overlap. 14,000 rows
-// of 64 + 2 x 8 heads of 128 (228 MB): 43.7 us, 5.2 TB/s; one row 2.1 us, 64 rows 2.5.
+// seq -> page table -> destination is resolved, so the two latencies overlap. 7,000 rows
+// of 48 + 2 x 8 heads of 128 (228 MB): 43.8 us, 5.2 TB/s; one row 2.1 us, 64 rows 2.6.
 
 #include "paged.cuh"
 
@@ -263,7 +263,7 @@ extern "C" int chr_nf4_rope_kv_paged(const chr_nf4_rope_kv_paged_t *args, void *
   a.rot = r.rot;
   a.tab_rows = r.tab_rows;
   a.zero_skipped = r.zero_skipped != 0;
-  // 16-byte pieces where every head, its rotated part and every row are made of them: 14,000 rows
+  // 16-byte pieces where every head, its rotated part and every row are made of them: 7,000 rows
   // take 44 us by pieces and 150 by elements, 64 rows 2.6 and 4.5
   const int tab_align = r.tab_f32 != 0 ? 16 : 8;
   const bool vec =
