@@ -49,9 +49,14 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+@functools.cache
+def _entry(name: str):
+    return getattr(_lib.load(), name)
+
+
 def _call(name: str, index: int, *args) -> None:
     """``name(*args, stream)`` with device ``index`` current, on its current stream."""
-    fn = getattr(_lib.load(), name)
+    fn = _entry(name)
     if index == _current_device():
         rc = fn(*args, _raw_stream(index))
     else:
@@ -133,15 +138,15 @@ def _head_rows(t: torch.Tensor, hd: int, index: int, what: str) -> tuple[int, in
     return rows, heads, step
 
 
-def _overlap(a: torch.Tensor, a_rows: int, a_step: int, a_row: int, b: torch.Tensor, b_rows: int, b_step: int,
-             b_row: int) -> bool:
-    """Whether two row views share memory; views of one stacked product (one step, side by side) do not."""
-    gap = (b.data_ptr() - a.data_ptr()) // 2
-    if gap >= (a_rows - 1) * a_step + a_row or -gap >= (b_rows - 1) * b_step + b_row:
+def _overlap(a: int, a_rows: int, a_step: int, b: int, b_rows: int, b_step: int, row: int) -> bool:
+    """Whether two views of rows of ``row`` bf16 elements, ``*_step`` apart, at addresses ``a`` and ``b``
+    share memory; views of one stacked product (one step, side by side) do not."""
+    gap = (b - a) // 2
+    if gap >= (a_rows - 1) * a_step + row or -gap >= (b_rows - 1) * b_step + row:
         return False
     if a_step == b_step:
         off = gap % a_step
-        return off < a_row or off + b_row > a_step
+        return off < row or off + row > a_step
     return True
 
 
@@ -197,28 +202,27 @@ def nf4_rope_kv_paged(
     tab_stride = step[0]
     if not 1 <= tab_rows <= _MOST or half < 1 or 2 * half > hd or (tab_rows > 1 and tab_stride < half):
         _fail(f"cos and sin must have 1..{hd // 2} columns and positions")
-    n_q = qs = os_ = 0
-    zero = 0
+    n_q = qs = os_ = zero = q_at = out_at = 0
     if q is not None:
         q_rows, n_q, qs = _head_rows(q, hd, device, "q")
+        q_at = q.data_ptr()
         if q_rows != rows or n_q < 1:
             _fail("q must have k's rows")
         if q_out is None:
             q_out = q.new_empty((rows, n_q, hd))
-            os_, zero = n_q * hd, 1
+            os_, zero, out_at = n_q * hd, 1, q_out.data_ptr()
         else:
             o_rows, o_heads, os_ = _head_rows(q_out, hd, device, "q_out")
             if o_rows != rows or o_heads != n_q:
                 _fail("q_out must have q's shape")
-            if (q_out.data_ptr() != q.data_ptr() or (os_ != qs and rows > 1)) and \
-                    _overlap(q_out, rows, os_, n_q * hd, q, rows, qs, n_q * hd):
+            out_at = q_out.data_ptr()
+            if (out_at != q_at or (os_ != qs and rows > 1)) and _overlap(out_at, rows, os_, q_at, rows, qs, n_q * hd):
                 _fail("q_out must be q or not overlap it")
     elif q_out is not None:
         _fail("q_out goes with q")
     _call("chr_nf4_rope_kv_paged", device, _ROPE(
-        *pages, 0 if q is None else q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
-        0 if q is None else q_out.data_ptr(), os_, cos.data_ptr(), sin.data_ptr(), max(tab_stride, half),
-        _vector(seq, rows, device, _I32, "seq"), _vector(slot, rows, device, _I64, "slot"),
+        *pages, q_at, qs, k.data_ptr(), ks, v.data_ptr(), vs, out_at, os_, cos.data_ptr(), sin.data_ptr(),
+        max(tab_stride, half), _vector(seq, rows, device, _I32, "seq"), _vector(slot, rows, device, _I64, "slot"),
         _vector(position, rows, device, _I64, "position"), tab_rows, f32, 2 * half, bool(interleaved), rows, n_q,
         zero, 0))
     return q_out
@@ -270,7 +274,7 @@ def nf4_attn_paged(
     elif out.dtype is not _BF16 or out.get_device() != device or out.numel() != rows * n_q * hd \
             or not out.is_contiguous():
         _fail(f"out must be contiguous bfloat16 [{rows}, {n_q * hd}] on cuda:{device}")
-    elif _overlap(out, rows, n_q * hd, n_q * hd, q, rows, qs, n_q * hd):
+    elif _overlap(out.data_ptr(), rows, n_q * hd, q.data_ptr(), rows, qs, n_q * hd):
         _fail("out must not overlap q")
     scale = float(scale)
     if not -3e38 < scale < 3e38:

@@ -159,12 +159,19 @@ def test_records_are_packed_in_the_order_of_their_fields():
 def test_overlap_of_row_views():
     from gpu.nf4.paged import _overlap
 
-    y = torch.empty((6, 100), dtype=torch.bfloat16)
-    q, k, late = y[:, :60], y[:, 60:], y[3:, :60]
-    flat = torch.empty(400, dtype=torch.bfloat16)
-    assert not _overlap(q, 6, 100, 60, k, 6, 100, 40) and not _overlap(k, 6, 100, 40, q, 6, 100, 60)
-    assert _overlap(q, 6, 100, 60, late, 3, 100, 60) and _overlap(late, 3, 100, 60, q, 6, 100, 60)
-    assert not _overlap(y[:3], 3, 100, 100, y[3:], 3, 100, 100)  # one behind the other
-    assert _overlap(q, 6, 100, 60, y[:, 30:90], 6, 100, 60) and _overlap(y[:, 30:90], 6, 100, 60, q, 6, 100, 60)
-    assert _overlap(flat, 4, 60, 60, flat, 3, 100, 60)           # steps that differ
-    assert not _overlap(flat[:200], 2, 100, 100, flat[200:], 2, 60, 60)
+    flat = torch.empty(1000, dtype=torch.bfloat16)
+
+    def both(a, b, row):
+        args = [(t.data_ptr(), t.shape[0], t.stride(0)) for t in (a, b)]
+        got = _overlap(*args[0], *args[1], row)
+        assert got == _overlap(*args[1], *args[0], row)
+        return got
+
+    y = flat[:600].view(6, 100)
+    q, k = y[:, :40], y[:, 60:]
+    assert not both(q, k, 40)                       # side by side in one product
+    assert both(q, y[3:, :40], 40) and both(q, q, 40)
+    assert both(q, y[:, 30:70], 40)
+    assert not both(y[:3], y[3:], 100)              # one behind the other
+    assert both(flat[:240].view(4, 60), flat[:300].view(3, 100)[:, :60], 60)  # steps that differ
+    assert not both(flat[:200].view(2, 100)[:, :60], flat[200:320].view(2, 60), 60)
