@@ -621,7 +621,9 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
       for (int q = 0; q < kGroups / 4; ++q) hits[q] = 0u;
       // (-inf, which pads the pieces and the ends, is never looked for)
       uint32_t ends = 0u;
-      if (warp == 0 || warp == kSampleWarps - 1) ends = __ballot_sync(0xffffffffu, (is(slice_edge(slice, warp != 0, lane)) & 0x8000u) != 0u);
+      if (warp == 0 || warp == kSampleWarps - 1) {
+        ends = __ballot_sync(0xffffffffu, (is(slice_edge(slice, warp != 0, lane)) & 0x8000u) != 0u);
+      }
       uint4 x[2], next[2];
       slice_pieces(slice, w0 + lane, 32, w1, x);
 #pragma unroll 1
