@@ -194,17 +194,18 @@ __device__ __forceinline__ void sts16(uint32_t addr, const uint4 &x) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
 }
 
-// Zeros for the rows behind the last sequence's, when the call asks for them.
+// Zeros for the rows that no sequence owns, in front of the first and behind the last, when the call asks for them.
 template <int HD>
-__device__ __forceinline__ void zero_tail_rows(const PagedAttnArgs &a, int cta, int G) {
+__device__ __forceinline__ void zero_unowned_rows(const PagedAttnArgs &a, int cta, int G) {
   if (a.zero_tail == 0 || a.p.q_start == nullptr) return;
-  const int last = min(max(__ldg(a.p.q_start + a.p.batch), 0), a.p.T);
+  const int first = min(max(__ldg(a.p.q_start), 0), a.p.T);
+  const int last = min(max(__ldg(a.p.q_start + a.p.batch), first), a.p.T);
   const long long width = static_cast<long long>(a.p.n_kv) * a.p.n_rep * HD / 8;
-  const long long n16 = (a.p.T - last) * width;
-  uint4 *dst = reinterpret_cast<uint4 *>(a.out) + last * width;
+  const long long front = first * width, owned = (last - first) * width, n16 = a.p.T * width - owned;
+  uint4 *dst = reinterpret_cast<uint4 *>(a.out);
   for (long long i = static_cast<long long>(cta) * blockDim.x + threadIdx.x; i < n16;
        i += static_cast<long long>(G) * blockDim.x) {
-    dst[i] = make_uint4(0, 0, 0, 0);
+    dst[i < front ? i : i + owned] = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -299,7 +300,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   }
   pdl_wait();
   pdl_trigger();
-  zero_tail_rows<HD>(a, cta, G);
+  zero_unowned_rows<HD>(a, cta, G);
   int n_word = walk_begin(a, walk, segs);
 
   const uint32_t ring = smem_u32(smem) + warp * S * L::kHalf;

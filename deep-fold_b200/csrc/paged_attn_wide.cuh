@@ -184,7 +184,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 
   pdl_wait();
   pdl_trigger();
-  zero_tail_rows<HD>(a, cta, G);
+  zero_unowned_rows<HD>(a, cta, G);
   const int n_first = walk_begin(a, walk, segs);
 
   const int shift = a.c.page_shift;

@@ -250,8 +250,9 @@ def nf4_attn_paged(
     One token per sequence is a decode step, a tree of drafted tokens is checked in one pass,
     and without ``tree`` many rows are a prompt chunk.
 
-    A row that sees nothing gives zeros. Rows of ``q`` behind the last sequence's are left alone in
-    a given ``out`` (which must not overlap ``q``), zero in a new one. See ``chr_nf4_attn_paged``."""
+    A row that sees nothing gives zeros. Rows of ``q`` that no sequence owns (in front of
+    ``q_start[0]``, from ``q_start[batch]`` on) are left alone in a given ``out`` (which must not
+    overlap ``q``), zero in a new one. See ``chr_nf4_attn_paged``."""
     pages, device = _pages(k_pages, v_pages, page_table)
     n_kv, hd, batch = pages[8:11]
     if hd not in PAGED_HEAD_DIMS:

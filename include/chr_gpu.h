@@ -445,11 +445,12 @@ int chr_nf4_rope_kv_paged(const chr_nf4_rope_kv_paged_t *args, void *stream);
  * the words is clear). GQA: n_q a multiple of n_kv, hd in {16, 32, 64, 128}.
  *   out[i, h, :] = softmax_t( scale * q[i, h, :] . k[t, h / n_rep] ) . v[t, h / n_rep]
  * q: bf16, rows q_stride elements apart (a multiple of 8), rotated already; out: bf16
- * [T, n_q * hd] contiguous. A row that sees nothing gives zeros; rows behind the last
- * sequence's are left alone (zero_tail = 0) or zeroed. FP32 scores, running softmax and
- * accumulation; probabilities are rounded to bf16 for the value product. Cache rows at
- * kv_len and beyond may hold anything; infinities and NaN in a new row reach the rows
- * that see it and no others. A cache row on a page outside the pool is seen by none.
+ * [T, n_q * hd] contiguous. A row that sees nothing gives zeros; rows that no sequence
+ * owns, in front of q_start[0] and from q_start[batch] on, are left alone (zero_tail = 0)
+ * or zeroed. FP32 scores, running softmax and accumulation; probabilities are rounded to
+ * bf16 for the value product. Cache rows at kv_len and beyond may hold anything;
+ * infinities and NaN in a new row reach the rows that see it and no others. A cache row on
+ * a page outside the pool is seen by none.
  * out must not overlap q. ws: chr_nf4_attn_paged_ws(...) floats, 16-byte aligned, no
  * initial contents needed; two calls that may overlap on the device need one each. Two
  * launches. Capturable: lengths, tables and masks are read on the device, and a replay
