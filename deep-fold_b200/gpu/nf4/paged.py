@@ -138,15 +138,15 @@ def _head_rows(t: torch.Tensor, hd: int, index: int, what: str) -> tuple[int, in
     return rows, heads, step
 
 
-def _overlap(a: int, a_rows: int, a_step: int, b: int, b_rows: int, b_step: int, row: int) -> bool:
-    """Whether two views of rows of ``row`` bf16 elements, ``*_step`` apart, at addresses ``a`` and ``b``
-    share memory; views of one stacked product (one step, side by side) do not."""
-    gap = (b - a) // 2
-    if gap >= (a_rows - 1) * a_step + row or -gap >= (b_rows - 1) * b_step + row:
+def _overlap(a: int, a_rows: int, a_step: int, b: int, b_rows: int, b_step: int, row: int, b_row: int = 0) -> bool:
+    """Whether two views of rows of ``row`` (``b``: ``b_row``, if given) bf16 elements, ``*_step`` apart, at
+    addresses ``a`` and ``b`` share memory; views of one stacked product (one step, side by side) do not."""
+    gap, b_row = (b - a) // 2, b_row or row
+    if gap >= (a_rows - 1) * a_step + row or -gap >= (b_rows - 1) * b_step + b_row:
         return False
     if a_step == b_step:
         off = gap % a_step
-        return off < row or off + row > a_step
+        return off < row or off + b_row > a_step
     return True
 
 
@@ -179,9 +179,11 @@ def nf4_rope_kv_paged(
 
     A row whose sequence, slot, position or page lies outside (``seq`` -1 marks padding) is
     skipped: no cache row is written, its row of a given ``q_out`` is left alone, of a new one
-    zero. Rows of one call must take different cache rows. See ``chr_nf4_rope_kv_paged``."""
+    zero. Rows of one call must take different cache rows. ``q_out`` must not overlap ``k`` or ``v``,
+    nor the pools each other; ``q``, ``k`` and ``v`` must not lie in cache rows the call writes. See
+    ``chr_nf4_rope_kv_paged``."""
     pages, device = _pages(k_pages, v_pages, page_table)
-    n_kv, hd, batch = pages[8:11]
+    kp, vp, _, kps, vps, _, n_pages, page, n_kv, hd, batch, _ = pages
     rows, heads, ks = _head_rows(k, hd, device, "k")
     v_rows, v_heads, vs = _head_rows(v, hd, device, "v")
     if heads != n_kv or v_heads != heads or v_rows != rows:
@@ -190,6 +192,11 @@ def nf4_rope_kv_paged(
         _fail("k must have rows")
     if seq is None and rows > batch:
         _fail(f"{rows} rows for {batch} sequences need seq")
+    k_at, v_at = k.data_ptr(), v.data_ptr()
+    gap = vp - kp
+    if gap < 2 * kps * n_pages and -gap < 2 * vps * n_pages \
+            and _overlap(kp, n_pages, kps, vp, n_pages, vps, page * n_kv * hd):
+        _fail("k_pages and v_pages must not overlap")
     f32 = cos.dtype is _F32
     tab = cos.shape
     step = cos.stride()
@@ -218,10 +225,18 @@ def nf4_rope_kv_paged(
             out_at = q_out.data_ptr()
             if (out_at != q_at or (os_ != qs and rows > 1)) and _overlap(out_at, rows, os_, q_at, rows, qs, n_q * hd):
                 _fail("q_out must be q or not overlap it")
+            # other threads read k and v in the same launch
+            far = 2 * os_ * rows
+            gap = k_at - out_at
+            if gap < far and -gap < 2 * ks * rows and _overlap(out_at, rows, os_, k_at, rows, ks, n_q * hd, n_kv * hd):
+                _fail("q_out must not overlap k")
+            gap = v_at - out_at
+            if gap < far and -gap < 2 * vs * rows and _overlap(out_at, rows, os_, v_at, rows, vs, n_q * hd, n_kv * hd):
+                _fail("q_out must not overlap v")
     elif q_out is not None:
         _fail("q_out goes with q")
     _call("chr_nf4_rope_kv_paged", device, _ROPE(
-        *pages, q_at, qs, k.data_ptr(), ks, v.data_ptr(), vs, out_at, os_, cos.data_ptr(), sin.data_ptr(),
+        *pages, q_at, qs, k_at, ks, v_at, vs, out_at, os_, cos.data_ptr(), sin.data_ptr(),
         max(tab_stride, half), _vector(seq, rows, device, _I32, "seq"), _vector(slot, rows, device, _I64, "slot"),
         _vector(position, rows, device, _I64, "position"), tab_rows, f32, 2 * half, bool(interleaved), rows, n_q,
         zero, 0))

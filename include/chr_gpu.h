@@ -418,6 +418,8 @@ typedef struct {
  * A row whose sequence, slot, position or page lies outside is skipped: it writes no cache
  * row, and its q_out row is left alone (zero_skipped = 0) or zeroed. Two rows of one call
  * must not take the same cache row, and no row a page that another sequence shares.
+ * What is written must be nobody's input: q_out overlaps neither k nor v (nor q, unless it is
+ * q), the pools do not overlap each other, and q, k and v lie outside the rows written.
  * Returns 0, -1 (null), -3 (dims), -6 (launch). Capturable. */
 typedef struct {
   chr_nf4_pages_t pages;

@@ -45,3 +45,65 @@ def test_rows_in_front_of_the_first_sequence(n_q, n_kv, hd, rows, kv, front, beh
     nf4_attn_paged(q, kp, vp, table, _i32(kv), 0.1, q_start=_i32(starts), out=out)
     assert (out[:front] == 3.0).all() and (out[starts[-1]:] == 3.0).all()
     assert torch.equal(out[front:starts[-1]], got[front:starts[-1]])
+
+
+def test_overlap_of_rows_of_two_widths():
+    """Against the elements themselves: never missed, and not reported where the steps are one."""
+    from gpu.nf4.paged import _overlap
+
+    flat = torch.empty(1000, dtype=BF16)
+
+    def elements(t):
+        first = (t.data_ptr() - flat.data_ptr()) // 2
+        return set((first + torch.arange(t.shape[0])[:, None] * t.stride(0) + torch.arange(t.shape[1])).flatten().tolist())
+
+    def both(a, b):
+        args = [(t.data_ptr(), t.shape[0], t.stride(0)) for t in (a, b)]
+        got = _overlap(*args[0], *args[1], a.shape[1], b.shape[1])
+        assert got == _overlap(*args[1], *args[0], b.shape[1], a.shape[1])
+        return got, bool(elements(a) & elements(b))
+
+    y = flat[:600].view(6, 100)
+    for a0, a1, b0, b1 in ((0, 60, 60, 80), (0, 60, 59, 80), (0, 60, 80, 100), (20, 30, 0, 20), (20, 30, 0, 21),
+                           (99, 100, 0, 99), (0, 100, 50, 51), (40, 60, 45, 46)):
+        got, shared = both(y[:, a0:a1], y[:, b0:b1])
+        assert got == shared
+        for a, b in ((y[:3, a0:a1], y[2:, b0:b1]), (y[:1, a0:a1], y[:, b0:b1]), (y[3:, a0:a1], y[:3, b0:b1])):
+            got, shared = both(a, b)
+            assert got or not shared
+    assert both(y[:1, :60], y[:1, 60:80]) == both(y[5:, 30:], y[5:, :30]) == (False, False)
+    assert both(flat[:240].view(4, 60), flat[240:300].view(3, 20)) == (False, False)
+    assert both(flat[:240].view(4, 60), flat[200:260].view(3, 20)) == (True, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 3])
+def test_append_refuses_to_write_over_its_inputs(rows):
+    from gpu.nf4 import nf4_rope_kv_paged
+
+    gen = _gen(2)
+    kp, vp, table = ref.make_cache(3, [20, 20, 20], 16, 2, 64, gen, poison=False)
+    y = torch.randn((rows, 12 * 64), generator=gen, device="cuda").to(BF16)
+    q, k, v = y.split([8 * 64, 2 * 64, 2 * 64], dim=1)
+    cos, sin = torch.ones((32, 32), device="cuda"), torch.zeros((32, 32), device="cuda")
+    slot = torch.full((rows,), 19, device="cuda")
+
+    def call(k, v, out, kp=kp, vp=vp):
+        return nf4_rope_kv_paged(q, k, v, kp, vp, table, cos, sin, slot, q_out=out)
+
+    other = torch.zeros_like(y)
+    out, inside = other[:, :512], other[:, 448:576]     # `inside` begins in the rows given for q_out
+    with pytest.raises(RuntimeError, match="q_out must not overlap k"):
+        call(inside, v, out)
+    with pytest.raises(RuntimeError, match="q_out must not overlap v"):
+        call(k, inside, out)
+    two = torch.zeros((kp.shape[0], 2) + tuple(kp.shape[1:]), dtype=BF16, device="cuda")
+    pages = two.view((-1,) + tuple(kp.shape[1:]))
+    for a, b in ((kp, kp), (two[:, 0], two[:, 0]), (pages[:6], pages[5:11])):
+        with pytest.raises(RuntimeError, match="k_pages and v_pages must not overlap"):
+            call(k, v, out, a, b)
+    assert not two.any() and not other.any()
+    assert call(k, v, q) is q                           # q, k and v side by side in one product
+    call(k, v, out, two[:, 0], two[:, 1])               # the pools' pages in turn
+    page = table[:rows, 1].long()
+    assert torch.equal(two[page, 1, 3].flatten(1), v) and torch.equal(two[page, 0, 3].flatten(1), k)
