@@ -35,6 +35,7 @@ struct PagedAttnArgs {
   long long q_stride;
   int tree_words, zero_tail;
   float c2;  // scale * log2(e)
+  uint32_t polls;  // limit of a wait
 };
 
 __device__ __forceinline__ void ldm_x4(uint32_t addr, uint32_t (&r)[4]) {
@@ -266,6 +267,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
+// What a warp had requested and not yet used when a wait of its ran out.
+struct ThinLate {
+  int slot, ahead;    // ring slots slot .. ahead-1, in order
+  uint32_t phase;     // parity of each slot's copy
+  uint32_t has_rows;  // by block: whether its halves were copied at all
+  uint32_t block;     // of the first, which is
+  int half;           // its K (0) or V (1) half
+};
+
 template <int HD, int NQ>
 __global__ void __launch_bounds__(kThinThreads, 2)
 attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -288,6 +298,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   at += L::kSegB;
   uint64_t *bars = reinterpret_cast<uint64_t *>(at);  // [warp][stage]
   __shared__ PagedWalk walk;
+  __shared__ ThinLate late[kThinWarps];
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g8 = lane >> 2, t4 = lane & 3;
@@ -387,11 +398,15 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         c_ids = c_s == c_early && c_t == segs[c_s].t0 ? n_ids : ids_of(c_s, c_t);
       }
     };
-    // The copy into the slot consumed next (bounded; nothing is in it when !live).
-    auto arrived = [&](bool live) {
+    // The copy into the slot consumed next, of half `half` of the block in use (bounded; nothing is in
+    // it when !live). Once a wait has run out, nothing is requested or computed any more.
+    auto arrived = [&](bool live, int half) {
       if (live && ok) {
-        ok = __all_sync(0xffffffffu, bar_poll(bar + slot, (phase >> slot) & 1u));
-        if (!ok && lane == 0) atomicExch(&g_attn_paged_status, 20);
+        ok = __all_sync(0xffffffffu, bar_poll(bar + slot, (phase >> slot) & 1u, a.polls));
+        if (!ok && lane == 0) {
+          atomicExch(&g_attn_paged_status, 20);
+          late[warp] = ThinLate{slot, ahead, phase, has_rows, n_used - 1, half};
+        }
         phase ^= 1u << slot;
       }
       return live && ok;
@@ -475,7 +490,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         uint32_t see[NQ];
         if (masked) seen16<NQ>(a, g, token, row, see);
         const uint32_t k_blk = ring + slot * L::kHalf;
-        live = arrived(live);
+        live = arrived(live, 0);
         slot = slot + 1 == S ? 0 : slot + 1;
         float s[NQ][4];  // keys g8 (0, 1) and g8 + 8 (2, 3) of the block, queries 2 t4, 2 t4 + 1
         if (live) {
@@ -556,7 +571,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           }
         }
         const uint32_t v_blk = ring + slot * L::kHalf;
-        live = arrived(live);
+        live = arrived(live, 1);
         slot = slot + 1 == S ? 0 : slot + 1;
         if (live) {
           if (row + 16 > g.kv_end) {
@@ -712,8 +727,13 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     __syncthreads();
   }
   if (!ok) {
-    // a copy is late: nothing leaves before the others in flight have landed
-    for (int i = 0; i < S; ++i) bar_poll(bar + i, (phase >> i) & 1u);
+    // nothing leaves before the copies in flight have landed, each within the full limit
+    __syncwarp();
+    const ThinLate l = late[warp];
+    int half = l.half;
+    for (int s = l.slot; s != l.ahead; s = s + 1 == S ? 0 : s + 1, ++half) {
+      if ((l.has_rows >> ((l.block + (half >> 1)) & 31)) & 1u) bar_poll(bar + s, (l.phase >> s) & 1u);
+    }
   }
 }
 
@@ -884,6 +904,12 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Pag
   }
 }
 
+// Limit of a wait, process-wide.
+uint32_t &attn_paged_polls() {
+  static uint32_t v = kPolls;
+  return v;
+}
+
 struct AttnForm {
   int M, tile, extra, ctas;
 };
@@ -997,6 +1023,10 @@ cudaError_t launch_wide(const PagedAttnArgs &a, int negate, int ctas, cudaStream
 
 using namespace chr;
 
+extern "C" void chr_nf4_set_attn_paged_polls(int32_t polls) {
+  attn_paged_polls() = polls < 0 ? kPolls : static_cast<uint32_t>(polls);
+}
+
 extern "C" int64_t chr_nf4_attn_paged_ws(int32_t T, int32_t batch, int32_t n_q, int32_t n_kv,
                                          int32_t hd) {
   if (T < 1 || batch < 1 || n_q < 1 || n_kv < 1 || n_q % n_kv != 0 || !head_dim_ok(hd)) return 0;
@@ -1051,6 +1081,7 @@ extern "C" int chr_nf4_attn_paged(const chr_nf4_attn_paged_t *args, void *stream
   a.tree_words = r.tree_words;
   a.zero_tail = r.zero_tail != 0;
   a.c2 = r.scale * 1.4426950408889634f;
+  a.polls = attn_paged_polls();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (f.M == kWideM) {

@@ -8,7 +8,7 @@
 
 namespace chr {
 
-constexpr uint32_t kPolls = 1u << 18;  // limit of every wait
+constexpr uint32_t kPolls = 1u << 18;  // limit of a wait
 
 __device__ __forceinline__ void bar_init(uint64_t *b, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");
@@ -20,9 +20,9 @@ __device__ __forceinline__ void bar_expect(uint64_t *b, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
 }
 // False when the phase of this parity did not complete within the poll limit.
-__device__ __forceinline__ bool bar_poll(uint64_t *b, uint32_t parity) {
+__device__ __forceinline__ bool bar_poll(uint64_t *b, uint32_t parity, uint32_t polls = kPolls) {
   const uint32_t addr = smem_u32(b);
-  for (uint32_t i = 0; i < kPolls; ++i) {
+  for (uint32_t i = 0; i < polls; ++i) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"

@@ -185,6 +185,7 @@ SIGNATURES = {
     "chr_nf4_attn_paged_ws": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
     "chr_nf4_attn_paged": (c_int, [c_void_p, c_void_p]),  # a packed ChrNf4AttnPaged
     "chr_nf4_attn_paged_status": (c_int, []),
+    "chr_nf4_set_attn_paged_polls": (None, [c_int32]),
     "chr_nf4_sample_commit_batch": (
         c_int,
         [c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

@@ -478,6 +478,11 @@ int chr_nf4_attn_paged(const chr_nf4_attn_paged_t *args, void *stream);
  * gave up, and the affected launch's output is undefined. */
 int chr_nf4_attn_paged_status(void);
 
+/* Poll limit of those waits (process-wide, taken at launch; negative restores 2^18). With a
+ * small one a test sees a wait run out; with 0 a wait that is not over gives up at once. The
+ * launch still ends by itself: what it has in flight is waited for with the full limit. */
+void chr_nf4_set_attn_paged_polls(int32_t polls);
+
 /* ---- Sampled pick ----------------------------------------------------------
  * One token per row drawn from its logits with the row's own settings and its own given
  * random number, then the commit of chr_nf4_pick_commit_batch (additive; the reference

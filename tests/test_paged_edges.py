@@ -107,3 +107,36 @@ def test_append_refuses_to_write_over_its_inputs(rows):
     call(k, v, out, two[:, 0], two[:, 1])               # the pools' pages in turn
     page = table[:rows, 1].long()
     assert torch.equal(two[page, 1, 3].flatten(1), v) and torch.equal(two[page, 0, 3].flatten(1), k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q,n_kv,hd,rows,kv", [
+    (8, 1, 128, [1, 1, 1], [2000, 5, 700]), (40, 8, 128, [1] * 64, [33 * i + 1 for i in range(64)]),
+    (4, 2, 64, [4, 0, 3], [900, 7, 64]), (4, 2, 16, [30, 1], [3000, 9]), (6, 1, 32, [3, 1], [40, 20000])])
+def test_thin_waits_that_run_out_say_so_and_the_call_ends(n_q, n_kv, hd, rows, kv):
+    """With no polls at all the first copy not there yet is given up: a status, a call that returns
+    with nothing in flight, and an ordinary call behind it as right as ever."""
+    from gpu.nf4 import _lib, nf4_attn_paged, nf4_attn_paged_status
+
+    lib = _lib.load()
+    gen = _gen(hd + len(rows))
+    kp, vp, table = ref.make_cache(len(kv), kv, 16, n_kv, hd, gen)
+    table[0, 1] = -1                                    # a block that is not copied among those that are
+    starts = [0]
+    for r in rows:
+        starts.append(starts[-1] + r)
+    q = torch.randn((starts[-1], n_q, hd), generator=gen, device="cuda").to(BF16)
+    call = lambda: nf4_attn_paged(q, kp, vp, table, _i32(kv), 0.1, q_start=_i32(starts))  # noqa: E731
+    want = call()
+    assert nf4_attn_paged_status() == 0
+    lib.chr_nf4_set_attn_paged_polls(0)
+    try:
+        for _ in range(3):
+            call()
+            assert nf4_attn_paged_status() == 20
+            assert nf4_attn_paged_status() == 0         # read and cleared
+    finally:
+        lib.chr_nf4_set_attn_paged_polls(-1)
+    for _ in range(3):
+        assert torch.equal(call(), want)
+    assert nf4_attn_paged_status() == 0
