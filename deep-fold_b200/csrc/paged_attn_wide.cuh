@@ -24,8 +24,8 @@
 // P is rounded to bf16 for the second product, its sum is not; everything else is FP32.
 //
 // Every wait is bounded; one that runs out leaves a code in a status word
-// (chr_nf4_attn_paged_status), the roles stop, copies in flight are waited for and the
-// tensor memory is freed.
+// (chr_nf4_attn_paged_status), the roles stop, copies and products in flight are waited for
+// (again with a limit) and the tensor memory is freed.
 
 #pragma once
 
@@ -58,16 +58,20 @@ struct WideBars {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], v_fixed[2];
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [query tile][buffer]
   uint64_t q_full[2];
+  uint64_t drained;  // all products issued are done
   uint32_t bad[4];  // pages of the last tiles that are none, a bit per page
   uint32_t odd;     // segments with infinities or NaN among the values not all rows see, a bit each
   uint32_t tmem;
   int fail;
 };
+static_assert(sizeof(WideBars) <= 256, "between the tiles and the segments");
+
+__device__ __forceinline__ bool given_up(const WideBars &w) { return *reinterpret_cast<const volatile int *>(&w.fail) != 0; }
 
 // Waits for a phase. One that does not complete within the poll limit sets `fail`, and from
 // then on every wait that would block returns at once: what is computed after that is
 // undefined, but stays in bounds and ends. False when a role has given up.
-__device__ __forceinline__ bool bar_wait(WideBars &w, uint64_t *b, uint32_t parity, int who) {
+__device__ __forceinline__ bool bar_wait(WideBars &w, uint64_t *b, uint32_t parity, int who, uint32_t polls) {
   const uint32_t addr = smem_u32(b);
   uint32_t done;
   asm volatile(
@@ -79,7 +83,7 @@ __device__ __forceinline__ bool bar_wait(WideBars &w, uint64_t *b, uint32_t pari
       : "memory");
   if (done) return true;
 #pragma unroll 1
-  for (uint32_t i = 0; i < kPolls; ++i) {
+  for (uint32_t i = 0; i < polls; ++i) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
@@ -88,7 +92,7 @@ __device__ __forceinline__ bool bar_wait(WideBars &w, uint64_t *b, uint32_t pari
         : "r"(addr), "r"(parity)
         : "memory");
     if (done) return true;
-    if (*reinterpret_cast<volatile int *>(&w.fail) != 0) return false;
+    if (given_up(w)) return false;
   }
   *reinterpret_cast<volatile int *>(&w.fail) = 1;
   atomicExch(&g_attn_paged_status, who);
@@ -167,6 +171,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       bar_init(&w.q_full[i], 128);
       bar_init(&w.v_fixed[i], 1);
     }
+    bar_init(&w.drained, 1);
     w.fail = 0;
     w.odd = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -238,7 +243,8 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             }
             const uint32_t bad = __ballot_sync(0xffffffffu, none);
             const int in_page = row & ((1 << shift) - 1);
-            if (n_kv >= 2) ok = bar_wait(w, &w.k_empty[st], ph ^ 1, 1);
+            // (after a give-up the products no longer wait for copies, and what they commit says nothing)
+            if (n_kv >= 2) ok = bar_wait(w, &w.k_empty[st], ph ^ 1, 1, a.polls) && !given_up(w);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             if (lane == 0) {
@@ -254,7 +260,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
                          g.kvh, in_page, id);
               }
             }
-            if (n_kv >= 2) ok = bar_wait(w, &w.v_empty[st], ph ^ 1, 2);
+            if (n_kv >= 2) ok = bar_wait(w, &w.v_empty[st], ph ^ 1, 2, a.polls) && !given_up(w);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             if (lane == 0) bar_expect(&w.v_full[st], L::kTileB);
@@ -271,7 +277,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             if (unseen < kWideTile) {
               // made fit for the second product: rows behind the last, which may hold anything,
               // become zeros, and so do infinities and NaN in those not all rows see
-              ok = __all_sync(0xffffffffu, bar_wait(w, &w.v_full[st], ph, 3));
+              ok = __all_sync(0xffffffffu, bar_wait(w, &w.v_full[st], ph, 3, a.polls));
               if (!ok) break;
               const int first = min(max(g.kv_end - t * kWideTile, 0), kWideTile);
               auto piece = [&](int i) {  // 16 bytes
@@ -293,11 +299,6 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             }
           }
         }
-        if (!ok) {
-          // a role gave up: the copies in flight land before the CTA leaves
-          for (uint32_t i = n_k >= 2 ? n_k - 2 : 0; i < n_k; ++i) bar_poll(&w.k_full[i & 1], (i >> 1) & 1);
-          for (uint32_t i = n_v >= 2 ? n_v - 2 : 0; i < n_v; ++i) bar_poll(&w.v_full[i & 1], (i >> 1) & 1);
-        }
       } else if (warp == 8) {
         // ---------------- products: a converged warp, one elected thread issues ----------------
         const uint32_t qk_desc = (1u << 4) | (1u << 7) | (1u << 10) | (negate ? 1u << 13 : 0u) |
@@ -308,7 +309,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         // operand descriptors of the first stage; a step of 16 elements adds a constant
         const uint64_t q_desc = tc_desc(base + L::kQ, 16), k_desc = tc_desc(base + L::kK, 16);
         const uint64_t v_desc = tc_desc(base + L::kV, L::kPiece);
-        auto wait = [&](uint64_t *bar, uint32_t parity, int who) { bar_wait(w, bar, parity, who); };
+        auto wait = [&](uint64_t *bar, uint32_t parity, int who) { bar_wait(w, bar, parity, who, a.polls); };
         // S = Q K^T for 64 rows of a K stage; `last`: the stage's last product
         auto qk = [&](int tile, int buf, int st, int half, bool last) {
           const uint64_t qd = q_desc + (tile * L::kTileB >> 4);
@@ -378,9 +379,21 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             ++n_s;
             if (two) ++n_s1;
           }
-          ok = __all_sync(0xffffffffu, *reinterpret_cast<volatile int *>(&w.fail) == 0);
+          ok = __all_sync(0xffffffffu, !given_up(w));
         }
       }
+    }
+    // Nothing is in flight when the CTA leaves, whichever role gave up, if one did: the last copies
+    // into each stage have landed, the products are done and their commits have arrived. Each wait
+    // has the full limit; without a give-up all but the last commits' are over.
+    if (warp == 9) {
+      for (uint32_t i = n_k >= 2 ? n_k - 2 : 0; i < n_k; ++i) bar_poll(&w.k_full[i & 1], (i >> 1) & 1);
+      for (uint32_t i = n_v >= 2 ? n_v - 2 : 0; i < n_v; ++i) bar_poll(&w.v_full[i & 1], (i >> 1) & 1);
+    } else {
+      __syncwarp();
+      if (elect_one()) tc_commit(&w.drained);
+      __syncwarp();
+      bar_poll(&w.drained, 0);
     }
   } else {
     for (int n_word = n_first; n_word != 0; n_word = next_batch(n_word)) {
@@ -446,7 +459,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             see[0] = seen32(a, g, token, key0);
             see[1] = seen32(a, g, token, key0 + 32);
           }
-          bar_wait(w, &w.s_full[tile][n_s & 1], (n_s >> 1) & 1, 10);
+          bar_wait(w, &w.s_full[tile][n_s & 1], (n_s >> 1) & 1, 10, a.polls);
           __syncwarp();
           tc_fence_after();
           if (idle) {  // what the product makes of these rows is not used
@@ -491,7 +504,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           if (__any_sync(0xffffffffu, turn_down)) {
             // The accumulator is this thread's once the last product into it is done. (That of
             // the step before, whose barrier this is too, ended before these scores began.)
-            bar_wait(w, &w.pv_done[tile][(n_s - 1) & 1], ((n_s - 1) >> 1) & 1, 11);
+            bar_wait(w, &w.pv_done[tile][(n_s - 1) & 1], ((n_s - 1) >> 1) & 1, 11, a.polls);
             __syncwarp();
             tc_fence_after();
             const float by = turn_down ? fast_exp2(m_run - m_new) : 1.f;
@@ -535,7 +548,7 @@ attn_paged_wide_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         q_ahead = si + 1 < n_now && segs[si + 1].rows > first_row;
         if (q_ahead) load_q(segs[si + 1]);
         // ---- the segment's result ----
-        ok = __all_sync(0xffffffffu, bar_wait(w, &w.pv_done[tile][(n_s - 1) & 1], ((n_s - 1) >> 1) & 1, 12));
+        ok = __all_sync(0xffffffffu, bar_wait(w, &w.pv_done[tile][(n_s - 1) & 1], ((n_s - 1) >> 1) & 1, 12, a.polls));
         if (!ok) break;
         tc_fence_after();
         if ((*reinterpret_cast<volatile uint32_t *>(&w.odd) >> si) & 1u) add_not_finite<HD>(a, g, token, mine, o_addr);

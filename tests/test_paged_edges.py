@@ -140,3 +140,41 @@ def test_thin_waits_that_run_out_say_so_and_the_call_ends(n_q, n_kv, hd, rows, k
     for _ in range(3):
         assert torch.equal(call(), want)
     assert nf4_attn_paged_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q,n_kv,hd,rows,kv,page,tree", [
+    (10, 2, 128, [52, 51], [700, 51], 64, False), (8, 2, 64, [103, 40, 0, 77], [1031, 400, 9, 77], 32, False),
+    (16, 1, 128, [300], [2300], 512, False), (40, 8, 128, [32] * 16, [2100 + 100 * i for i in range(16)], 64, True),
+    (5, 1, 64, [600, 30], [9000, 400], 16, False)])
+def test_wide_waits_that_run_out_say_so_and_the_call_ends(n_q, n_kv, hd, rows, kv, page, tree):
+    """As for the thin form: whichever role gives up first, copies and products in flight are waited for."""
+    from gpu.nf4 import _lib, nf4_attn_paged, nf4_attn_paged_status
+
+    lib = _lib.load()
+    gen = _gen(hd + len(rows))
+    kp, vp, table = ref.make_cache(len(kv), kv, page, n_kv, hd, gen)
+    starts = [0]
+    for r in rows:
+        starts.append(starts[-1] + r)
+    q = torch.randn((starts[-1], n_q, hd), generator=gen, device="cuda").to(BF16)
+    mask = None
+    if tree:
+        mask = torch.tensor([[(2 << i) - 1] for r in rows for i in range(r)], device="cuda")
+    call = lambda: nf4_attn_paged(q, kp, vp, table, _i32(kv), 0.1, q_start=_i32(starts), tree=mask)  # noqa: E731
+    want = call()
+    assert nf4_attn_paged_status() == 0
+    try:
+        for polls in (0, 0, 1):
+            lib.chr_nf4_set_attn_paged_polls(polls)
+            got = call()
+            status = nf4_attn_paged_status()
+            assert 1 <= status <= 12 if polls == 0 else 0 <= status <= 12
+            if status == 0:
+                assert torch.equal(got, want)           # every wait was over in time
+            assert nf4_attn_paged_status() == 0
+    finally:
+        lib.chr_nf4_set_attn_paged_polls(-1)
+    for _ in range(3):
+        assert torch.equal(call(), want)
+    assert nf4_attn_paged_status() == 0
