@@ -303,9 +303,11 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g8 = lane >> 2, t4 = lane & 3;
   const int G = gridDim.x, cta = blockIdx.x;
-  if (tid < kThinWarps * S) bar_init(bars + tid, 1);
+  if (tid < kThinWarps * S) {
+    bar_init(bars + tid, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");  // a thread's own initialisations
+  }
   if (tid == 0) {
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_map(&k_map);
     prefetch_map(&v_map);
   }
