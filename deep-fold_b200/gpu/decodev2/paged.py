@@ -14,8 +14,8 @@ from collections.abc import Sequence
 
 import torch
 
-from gpu.nf4 import (nf4_attn_paged, nf4_pick_commit_batch, nf4_rms_rows, nf4_rope_kv_paged, nf4_sample_commit_batch,
-                     nf4_silu_mul)
+from gpu.nf4 import (nf4_attn_paged, nf4_attn_paged_status, nf4_pick_commit_batch, nf4_rms_rows, nf4_rope_kv_paged,
+                     nf4_sample_commit_batch, nf4_silu_mul)
 
 from .batch import Sampling, _linear
 from .embed import gather_embed
@@ -97,7 +97,10 @@ class PagedKV:
 
 class PagedBatch:
     """``batch`` sequences over one paged cache. ``rope`` are keyword arguments of
-    ``rope_tables_scaled`` (scaling for contexts longer than the weights were trained on)."""
+    ``rope_tables_scaled`` (scaling for contexts longer than the weights were trained on).
+
+    ``append``, ``step`` and ``pick`` leave their results on the device; ``check``, which ``generate``
+    calls, tells whether the attention that made them ran to its end."""
 
     def __init__(self, weights: DeviceWeights, batch: int, n_pages: int, *, page: int = 64, max_seq: int | None = None,
                  rope: dict | None = None) -> None:
@@ -212,6 +215,14 @@ class PagedBatch:
         self.lens[seq] = at + len(path)
         kv.release(seq, self.lens[seq])
 
+    def check(self) -> None:
+        """Raises if a wait of the attention ran out since the last look: the tokens picked and the rows
+        appended since are then undefined. Synchronises."""
+        code = nf4_attn_paged_status(self.device)
+        if code:
+            raise RuntimeError(f"paged attention gave up a wait (status {code}): the results since the last check, "
+                               "cache rows included, are undefined")
+
     def reset(self) -> None:
         for b in range(self.batch):
             self.kv.release(b)
@@ -236,4 +247,5 @@ class PagedBatch:
         for i in range(int(n_new)):
             ui = None if u is None else u[i]
             trace[i].copy_(self.pick(logits, sampling, ui) if i == 0 else self.step(sampling, ui))
+        self.check()
         return trace.t().tolist()

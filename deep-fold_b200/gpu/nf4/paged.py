@@ -310,9 +310,12 @@ def _ws_floats(index: int, rows: int, batch: int, n_q: int, n_kv: int, hd: int) 
         return int(_lib.load().chr_nf4_attn_paged_ws(rows, batch, n_q, n_kv, hd))
 
 
-def nf4_attn_paged_status() -> int:
-    """Read and clear the paged attention's status word (0 = healthy). Synchronises."""
-    return int(_lib.load().chr_nf4_attn_paged_status())
+def nf4_attn_paged_status(device: torch.device | int | str | None = None) -> int:
+    """Read and clear the paged attention's status word on ``device`` (default: the current one):
+    0 = healthy, else a bounded wait of some launch since the last look ran out and that launch's
+    output is undefined. Synchronises the device."""
+    with torch.cuda.device(device):
+        return int(_lib.load().chr_nf4_attn_paged_status())
 
 
 def nf4_sample_commit_batch(

@@ -178,3 +178,33 @@ def test_wide_waits_that_run_out_say_so_and_the_call_ends(n_q, n_kv, hd, rows, k
     for _ in range(3):
         assert torch.equal(call(), want)
     assert nf4_attn_paged_status() == 0
+
+
+def _weights(spec, seed=0):
+    from gpu.decodev2 import DeviceWeights, build
+
+    return DeviceWeights.from_synth(build(spec, seed), "cuda", BF16)
+
+
+@pytest.mark.gpu
+def test_generation_raises_when_the_attention_gave_up():
+    """The tokens of a run in which a wait ran out are not handed out; the next run is as ever."""
+    from gpu.decodev2 import MEDIUM_LLAMA, PagedBatch
+    from gpu.nf4 import _lib, nf4_attn_paged_status
+
+    lib = _lib.load()
+    batch = PagedBatch(_weights(MEDIUM_LLAMA), 2, 8, page=16, max_seq=32)
+    prompts = [[1, 3, 5, 7], [9, 8]]
+    want = batch.generate(prompts, 5)
+    lib.chr_nf4_set_attn_paged_polls(0)
+    try:
+        with pytest.raises(RuntimeError, match="gave up a wait"):
+            batch.generate(prompts, 5)
+        batch.append([[1], [2]])
+        with pytest.raises(RuntimeError, match="gave up a wait"):
+            batch.check()
+    finally:
+        lib.chr_nf4_set_attn_paged_polls(-1)
+    batch.check()                                       # said once
+    assert batch.generate(prompts, 5) == want
+    assert nf4_attn_paged_status() == nf4_attn_paged_status(0) == nf4_attn_paged_status(batch.device) == 0
