@@ -114,6 +114,7 @@ class PagedBatch:
         self.cos, self.sin = rope_tables_scaled(self.kv.max_seq, spec.head_dim, spec.rope_theta, device=dev, **(rope or {}))
         #: cache rows of every sequence, and the token each one goes on with (not in the cache yet)
         self.lens = [0] * self.batch
+        self._open: list[list[int]] = [[] for _ in range(self.batch)]  # parents of the drafts behind ``lens``
         self.token = torch.zeros(self.batch, dtype=torch.int64, device=dev)
         self.prob = torch.ones(self.batch, dtype=torch.float32, device=dev)
         self._scratch = torch.zeros((self.batch, 16), dtype=torch.uint8, device=dev)
@@ -179,6 +180,9 @@ class PagedBatch:
                                tree=None if trees is None else tree_masks(trees, self.device), rows=last)
         if trees is None:
             self.lens = kv_len
+        for b, r in enumerate(rows):
+            if len(r):  # what was drafted there before is overwritten
+                self._open[b] = [] if trees is None else list(trees[b])
         return logits
 
     def pick(self, logits: torch.Tensor, sampling: Sampling | None = None, u: torch.Tensor | None = None) -> torch.Tensor:
@@ -196,14 +200,21 @@ class PagedBatch:
             self.kv.reserve(b, n + 1)
         logits = self._forward(self.token, self._i64(self.lens), self._i32([n + 1 for n in self.lens]))
         self.lens = [n + 1 for n in self.lens]
+        self._open = [[] for _ in range(self.batch)]
         return self.pick(logits, sampling, u)
 
     def accept(self, seq: int, path: Sequence[int], drafts: int) -> None:
-        """Keeps the drafts ``path`` (indices of the sequence's ``drafts`` last appended, each the
-        child of the one before) as the sequence's next rows and drops the others."""
-        at, kv = self.lens[seq], self.kv
-        if list(path) != sorted(set(path)) or (len(path) and not 0 <= path[0] <= path[-1] < drafts):
-            raise ValueError("a path rises through the drafts")
+        """Keeps the drafts ``path`` (indices of the sequence's ``drafts`` last appended, from a root down,
+        each the child of the one before) as the sequence's next rows and drops the others."""
+        at, kv, parents = self.lens[seq], self.kv, self._open[seq]
+        if drafts != len(parents):
+            raise ValueError(f"sequence {seq} has {len(parents)} drafts open, not {drafts}")
+        up = -1
+        for i in path:
+            if not 0 <= i < drafts or parents[i] != up:
+                raise ValueError(f"draft {i} is not {'a root' if up < 0 else f'a child of {up}'}")
+            up = i
+        self._open[seq] = []
         src = [at + i for i in path]
         dst = list(range(at, at + len(path)))
         if src != dst:
@@ -227,6 +238,7 @@ class PagedBatch:
         for b in range(self.batch):
             self.kv.release(b)
         self.lens = [0] * self.batch
+        self._open = [[] for _ in range(self.batch)]
 
     @torch.no_grad()
     def generate(self, prompts: Sequence[Sequence[int]], n_new: int, *, sampling: Sampling | None = None,

@@ -208,3 +208,38 @@ def test_generation_raises_when_the_attention_gave_up():
     batch.check()                                       # said once
     assert batch.generate(prompts, 5) == want
     assert nf4_attn_paged_status() == nf4_attn_paged_status(0) == nf4_attn_paged_status(batch.device) == 0
+
+
+@pytest.mark.gpu
+def test_accept_takes_a_chain_of_children_only():
+    """From a root down, each draft the child of the one before, of the drafts appended last."""
+    from gpu.decodev2 import MEDIUM_LLAMA, PagedBatch
+
+    batch = PagedBatch(_weights(MEDIUM_LLAMA), 2, 8, page=16, max_seq=32)
+    batch.append([[1, 3, 5, 7], [9, 8]])
+    tree = [[-1, 0, 0, 1, 2, -1], [-1, -1]]
+    batch.append([[4, 5, 6, 7, 8, 9], [3, 2]], trees=tree)
+    before = [list(batch.lens), [list(o) for o in batch.kv.owned]]
+    for path in ([1], [0, 3], [0, 1, 2], [0, 1, 4], [1, 3], [0, 5], [6], [-1], [0, 0], [3, 1]):
+        with pytest.raises(ValueError):
+            batch.accept(0, path, 6)
+    for drafts in (5, 7, 0):
+        with pytest.raises(ValueError):
+            batch.accept(0, [0, 1], drafts)
+    assert [list(batch.lens), [list(o) for o in batch.kv.owned]] == before
+    batch.accept(0, [0, 2, 4], 6)
+    with pytest.raises(ValueError):          # its drafts are settled
+        batch.accept(0, [0, 2, 4], 6)
+    batch.accept(1, [1], 2)
+    assert batch.lens == [7, 3]
+    batch.append([[4], [5, 6]], trees=[[-1], [-1, 0]])
+    batch.accept(1, [], 2)                   # none kept
+    assert batch.lens == [7, 3]
+    batch.append([[2], [2]])                 # takes the rows of sequence 0's open draft
+    with pytest.raises(ValueError):
+        batch.accept(0, [0], 1)
+    batch.append([[4], []], trees=[[-1], []])
+    batch.token.fill_(1)
+    batch.step()                             # so does a step
+    with pytest.raises(ValueError):
+        batch.accept(0, [0], 1)
