@@ -76,13 +76,22 @@ class PagedKV:
 
     def reserve(self, seq: int, rows: int) -> None:
         """Sees to it that sequence ``seq`` has pages for ``rows`` cache rows."""
-        if rows > self.max_seq:
-            raise ValueError(f"{rows} rows exceed max_seq={self.max_seq}")
-        own = self.owned[seq]
-        have, need = len(own), -(-rows // self.page)
-        if need - have > len(self._free):
-            raise RuntimeError(f"out of cache pages: sequence {seq} needs {need - have}, {len(self._free)} are free")
-        if need > have:
+        self.reserve_all({seq: rows})
+
+    def reserve_all(self, rows: dict[int, int]) -> None:
+        """``reserve`` for several sequences (rows by sequence): all of them, or none if it raises."""
+        more = {}
+        for seq, n in rows.items():
+            if n > self.max_seq:
+                raise ValueError(f"{n} rows exceed max_seq={self.max_seq}")
+            have, need = len(self.owned[seq]), -(-n // self.page)
+            if need > have:
+                more[seq] = have, need
+        lack = sum(need - have for have, need in more.values())
+        if lack > len(self._free):
+            raise RuntimeError(f"out of cache pages: sequences {list(more)} need {lack}, {len(self._free)} are free")
+        for seq, (have, need) in more.items():
+            own = self.owned[seq]
             own.extend(self._free.pop() for _ in range(need - have))
             self.table[seq, have:need] = torch.tensor(own[have:need], dtype=torch.int32)
 
@@ -159,21 +168,23 @@ class PagedBatch:
         """One pass over new rows of every sequence (none for some): prompt chunks, or with ``trees``
         (a parent list per sequence) drafted tokens. Their keys and values go to the cache rows
         behind ``lens``, which it leaves alone for drafts and advances otherwise. Returns the
-        logits of all rows, in order, or of each sequence's last row (``last_only``)."""
+        logits of all rows, in order, or of each sequence's last row (``last_only``). A call that
+        raises has taken no pages."""
         if len(rows) != self.batch or not any(len(r) for r in rows):
             raise ValueError(f"need rows for {self.batch} sequences")
         if trees is not None and [len(t) for t in trees] != [len(r) for r in rows]:
             raise ValueError("a tree has one parent per draft")
+        if any(len(r) and not 0 <= min(r) <= max(r) < self.spec.vocab for r in rows):
+            raise ValueError(f"a token outside 0..{self.spec.vocab - 1}")
         start, seq, slot, position, kv_len = [0], [], [], [], []
         for b, r in enumerate(rows):
             n, at = len(r), self.lens[b]
-            if n:
-                self.kv.reserve(b, at + n)
             start.append(start[-1] + n)
             seq += [b] * n
             slot += range(at, at + n)
             position += range(at, at + n) if trees is None else [at + d for d in tree_depths(trees[b])]
             kv_len.append(at + n)
+        self.kv.reserve_all({b: kv_len[b] for b, r in enumerate(rows) if len(r)})
         last = self._i64([e - 1 for e, r in zip(start[1:], rows) if len(r)]) if last_only else None
         logits = self._forward(self._i64([t for r in rows for t in r]), self._i64(slot), self._i32(kv_len),
                                seq=self._i32(seq), position=self._i64(position), q_start=self._i32(start),
@@ -196,8 +207,7 @@ class PagedBatch:
 
     def step(self, sampling: Sampling | None = None, u: torch.Tensor | None = None) -> torch.Tensor:
         """Feeds every sequence its ``token`` and picks the next one."""
-        for b, n in enumerate(self.lens):
-            self.kv.reserve(b, n + 1)
+        self.kv.reserve_all({b: n + 1 for b, n in enumerate(self.lens)})
         logits = self._forward(self.token, self._i64(self.lens), self._i32([n + 1 for n in self.lens]))
         self.lens = [n + 1 for n in self.lens]
         self._open = [[] for _ in range(self.batch)]

@@ -243,3 +243,50 @@ def test_accept_takes_a_chain_of_children_only():
     batch.step()                             # so does a step
     with pytest.raises(ValueError):
         batch.accept(0, [0], 1)
+
+
+@pytest.mark.gpu
+def test_a_refused_append_or_step_takes_nothing():
+    from gpu.decodev2 import MEDIUM_LLAMA, PagedBatch
+
+    batch = PagedBatch(_weights(MEDIUM_LLAMA), 2, 3, page=16, max_seq=40)
+    batch.append([list(range(1, 17)), [2]])
+    state = lambda: (list(batch.lens), [list(o) for o in batch.kv.owned], batch.kv.free_pages,  # noqa: E731
+                     batch.kv.table.tolist())
+    before = state()
+    refused = [(RuntimeError, "out of cache pages", dict(rows=[[1], [1] * 16])),
+               (ValueError, "max_seq", dict(rows=[[1], [1] * 40])),
+               (ValueError, "draft", dict(rows=[[1], [1]], trees=[[-1], [0]])),
+               (ValueError, "token", dict(rows=[[1], [MEDIUM_LLAMA.vocab]])),
+               (ValueError, "token", dict(rows=[[-1], [1]])),
+               (ValueError, "one parent", dict(rows=[[1], [1]], trees=[[-1]]))]
+    for kind, what, kw in refused:
+        with pytest.raises(kind, match=what):
+            batch.append(**kw)
+        assert state() == before
+    batch.append([[], [3] * 15])
+    before = state()
+    with pytest.raises(RuntimeError, match="out of cache pages"):  # both need a page, one is left
+        batch.step()
+    assert state() == before
+
+
+def test_pages_for_several_sequences_or_for_none():
+    from gpu.decodev2 import MEDIUM_LLAMA, PagedKV
+
+    kv = PagedKV(MEDIUM_LLAMA, 3, 5, page=16, max_seq=64, device="cpu")
+    kv.reserve_all({0: 16, 2: 20})
+    state = lambda: ([list(o) for o in kv.owned], kv.free_pages, kv.table.tolist())  # noqa: E731
+    before = state()
+    assert [len(o) for o in before[0]] == [1, 0, 2] and before[1] == 2
+    for kind, what, rows in ((RuntimeError, "out of cache pages", {0: 17, 1: 1, 2: 33}),
+                             (ValueError, "max_seq", {0: 17, 1: 65}), (ValueError, "max_seq", {1: 65, 0: 17})):
+        with pytest.raises(kind, match=what):
+            kv.reserve_all(rows)
+        assert state() == before
+    kv.reserve_all({0: 17, 1: 16, 2: 32})
+    assert [len(o) for o in kv.owned] == [2, 1, 2] and kv.free_pages == 0
+    assert sorted(sum(kv.owned, [])) == [0, 1, 2, 3, 4]
+    for b in range(3):
+        n = len(kv.owned[b])
+        assert kv.table[b, :n].tolist() == kv.owned[b] and (kv.table[b, n:] == -1).all()
