@@ -290,3 +290,48 @@ def test_pages_for_several_sequences_or_for_none():
     for b in range(3):
         n = len(kv.owned[b])
         assert kv.table[b, :n].tolist() == kv.owned[b] and (kv.table[b, n:] == -1).all()
+
+
+@pytest.mark.parametrize("rot,theta,factor,original", [(128, 1e6, 4.0, 32768), (64, 1e4, 8.0, 4096)])
+def test_yarn_ramp_over_pairs(rot, theta, factor, original):
+    """The blend of released checkpoints, its borders found by bisection over the turns of a pair."""
+    from gpu.decodev2 import rope_tables_scaled
+
+    def index_of(turns):
+        lo, hi = 0.0, float(rot)
+        for _ in range(200):
+            mid = (lo + hi) / 2
+            lo, hi = (mid, hi) if original * theta ** (-2 * mid / rot) / (2 * math.pi) > turns else (lo, mid)
+        return lo
+
+    first, last = math.floor(index_of(32)), math.ceil(index_of(1))
+    if rot == 128:
+        assert (first, last) == (23, 40)
+    args = dict(scaling="yarn", factor=factor, original=original, device="cpu", dtype=torch.float64)
+    cos, sin = rope_tables_scaled(64, rot, theta, ramp="pairs", **args)
+    gain = 1 + 0.1 * math.log(factor)
+    for i in range(rot // 2):
+        share = min(max((i - first) / (last - first), 0.0), 1.0)     # of the divided angle
+        inv = theta ** (-2 * i / rot) * (1 - share + share / factor)
+        for p in (0, 1, 63):
+            assert abs(float(cos[p, i]) - gain * math.cos(p * inv)) <= 1e-12
+            assert abs(float(sin[p, i]) - gain * math.sin(p * inv)) <= 1e-12
+    assert not torch.equal(cos, rope_tables_scaled(64, rot, theta, ramp="turns", **args)[0])
+    assert torch.equal(rope_tables_scaled(64, rot, theta, **args)[0], rope_tables_scaled(64, rot, theta, ramp="turns", **args)[0])
+
+
+def test_yarn_ramps_at_their_ends():
+    from gpu.decodev2 import rope_tables_scaled
+
+    args = dict(scaling="yarn", factor=4.0, device="cpu", dtype=torch.float64)
+    # every pair turns often: none is slowed; every pair turns less than once: all are but the first,
+    # at which both borders, drawn to the pairs there are, then lie
+    for original, slowed in ((10**9, [1.0] * 8), (4, [1.0] + [4.0] * 7)):
+        cos, sin = rope_tables_scaled(9, 16, 100.0, original=original, ramp="pairs", **args)
+        for i in range(8):
+            inv = 100.0 ** (-2 * i / 16) / slowed[i]
+            assert abs(float(sin[8, i]) - (1 + 0.1 * math.log(4.0)) * math.sin(8 * inv)) <= 1e-12
+    with pytest.raises(ValueError, match="ramp"):
+        rope_tables_scaled(8, 64, 1e4, original=1024, ramp="other", **args)
+    with pytest.raises(ValueError, match="ramp"):
+        rope_tables_scaled(8, 64, 1.0, original=1024, ramp="pairs", **args)
