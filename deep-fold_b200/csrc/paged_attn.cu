@@ -906,6 +906,10 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Pag
   }
 }
 
+// A lane looks up to 32 tiles of 64 (one of 128) rows past an item's end: cache rows, and places
+// that far behind them, are numbered in 32 bits.
+constexpr long long kMaxRows = 0x7fffffffll - 8192;
+
 // Limit of a wait, process-wide.
 uint32_t &attn_paged_polls() {
   static uint32_t v = kPolls;
@@ -1058,7 +1062,9 @@ extern "C" int chr_nf4_attn_paged(const chr_nf4_attn_paged_t *args, void *stream
     return kAlign;
   }
   const int n_rep = r.n_q / a.c.n_kv;
-  a.p.cap = static_cast<int>(static_cast<long long>(a.c.max_pages) << a.c.page_shift);
+  const long long cap = static_cast<long long>(a.c.max_pages) << a.c.page_shift;
+  if (cap > kMaxRows) return kDims;
+  a.p.cap = static_cast<int>(cap);
   const AttnForm f = form_of(r.T, a.c.batch, n_rep, hd);
   if (r.ws_floats < ws_floats_of(f.ctas, f.M, hd)) return kWorkspace;
   a.p.q_start = static_cast<const int32_t *>(r.q_start);

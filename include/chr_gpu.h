@@ -441,10 +441,11 @@ int chr_nf4_rope_kv_paged(const chr_nf4_rope_kv_paged_t *args, void *stream);
 /* Attention of T new rows over the paged cache. Sequence b owns rows q_start[b] ..
  * q_start[b+1]-1 of q (device int32 [batch + 1], not decreasing, within 0..T; NULL: T ==
  * batch, row b is sequence b's) and kv_len[b] cache rows (device int32, taken within 0 ..
- * max_pages * page), its n_b new rows the last n_b of them. New row i sees cache row t < base = kv_len[b] - n_b, and of the new
- * rows those with t - base <= i, or, with tree given, those whose bit t - base is set in
- * the tree_words 64-bit words of the row's mask (device uint64 [T, tree_words]; a bit past
- * the words is clear). GQA: n_q a multiple of n_kv, hd in {16, 32, 64, 128}.
+ * max_pages * page, which must not exceed 2^31 - 8193), its n_b new rows the last n_b of
+ * them. New row i sees cache row t < base = kv_len[b] - n_b, and of the new rows those with
+ * t - base <= i, or, with tree given, those whose bit t - base is set in the tree_words
+ * 64-bit words of the row's mask (device uint64 [T, tree_words]; a bit past the words is
+ * clear). GQA: n_q a multiple of n_kv, hd in {16, 32, 64, 128}.
  *   out[i, h, :] = softmax_t( scale * q[i, h, :] . k[t, h / n_rep] ) . v[t, h / n_rep]
  * q: bf16, rows q_stride elements apart (a multiple of 8), rotated already; out: bf16
  * [T, n_q * hd] contiguous. A row that sees nothing gives zeros; rows that no sequence

@@ -335,3 +335,21 @@ def test_yarn_ramps_at_their_ends():
         rope_tables_scaled(8, 64, 1e4, original=1024, ramp="other", **args)
     with pytest.raises(ValueError, match="ramp"):
         rope_tables_scaled(8, 64, 1.0, original=1024, ramp="pairs", **args)
+
+
+def test_attention_refuses_caches_whose_rows_pass_32_bits():
+    """The C entry's checks need no GPU: places a few tiles behind the last cache row are still counted in
+    32 bits, so a table that reaches to 2^31 rows is refused."""
+    import ctypes
+
+    from gpu.nf4 import _lib
+
+    def call(max_pages, page):
+        pages = _lib.ChrNf4Pages(k=4096, v=4096, table=4096, k_page_stride=page * 128, v_page_stride=page * 128,
+                                 table_stride=max_pages, n_pages=8, page=page, n_kv=2, hd=64, batch=2, max_pages=max_pages)
+        args = _lib.ChrNf4AttnPaged(pages=pages, q=4096, q_stride=512, out=4096, q_start=4096, kv_len=4096, T=3, n_q=8,
+                                    scale=0.1, ws=4096, ws_floats=0)
+        return _lib.load().chr_nf4_attn_paged(ctypes.byref(args), None)
+
+    assert call((1 << 27) - 1, 16) == -3 and call((1 << 15) - 1, 65536) == -7
+    assert call((1 << 27) - 512, 16) == -3 and call((1 << 27) - 513, 16) == -7   # past the rows: the workspace's check
