@@ -405,9 +405,14 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     auto arrived = [&](bool live, int half) {
       if (live && ok) {
         ok = __all_sync(0xffffffffu, bar_poll(bar + slot, (phase >> slot) & 1u, a.polls));
-        if (!ok && lane == 0) {
-          atomicExch(&g_attn_paged_status, 20);
-          late[warp] = ThinLate{slot, ahead, phase, has_rows, n_used - 1, half};
+        if (!ok) {
+          ThinLate &l = late[warp];
+          l.slot = slot;
+          l.ahead = ahead;
+          l.phase = phase;
+          l.has_rows = has_rows;
+          l.block = n_used - 1;
+          l.half = half;
         }
         phase ^= 1u << slot;
       }
@@ -730,6 +735,7 @@ attn_paged_thin_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   }
   if (!ok) {
     // nothing leaves before the copies in flight have landed, each within the full limit
+    if (lane == 0) atomicExch(&g_attn_paged_status, 20);
     __syncwarp();
     const ThinLate l = late[warp];
     int half = l.half;
