@@ -933,6 +933,10 @@ AttnForm form_of(int T, int batch, int n_rep, int hd) {
   // items of 32; of 255 rows 102 and 455. From 17 to 32 rows it is a draw: 20 rows, 16 sequences of
   // 2100 to 6000 cache rows 67 wide and 75 thin, two such 31.6 and 28.4, 32 of 100 to 900
   // 42 and 37.
+  // The mean is of all sequences, so a call that mixes a long chunk with single tokens or with
+  // sequences without rows takes one form for both: a chunk of 256 rows (45 us alone) in a batch of 64 that
+  // has no other rows takes 70 in the thin form; one of 512 beside 63 tokens (46 and 54 alone) 109 in the
+  // wide one; one of 1024 beside 255 tokens (58 and 165 alone) 388 in the thin one.
   const long long rows = (static_cast<long long>(T) + batch - 1) / batch * n_rep;
   const int sms = std::min(sm_count(), kMaxCtas / 2);
   AttnForm f;

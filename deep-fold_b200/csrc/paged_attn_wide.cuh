@@ -14,9 +14,11 @@
 // products take 2 x (2 x 8 x 48 + 8 x 64) = 2560 clocks - the 128 x 64 one is held up by the
 // 128 bytes a clock its operands are read at, hence 48 - and the exps 2048 (32768 at 16 a clock).
 // (With one S buffer of 128 columns per tile, products 2048 clocks, the chain of both was 4100.)
-// Measured 2.0 us per 128 cache rows and 256 queries, at the 1.5 to 1.8 GHz that the power cap leaves;
+// Measured 2.0 us per 128 cache rows and 256 queries where these come from L2, at the 1.5 to 1.8 GHz
+// that the power cap leaves, 2.8 where they come from HBM (one warp looks the pages up and requests
+// K behind the wait for V's stage, so that little more than a stage of each is on the way);
 // a segment costs 5 us more for its start and its result. Three chunks of 2047 rows over
-// caches of up to 4096, 40 / 8 heads of 128 (349 GFLOP): 364 us replayed, 412 as calls among others.
+// caches of up to 4096, 40 / 8 heads of 128 (349 GFLOP): 360 to 405 us by the clock.
 // The running
 // maximum a row subtracts is raised only when the new one is more than 8
 // (in log2) above it: P then stays below 2^8, which bf16 holds as exactly as 1, and the

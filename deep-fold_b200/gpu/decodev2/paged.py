@@ -109,7 +109,10 @@ class PagedBatch:
     ``rope_tables_scaled`` (scaling for contexts longer than the weights were trained on).
 
     ``append``, ``step`` and ``pick`` leave their results on the device; ``check``, which ``generate``
-    calls, tells whether the attention that made them ran to its end."""
+    calls, tells whether the attention that made them ran to its end.
+
+    Rotated queries and probabilities are bf16 here, where the dense cache's decode keeps two bf16 terms of
+    each: logits differ by roundings, and tokens can where two are that close."""
 
     def __init__(self, weights: DeviceWeights, batch: int, n_pages: int, *, page: int = 64, max_seq: int | None = None,
                  rope: dict | None = None) -> None:

@@ -265,6 +265,11 @@ def nf4_attn_paged(
     One token per sequence is a decode step, a tree of drafted tokens is checked in one pass,
     and without ``tree`` many rows are a prompt chunk.
 
+    Probabilities are rounded to bf16 for the value product, as the prompt attention of the dense
+    cache does (its decode attention keeps them, and the query it rotates, in two bf16 terms). One form
+    is chosen for the whole call from the mean rows per sequence: a long chunk and many single
+    tokens go faster as two calls. A wait that runs out is reported by ``nf4_attn_paged_status``.
+
     A row that sees nothing gives zeros. Rows of ``q`` that no sequence owns (in front of
     ``q_start[0]``, from ``q_start[batch]`` on) are left alone in a given ``out`` (which must not
     overlap ``q``), zero in a new one. See ``chr_nf4_attn_paged``."""

@@ -451,13 +451,15 @@ int chr_nf4_rope_kv_paged(const chr_nf4_rope_kv_paged_t *args, void *stream);
  * [T, n_q * hd] contiguous. A row that sees nothing gives zeros; rows that no sequence
  * owns, in front of q_start[0] and from q_start[batch] on, are left alone (zero_tail = 0)
  * or zeroed. FP32 scores, running softmax and accumulation; probabilities are rounded to
- * bf16 for the value product. Cache rows at kv_len and beyond may hold anything;
- * infinities and NaN in a new row reach the rows that see it and no others. A cache row on
- * a page outside the pool is seen by none.
- * out must not overlap q. ws: chr_nf4_attn_paged_ws(...) floats, 16-byte aligned, no
- * initial contents needed; two calls that may overlap on the device need one each. Two
- * launches. Capturable: lengths, tables and masks are read on the device, and a replay
- * follows what they hold then.
+ * bf16 for the value product (q is bf16 as given; the dense decode entries keep the query
+ * they rotate, and the probabilities, in two bf16 terms). One form is chosen for the whole
+ * call from T / batch: a long chunk and many single tokens go faster as two calls.
+ * Cache rows at kv_len and beyond may hold anything; infinities and NaN in a new row reach
+ * the rows that see it and no others. A cache row on a page outside the pool is seen by
+ * none. out must overlap neither q nor the pools. ws: chr_nf4_attn_paged_ws(...) floats of
+ * the device the call runs on, 16-byte aligned, no initial contents needed; two calls that
+ * may overlap on the device need one each. Two launches. Capturable: lengths, tables and
+ * masks are read on the device, and a replay follows what they hold then.
  * Returns 0, -1 (null), -3 (dims), -5 (alignment: q, out, ws, pools 16 bytes), -6, -7. */
 int64_t chr_nf4_attn_paged_ws(int32_t T, int32_t batch, int32_t n_q, int32_t n_kv, int32_t hd);
 typedef struct {
@@ -474,9 +476,9 @@ typedef struct {
 } chr_nf4_attn_paged_t;
 int chr_nf4_attn_paged(const chr_nf4_attn_paged_t *args, void *stream);
 
-/* Reads and clears the paged attention's device status word (synchronises the device): 0 =
- * every bounded wait of its tensor-core form completed; else the number of the wait that
- * gave up, and the affected launch's output is undefined. */
+/* Reads and clears the paged attention's status word of the current device (synchronises
+ * it): 0 = every bounded wait for a copy or a product completed; else the number of the wait
+ * that gave up, and the affected launch's output is undefined. */
 int chr_nf4_attn_paged_status(void);
 
 /* Poll limit of those waits (process-wide, taken at launch; negative restores 2^18). With a
